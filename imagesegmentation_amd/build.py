@@ -8,10 +8,12 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 OUT = os.path.join(_HERE, "libisg.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-shared", "-Wall", "-Wno-unused-function"]
-# Per-file extras.  The fused backward is built without the SLP vectoriser: it packs the gate arithmetic into
-# v_pk_*_f32 instructions, which issue slower than the two scalar instructions they replace on this chip and cost
-# ~30 vector registers (measured: -2 % on the 16-channel kernel, nothing lost on the others).
+# (no packed float instructions: some forms of v_pk_*_f32, which -O3 makes of ordinary float code by itself, have given
+# wrong results on this chip now and then; hipcc's host pass does not know the feature and says so, harmlessly)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-shared", "-Wall", "-Wno-unused-function"] + NO_PACKED_F32
+# Per-file extras.  The fused backward is built without the SLP vectoriser: with it the gate arithmetic is laid out in
+# register pairs, which costs ~30 vector registers (measured: -2 % on the 16-channel kernel, nothing lost on the others).
 EXTRA_FLAGS = {"isg_convlstm_bwd.hip": ["-fno-slp-vectorize"]}
 
 
