@@ -72,6 +72,12 @@ SIGNATURES = {
     "isg_copy_channel_slice": (_int, [_vp, _vp, _vp, _vp, _int, _ll, _ll, _ll, _vp]),
     "isg_a3c_loss_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _vp, _vp]),
     "isg_a3c_loss_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _vp, _vp]),
+    "isg_token_logprobs_fwd": (_int, [_vp, _ll, _vp, _int, _vp, _int, _int, _int, _f32, _int, _vp, _vp, _vp, _vp, _vp,
+                                      _vp]),
+    "isg_token_logprobs_bwd": (_int, [_vp, _ll, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _f32, _int,
+                                      _vp, _vp]),
+    "isg_distill_fwd": (_int, [_vp, _ll, _vp, _vp, _int, _vp, _int, _int, _int, _int, _f32, _int, _vp, _vp, _vp]),
+    "isg_distill_bwd": (_int, [_vp, _ll, _vp, _vp, _int, _vp, _vp, _int, _int, _int, _int, _f32, _int, _vp, _vp]),
     "isg_rollout_record": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _vp, _vp]),
     "isg_gae": (_int, [_vp, _vp, _vp, _vp, _int, _int, _f64, _f64, _vp, _vp, _vp]),
     "isg_column_sums_workspace_bytes": (_ll, [_int]),

@@ -1,9 +1,13 @@
-"""Softmax cross-entropy, argmax and sampling over the vertex class grid, on the libisg kernels
-(isg_softmax_xent_fwd / _bwd, isg_argmax_rows, isg_sample_rows)."""
+"""Softmax cross-entropy, argmax, sampling, log-probabilities and distillation over the vertex class grid, on the libisg
+kernels (isg_softmax_xent_fwd / _bwd, isg_argmax_rows, isg_sample_rows, isg_token_logprobs_*, isg_distill_*)."""
+import contextlib
+import typing
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ..ops import dtype_code
+from ..ops import dtype_code, pixel_stride
 
 
 def _rows(logits):
@@ -158,6 +162,237 @@ def sample_actions(logits, seed, grid_side, row_offset=0, row_offset_dev=None, o
                                        _lib.ptr(row_offset_dev), int(grid_side), _lib.ptr(out), _lib.current_stream())
     _lib.check(rc, "isg_sample_actions")
     return out
+
+
+# ---- log-probabilities, entropy, alternatives ------------------------------------------------------------------------
+TOP_MAX = 64             # ISG_TOP_MAX
+DISTILL_MAX = 1024       # ISG_DISTILL_MAX
+CLASSES_MAX = 1 << 20    # ISG_CLASSES_MAX
+
+
+class TokenLogprobs(typing.NamedTuple):
+    """What ``token_logprobs`` returns; ``logprobs`` is None without tokens, the ``top_*`` are None with top = 0."""
+    logprobs: typing.Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logprobs: typing.Optional[torch.Tensor]
+    top_classes: typing.Optional[torch.Tensor]
+
+
+def _class_rows(logits, what):
+    """(logits, rows, classes, elements from row to row) as the kernels read them: float32 or bfloat16, a row's classes
+    adjacent, rows evenly spaced - in place where the tensor is that (a column slice of padded logits, every other step of a batch), a
+    copy otherwise."""
+    if not torch.is_tensor(logits) or logits.dim() < 1 or not logits.is_floating_point():
+        raise TypeError("%s: logits must be a floating-point tensor of at least one axis" % what)
+    cols = logits.shape[-1]
+    if not 1 <= cols <= CLASSES_MAX:
+        raise ValueError("%s: %d classes (1 to %d)" % (what, cols, CLASSES_MAX))
+    if not logits.is_cuda:
+        raise RuntimeError("%s: logits must live on the GPU: libisg has no CPU path" % what)
+    z = logits if logits.dtype in (torch.float32, torch.bfloat16) else logits.float()
+    rows = z.numel() // cols
+    if z.is_contiguous():
+        return z, rows, cols, cols
+    stride = pixel_stride(z) if z.dim() > 1 else None
+    if stride is None or stride < cols:
+        return z.contiguous(), rows, cols, cols
+    return z, rows, cols, stride
+
+
+def _row_argument(t, shape, kinds, device, what):
+    """A per-row tensor of one of the ``kinds`` in the rows' shape, contiguous."""
+    if not torch.is_tensor(t) or t.dtype not in kinds:
+        raise TypeError("%s must be a tensor of %s" % (what, " or ".join(str(k).replace("torch.", "") for k in kinds)))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have the shape %s, not %s" % (what, tuple(shape), tuple(t.shape)))
+    if t.device != device:
+        raise ValueError("%s lives on %s, the logits on %s" % (what, t.device, device))
+    return t.contiguous()
+
+
+def _temperature(value, what):
+    value = float(value)
+    if not 1e-30 <= value <= 1e30:
+        raise ValueError("%s: temperature %g (positive and finite)" % (what, value))
+    return value
+
+
+def _on_device(t):
+    """The kernels launch on the current device's stream: for a tensor of another device that one is made current."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
+    rows, cols, stride = geometry
+    new = lambda shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=z.device)
+    logp = new([rows]) if tokens is not None else None
+    entropy = new([rows])
+    top_logp, top_cls = (new([rows, top]), new([rows, top], torch.int32)) if top else (None, None)
+    stats = new([rows, 4]) if keep else None
+    with _on_device(z):
+        rc = _lib.lib().isg_token_logprobs_fwd(
+            z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4, _lib.ptr(live),
+            rows, cols, dtype_code(z.dtype), temperature, top, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp),
+            _lib.ptr(top_cls), _lib.ptr(stats), _lib.current_stream())
+    _lib.check(rc, "isg_token_logprobs_fwd")
+    return logp, entropy, top_logp, top_cls, stats
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, live, top, temperature):
+        z, rows, cols, stride = _class_rows(logits, "token_logprobs")
+        logp, entropy, top_logp, top_cls, stats = _logprobs_forward(z, (rows, cols, stride), tokens, live, top,
+                                                                    temperature, True)
+        ctx.save_for_backward(z, tokens, live, top_cls, stats)
+        ctx.call = (rows, cols, stride, top, temperature)
+        ctx.shape, ctx.in_dtype = logits.shape, logits.dtype
+        if top_cls is not None:
+            ctx.mark_non_differentiable(top_cls)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_cls
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp, dentropy, dtop, _):
+        if dlogp is None and dentropy is None and dtop is None:
+            return None, None, None, None, None
+        z, tokens, live, top_cls, stats = ctx.saved_tensors
+        rows, cols, stride, top, temperature = ctx.call
+        f32 = lambda t: None if t is None else t.to(torch.float32).contiguous()
+        dlogp, dentropy, dtop = f32(dlogp), f32(dentropy), f32(dtop)
+        dz = torch.empty([rows, cols], dtype=z.dtype, device=z.device)
+        with _on_device(z):
+            rc = _lib.lib().isg_token_logprobs_bwd(
+                z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4,
+                _lib.ptr(live), _lib.ptr(top_cls), _lib.ptr(stats), _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(dtop),
+                rows, cols, dtype_code(z.dtype), temperature, top, _lib.ptr(dz), _lib.current_stream())
+        _lib.check(rc, "isg_token_logprobs_bwd")
+        return dz.reshape(ctx.shape).to(ctx.in_dtype), None, None, None, None
+
+
+def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
+    """Log-probabilities of given classes, entropies and the most probable classes of softmax(logits / temperature),
+    from one pass over the logits (isg_token_logprobs_fwd); differentiable in the logits through everything but the
+    classes (isg_token_logprobs_bwd; first derivatives only).
+
+    logits [..., K] (float32 and bfloat16 as they are, also with rows evenly apart; others through float32),
+    tokens int32 or int64 [...] or None, top = how many of the largest logits to report (0 to 64, at most K; equal
+    logits lowest class first), live bool or uint8 [...] or None: rows without it are not read and give zeros (class
+    -1) and no gradient - steps past a sequence's duration.  Logits of -inf are classes without probability.
+
+    Returns ``TokenLogprobs``: logprobs float32 [...] (NaN for a class outside [0, K)), entropy float32 [...],
+    top_logprobs float32 [..., top], top_classes int32 [..., top]."""
+    if not torch.is_tensor(logits) or logits.dim() < 1:
+        raise TypeError("token_logprobs: logits must be a floating-point tensor of at least one axis")
+    lead = logits.shape[:-1]
+    top = int(top)
+    if not 0 <= top <= min(TOP_MAX, logits.shape[-1]):
+        raise ValueError("token_logprobs: top %d of %d classes (0 to %d)" % (top, logits.shape[-1], TOP_MAX))
+    temperature = _temperature(temperature, "token_logprobs")
+    if tokens is not None:
+        tokens = _row_argument(tokens, lead, (torch.int32, torch.int64), logits.device, "token_logprobs: tokens")
+    if live is not None:
+        live = _row_argument(live, lead, (torch.bool, torch.uint8), logits.device, "token_logprobs: live")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        logp, entropy, top_logp, top_cls = _TokenLogprobs.apply(logits, tokens, live, top, temperature)
+    else:
+        z, rows, cols, stride = _class_rows(logits.detach(), "token_logprobs")
+        logp, entropy, top_logp, top_cls, _ = _logprobs_forward(z, (rows, cols, stride), tokens, live, top, temperature,
+                                                                False)
+    if len(lead) != 1:
+        logp = logp.reshape(lead) if logp is not None else None
+        entropy = entropy.reshape(lead)
+        if top:
+            top_logp, top_cls = top_logp.reshape(lead + (top,)), top_cls.reshape(lead + (top,))
+    return TokenLogprobs(logp, entropy, top_logp, top_cls)
+
+
+# ---- distillation -----------------------------------------------------------------------------------------------------
+def _distill_forward(z, geometry, values, classes, live, temperature, tail, keep):
+    rows, cols, stride = geometry
+    loss = torch.empty([rows], dtype=torch.float32, device=z.device)
+    stats = torch.empty([rows, 8], dtype=torch.float32, device=z.device) if keep else None
+    with _on_device(z):
+        rc = _lib.lib().isg_distill_fwd(z.data_ptr(), stride, _lib.ptr(values), _lib.ptr(classes), classes.element_size(),
+                                        _lib.ptr(live), rows, cols, values.shape[-1], dtype_code(z.dtype), temperature,
+                                        tail, _lib.ptr(loss), _lib.ptr(stats), _lib.current_stream())
+    _lib.check(rc, "isg_distill_fwd")
+    return loss, stats
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, classes, live, temperature, tail):
+        z, rows, cols, stride = _class_rows(logits, "distill_rows")
+        loss, stats = _distill_forward(z, (rows, cols, stride), values, classes, live, temperature, tail, True)
+        ctx.save_for_backward(z, values, classes, stats)
+        ctx.call = (rows, cols, stride, temperature, tail)
+        ctx.shape, ctx.in_dtype = logits.shape, logits.dtype
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        z, values, classes, stats = ctx.saved_tensors
+        rows, cols, stride, temperature, tail = ctx.call
+        g = dloss.to(torch.float32).contiguous()
+        dz = torch.empty([rows, cols], dtype=z.dtype, device=z.device)
+        with _on_device(z):
+            rc = _lib.lib().isg_distill_bwd(z.data_ptr(), stride, _lib.ptr(values), _lib.ptr(classes),
+                                            classes.element_size(), _lib.ptr(stats), _lib.ptr(g), rows, cols,
+                                            values.shape[-1], dtype_code(z.dtype), temperature, tail, _lib.ptr(dz),
+                                            _lib.current_stream())
+        _lib.check(rc, "isg_distill_bwd")
+        return dz.reshape(ctx.shape).to(ctx.in_dtype), None, None, None, None, None
+
+
+def distill_rows(logits, teacher_values, teacher_classes, temperature=1.0, tail=False, live=None):
+    """Per-row divergence of softmax(logits / temperature) from a teacher's k most probable classes (isg_distill_fwd /
+    isg_distill_bwd), float32 [...], differentiable in the logits (first derivatives only): sum_j q_j (log q_j -
+    log p_j).  The teacher takes no gradient.
+
+    logits [..., K] as ``token_logprobs`` takes them; teacher_values float [..., k] and teacher_classes int32 or int64
+    [..., k], k from 1 to 1024: what ``token_logprobs(teacher_logits, top=k, temperature=temperature)`` returns.  A
+    negative class is no entry; a class outside the row makes the row NaN.
+
+    tail=False: q = softmax(teacher_values / temperature) over the entries (the teacher's logits); tail=True: the values
+    are log-probabilities at this temperature and the mass they leave is one more class, set against the student's mass
+    outside the entries (where no class is left outside, up to 1e-5 of remaining mass counts as rounding, more gives an
+    infinite loss).  live: as in ``token_logprobs``.  (A loss that mixes temperatures multiplies by temperature^2
+    to keep the gradients' size; that factor is the caller's.)"""
+    if not torch.is_tensor(logits) or logits.dim() < 1:
+        raise TypeError("distill_rows: logits must be a floating-point tensor of at least one axis")
+    lead = logits.shape[:-1]
+    temperature = _temperature(temperature, "distill_rows")
+    if not torch.is_tensor(teacher_values) or not teacher_values.is_floating_point():
+        raise TypeError("distill_rows: teacher_values must be a floating-point tensor")
+    k = teacher_values.shape[-1] if teacher_values.dim() else 0
+    if not 1 <= k <= DISTILL_MAX:
+        raise ValueError("distill_rows: %d classes of the teacher (1 to %d)" % (k, DISTILL_MAX))
+    values = teacher_values.detach()
+    values = _row_argument(values if values.dtype == torch.float32 else values.float(), lead + (k,), (torch.float32,),
+                           logits.device, "distill_rows: teacher_values")
+    classes = _row_argument(teacher_classes, lead + (k,), (torch.int32, torch.int64), logits.device,
+                            "distill_rows: teacher_classes")
+    if live is not None:
+        live = _row_argument(live, lead, (torch.bool, torch.uint8), logits.device, "distill_rows: live")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        loss = _Distill.apply(logits, values, classes, live, temperature, int(bool(tail)))
+    else:
+        z, rows, cols, stride = _class_rows(logits.detach(), "distill_rows")
+        loss, _ = _distill_forward(z, (rows, cols, stride), values, classes, live, temperature, int(bool(tail)), False)
+    return loss if len(lead) == 1 else loss.reshape(lead)
+
+
+def distill_mean(logits, teacher_values, teacher_classes, temperature=1.0, tail=False, live=None):
+    """``distill_rows`` averaged over the live rows (over every row without ``live``); 0 when none is live."""
+    loss = distill_rows(logits, teacher_values, teacher_classes, temperature, tail, live)
+    if live is None:
+        return loss.mean()
+    return loss.sum() / live.sum().clamp(min=1)
 
 
 def decode_begin(true_vertices, num_true, hist, steps):

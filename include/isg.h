@@ -371,6 +371,54 @@ int isg_a3c_loss_bwd(const void* logits, const float* vf, const int32_t* actions
                      const unsigned char* live, const float* stats, const float* upstream3, int rows, int cols, int dtype,
                      void* dlogits, float* dvf, void* stream);
 
+/* Log-probabilities of given classes, with the row's entropy and its most probable classes: what a policy's update
+ * needs of the actions taken (reference polyrl/a3c/a3c.py:201-207 for log-probability and entropy), what scoring a
+ * decoded polygon needs of its vertices, and what a teacher hands to isg_distill_fwd.  With p = softmax(z / temperature)
+ * over a row z of logits:
+ *   logprobs[r] = log p[tokens[r]] (NaN for a class the row does not have; tokens NULL: not computed, logprobs unused)
+ *   entropy[r]  = -sum_c p_c log p_c
+ *   top_classes / top_logprobs [r][top]: the classes of the `top` largest logits in falling order, equal logits by
+ *     class (lowest first, NaN last), and their log-probabilities
+ *   stats float [r][4] (may be NULL): what isg_token_logprobs_bwd reads.
+ * A logit of -inf is a class without probability; a row of nothing else has log-probability -inf everywhere, entropy 0
+ * and a zero gradient.  live uint8 [rows] (may be NULL): rows with 0 are not read, their outputs are 0 (classes -1)
+ * and their gradient is 0.  logits `dtype` with rows row_stride >= cols elements apart; tokens are int32 or int64
+ * (token_bytes 4 or 8).  0 <= top <= ISG_TOP_MAX, cols <= ISG_CLASSES_MAX, temperature in [1e-30, 1e30].
+ * isg_token_logprobs_bwd: dlogits `dtype` [rows][cols] (dense, not the logits themselves) from the gradients of the
+ * three outputs (float; each may be NULL: no gradient arrives there).  No atomics: the same call gives the same bits. */
+#define ISG_TOP_MAX 64
+#define ISG_CLASSES_MAX (1 << 20)
+int isg_token_logprobs_fwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
+                           const unsigned char* live, int rows, int cols, int dtype, float temperature, int top,
+                           float* logprobs, float* entropy, float* top_logprobs, int32_t* top_classes, float* stats,
+                           void* stream);
+int isg_token_logprobs_bwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
+                           const unsigned char* live, const int32_t* top_classes, const float* stats,
+                           const float* dlogprobs, const float* dentropy, const float* dtop_logprobs, int rows, int cols,
+                           int dtype, float temperature, int top, void* dlogits, void* stream);
+
+/* Distillation from a teacher's k most probable classes (no counterpart in the reference, whose nets train on labels
+ * only, polyrnn/Model.py:98-100): the divergence of p = softmax(z / temperature) from the teacher's q,
+ *   loss[r] = sum_j q_j (log q_j - log p[classes[r][j]])     (+ q_rest (log q_rest - log p_rest) with tail)
+ *   tail = 0: q = softmax(values[r] / temperature) over the k entries (logits or log-probabilities);
+ *   tail = 1: values are log-probabilities at this temperature, q_j = exp(values[r][j]); what is left of the teacher's
+ *             mass, q_rest = max(0, 1 - sum_j q_j), is one more class, p_rest the student's mass outside the entries;
+ *             where no class outside has any, a q_rest up to 1e-5 (rounding of the values) counts as none and a larger one
+ *             makes the loss +inf.
+ * values float [rows][k]; classes int32 or int64 (class_bytes) [rows][k]: a negative class is no entry (fewer than k
+ * alternatives), one the row does not have (>= cols) makes loss and gradient of the row NaN, a class given twice takes
+ * both masses.  A row without entries has loss 0 and no gradient.  live, row_stride, temperature: as above; k <=
+ * ISG_DISTILL_MAX.  stats float [rows][8] (may be NULL without a backward pass).
+ * isg_distill_bwd: dlogits `dtype` [rows][cols] (dense, not the logits themselves) from dloss float [rows]; the values
+ * take no gradient. */
+#define ISG_DISTILL_MAX 1024
+int isg_distill_fwd(const void* logits, long long row_stride, const float* values, const void* classes, int class_bytes,
+                    const unsigned char* live, int rows, int cols, int k, int dtype, float temperature, int tail,
+                    float* loss, float* stats, void* stream);
+int isg_distill_bwd(const void* logits, long long row_stride, const float* values, const void* classes, int class_bytes,
+                    const float* stats, const float* dloss, int rows, int cols, int k, int dtype, float temperature,
+                    int tail, void* dlogits, void* stream);
+
 /* out[c] = sum over rows of x[r][c] (float, overwritten; a fixed order of additions): the bias gradient of the dense
  * head, tf.gradients of the bias add in reference polyrnn/History2LargeExperiment.py:48-50, whose rows are every
  * (sample, step) of a batch - tens of thousands in a policy update.  x `dtype` [rows][cols];

@@ -1,0 +1,137 @@
+"""Log-probability and distillation operators without a GPU: the float64 references' gradients against central
+differences, and every refusal of the C entry points and of the Python calls."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import helpers_logprobs as ref
+from imagesegmentation_amd import _lib
+from imagesegmentation_amd.polyrnn import decode
+
+
+def _differences(f, z, h=1e-5):
+    g = np.zeros_like(z)
+    for i in np.ndindex(*z.shape):
+        hi, lo = z.copy(), z.copy()
+        hi[i] += h
+        lo[i] -= h
+        g[i] = (f(hi) - f(lo)) / (2 * h)
+    return g
+
+
+def test_reference_logprob_gradient_against_differences():
+    rs = np.random.RandomState(0)
+    z, T = rs.randn(3, 9) * 2, 1.7
+    tokens = np.array([2, 8, 0])
+    gl, gh, gt = rs.randn(3), rs.randn(3), rs.randn(3, 4)
+    order = ref.token_logprobs(z, T, tokens, 4)["top_classes"]
+
+    def f(y):
+        logp, p, _ = ref.softmax(y, T)
+        return (gl * logp[np.arange(3), tokens] + gh * ref.entropy(logp, p) +
+                (gt * np.take_along_axis(logp, order, axis=1)).sum(axis=1)).sum()
+    dz, _ = ref.token_logprobs_grad(z, T, tokens, order, gl, gh, gt, "f32")
+    # central differences at h = 1e-5: third derivatives of order 10 give 1e-9, cancellation 1e-15 / 1e-5 = 1e-10
+    assert np.abs(dz - _differences(f, z)).max() < 1e-8
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_reference_distillation_gradient_against_differences(tail):
+    rs = np.random.RandomState(1)
+    z, T = rs.randn(4, 9) * 2, 1.3
+    classes = np.array([[0, 3, 7], [8, 8, 2], [5, -1, 1], [-1, -1, -1]])  # a class twice, absent entries, no entry
+    values = np.log(rs.dirichlet(np.ones(5), size=4)[:, :3])
+    g = rs.randn(4)
+    f = lambda y: (g * ref.distill(y, values, classes, T, tail)["loss"]).sum()
+    dz = ref.distill(z, values, classes, T, tail, g)["dlogits"]
+    assert np.abs(dz - _differences(f, z)).max() < 1e-8
+    assert np.all(dz[3] == 0) or tail
+
+
+ONE, TWO = ctypes.c_void_p(4096), ctypes.c_void_p(8192)  # never read: every call below fails its checks first
+
+
+def _fwd(logits=ONE, stride=100, tokens=ONE, tb=4, rows=2, cols=100, dtype=1, T=1.0, top=0, out=ONE, ent=ONE, tl=ONE,
+         tc=ONE):
+    return _lib.lib().isg_token_logprobs_fwd(logits, stride, tokens, tb, None, rows, cols, dtype, T, top, out, ent, tl, tc,
+                                             None, None)
+
+
+def _bwd(logits=ONE, stride=100, tokens=ONE, tb=4, tc=ONE, stats=ONE, gl=ONE, gt=None, rows=2, cols=100, dtype=1, T=1.0,
+         top=0, out=TWO):
+    return _lib.lib().isg_token_logprobs_bwd(logits, stride, tokens, tb, None, tc, stats, gl, None, gt, rows, cols, dtype, T,
+                                             top, out, None)
+
+
+def _dfwd(logits=ONE, stride=100, values=ONE, classes=ONE, cb=4, rows=2, cols=100, k=4, dtype=1, T=1.0, tail=0, loss=ONE):
+    return _lib.lib().isg_distill_fwd(logits, stride, values, classes, cb, None, rows, cols, k, dtype, T, tail, loss, None,
+                                      None)
+
+
+def _dbwd(logits=ONE, stride=100, values=ONE, classes=ONE, cb=4, stats=ONE, g=ONE, rows=2, cols=100, k=4, dtype=1, T=1.0,
+          tail=0, out=TWO):
+    return _lib.lib().isg_distill_bwd(logits, stride, values, classes, cb, stats, g, rows, cols, k, dtype, T, tail, out, None)
+
+
+@pytest.mark.parametrize("call", [_fwd, _bwd, _dfwd, _dbwd])
+def test_entry_points_refuse_bad_shapes_types_and_temperatures(call):
+    err = lambda: _lib.lib().isg_last_error()
+    assert call(rows=-1) == -1 and call(cols=0) == -1
+    assert call(cols=(1 << 20) + 1, stride=1 << 21) == -1 and b"classes" in err()
+    assert call(stride=99) == -1 and b"apart" in err()
+    assert call(dtype=2) == -2 and b"dtype" in err()
+    for T in (0.0, -1.0, float("nan"), float("inf"), 1e-31):
+        assert call(T=T) == -1 and b"temperature" in err()
+    assert call(logits=None) == -1 and b"null" in err()
+    assert call(rows=0, logits=None) == 0  # nothing to do
+
+
+def test_entry_points_refuse_what_is_their_own():
+    err = lambda: _lib.lib().isg_last_error()
+    assert _fwd(top=65) == -1 and _fwd(top=-1) == -1 and _fwd(cols=8, top=9) == -1 and b"top" in err()
+    assert _fwd(tb=2) == -1 and b"bytes" in err()
+    assert _fwd(out=None) == -1 and _fwd(ent=None) == -1 and _fwd(top=3, tl=None) == -1 and _fwd(top=3, tc=None) == -1
+    assert _bwd(top=65) == -1 and _bwd(tokens=None) == -1 and _bwd(stats=None) == -1
+    assert _bwd(gt=ONE) == -1 and _bwd(gt=ONE, top=3, tc=None) == -1  # gradients of alternatives there are none of
+    assert _bwd(out=ONE) == -1 and b"alias" in err()
+    assert _dfwd(k=0) == -1 and _dfwd(k=1025) == -1 and _dfwd(tail=2) == -1 and _dfwd(cb=1) == -1
+    assert _dfwd(values=None) == -1 and _dfwd(classes=None) == -1 and _dfwd(loss=None) == -1
+    assert _dbwd(k=0) == -1 and _dbwd(stats=None) == -1 and _dbwd(g=None) == -1 and _dbwd(out=None) == -1
+    assert _dbwd(out=ONE) == -1 and b"alias" in err()
+
+
+def test_python_calls_refuse_what_they_cannot_take():
+    z = torch.zeros([4, 10])
+    tok = torch.zeros([4], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        decode.token_logprobs(z, tok)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        decode.distill_rows(z, z[:, :3].contiguous(), torch.zeros([4, 3], dtype=torch.int32))
+    for bad in (dict(top=-1), dict(top=11), dict(temperature=0.0), dict(temperature=float("nan"))):
+        with pytest.raises(ValueError):
+            decode.token_logprobs(z, tok, **bad)
+    with pytest.raises(ValueError, match="0 to 64"):
+        decode.token_logprobs(torch.zeros([4, 100]), tok, top=65)
+    with pytest.raises(TypeError):
+        decode.token_logprobs(z, tok.float())
+    with pytest.raises(ValueError, match="shape"):
+        decode.token_logprobs(z, tok[:3])
+    with pytest.raises(TypeError):
+        decode.token_logprobs(z, tok, live=tok)
+    with pytest.raises(TypeError):
+        decode.token_logprobs(z.long(), tok)
+    with pytest.raises(TypeError):
+        decode.token_logprobs(torch.zeros([]))
+    v, c = torch.zeros([4, 3]), torch.zeros([4, 3], dtype=torch.int64)
+    for bad in ((v[:, :0], c[:, :0]), (torch.zeros([4, 1025]), torch.zeros([4, 1025], dtype=torch.int64)), (v, c[:, :2]),
+                (v[:3], c[:3])):
+        with pytest.raises(ValueError):
+            decode.distill_rows(z, *bad)
+    with pytest.raises(TypeError):
+        decode.distill_rows(z, c, c)
+    with pytest.raises(TypeError):
+        decode.distill_rows(z, v, v)
+    with pytest.raises(ValueError):
+        decode.distill_rows(z, v, c, live=torch.ones([3], dtype=torch.bool))

@@ -1,0 +1,497 @@
+"""token_logprobs and distill_rows on the GPU against float64 references, within bounds derived from the arithmetic
+(helpers_logprobs): sizes around every internal boundary, masks that leave little or nothing of a row, ties, dead rows,
+strides, types, streams and captured graphs."""
+import numpy as np
+import pytest
+
+import helpers_logprobs as ref
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+DEV = "cuda:0"
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _decode():
+    from imagesegmentation_amd.polyrnn import decode
+    return decode
+
+
+def _f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _logits(rows, cols, dtype, kind, seed):
+    """Rows of one kind; what the kernel sees (rounded to its type) comes back as float64 too."""
+    rs = np.random.RandomState(seed)
+    z = rs.randn(rows, cols) * 3
+    lowest = torch.finfo(DT[dtype]).min
+    if kind == "peaked":
+        z[np.arange(rows), rs.randint(0, cols, rows)] += 20
+    elif kind == "ties":
+        z = np.round(z)
+    elif kind == "rising":
+        z = np.sort(z, axis=1)
+    elif kind == "constant":
+        z[:] = rs.randn(rows, 1)
+    elif kind == "masked":
+        z[rs.rand(rows, cols) < 0.6] = -np.inf
+        z[0, :] = -np.inf               # nothing left
+        z[-1, :] = -np.inf
+        z[-1, cols // 2] = 1.5          # one class left
+    elif kind == "lowest":
+        z[rs.rand(rows, cols) < 0.6] = lowest
+        z[0, :] = lowest                # a uniform row
+    elif kind == "zeros":
+        z[:] = 0.0
+        z[:, ::2] = -0.0                # equal to 0: the lower class first
+    t = torch.tensor(z, dtype=DT[dtype], device=DEV)
+    return t, _f64(t)
+
+
+def _check_logprobs(t, z, T, tokens, top, dtype, live=None, seed=0, graded=True):
+    decode = _decode()
+    rs = np.random.RandomState(seed + 99)
+    rows = z.shape[0]
+    t = t.detach().requires_grad_(graded)
+    tok = None if tokens is None else torch.tensor(tokens, device=DEV)
+    lv = None if live is None else torch.tensor(live, device=DEV)
+    out = decode.token_logprobs(t, tok, top=top, temperature=T, live=lv)
+    want = ref.token_logprobs(z, T, tokens, top)
+    on = np.ones([rows], bool) if live is None else live
+    for name in ("logprobs", "entropy", "top_logprobs"):
+        got = getattr(out, name)
+        if got is None:
+            assert name not in want
+            continue
+        assert got.dtype == torch.float32
+        got = _f64(got)
+        ref.close(got[on], want[name][on], want[name + "_tol"][on])
+        assert np.all(got[~on] == 0)
+    if top:
+        got = out.top_classes.cpu().numpy()
+        assert got.dtype == np.int32 and np.array_equal(got[on], want["top_classes"][on]) and np.all(got[~on] == -1)
+    if not graded:
+        return
+    gl = rs.randn(rows).astype(np.float32) if tokens is not None else None
+    gh = rs.randn(rows).astype(np.float32)
+    gt = rs.randn(rows, top).astype(np.float32) if top else None
+    outs, gs = [out.entropy], [gh]
+    if gl is not None:
+        outs, gs = outs + [out.logprobs], gs + [gl]
+    if gt is not None:
+        outs, gs = outs + [out.top_logprobs], gs + [gt]
+    dz, = torch.autograd.grad(outs, t, [torch.tensor(g, device=DEV) for g in gs])
+    f = lambda g: None if g is None else g.astype(np.float64)
+    wd, wtol = ref.token_logprobs_grad(z, T, tokens, want.get("top_classes"), f(gl), f(gh), f(gt), dtype)
+    assert dz.dtype == t.dtype and dz.shape == t.shape
+    got = _f64(dz)
+    ref.close(got[on], wd[on], wtol[on])
+    assert np.all(got[~on] == 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols,top", [(1, 1, 1), (3, 2, 2), (2, 7, 7), (5, 8, 3), (4, 63, 5), (4, 64, 64), (4, 65, 64),
+                                           (7, 127, 0), (3, 255, 64), (3, 257, 1), (6, 511, 8), (6, 513, 20), (33, 784, 5),
+                                           (33, 785, 64), (2, 1023, 33), (2, 1025, 32), (3, 2047, 64), (3, 2048, 16),
+                                           (3, 2049, 64), (2, 4096, 17), (2, 4097, 64), (2, 8191, 3), (2, 8193, 64),
+                                           (2, 16385, 20), (1, 50177, 64), (3, 131071, 20)])
+def test_logprobs_over_sizes(rows, cols, top, dtype):
+    t, z = _logits(rows, cols, dtype, "peaked", rows * 7 + cols)
+    tokens = np.random.RandomState(cols).randint(0, cols, [rows])
+    tokens[0] = int(np.argmax(z[0]))
+    _check_logprobs(t, z, 1.0, tokens, top, dtype, seed=cols)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [5, 96, 785, 2500, 9000, 40000])
+@pytest.mark.parametrize("kind", ["ties", "rising", "constant", "masked", "lowest", "zeros"])
+def test_logprobs_over_masks_and_ties(kind, cols, dtype):
+    rows = 5
+    t, z = _logits(rows, cols, dtype, kind, cols)
+    tokens = np.random.RandomState(cols).randint(0, cols, [rows])
+    for top in (0, min(cols, 3), min(cols, 64)):
+        _check_logprobs(t, z, 0.7, tokens, top, dtype, seed=cols + top)
+
+
+@pytest.mark.parametrize("T", [0.05, 0.7, 4.0, 1000.0])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logprobs_over_temperatures(T, dtype):
+    t, z = _logits(9, 785, dtype, "peaked", 11)
+    tokens = np.arange(9) * 80
+    _check_logprobs(t, z, T, tokens, 20, dtype)
+    _check_logprobs(t, z, T, None, 20, dtype)
+    _check_logprobs(t, z, T, None, 0, dtype)
+
+
+@pytest.mark.parametrize("cols", [785, 12000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_dead_rows_are_not_read(cols, dtype):
+    """NaN and infinities in rows that are not live reach no output and no gradient."""
+    t, z = _logits(12, cols, dtype, "peaked", 3)
+    live = np.array([True, False, True, True, False, False, True, False, True, True, True, False])
+    t[torch.tensor(~live, device=DEV)] = float("nan")
+    t[1] = float("inf")
+    tokens = np.full([12], 17)
+    tokens[4] = 10 ** 9  # a token of a dead row is not looked at
+    _check_logprobs(t, z, 1.3, tokens, 9, dtype, live=live)
+    _check_logprobs(t, z, 1.3, tokens, 0, dtype, live=np.zeros([12], bool))
+    decode = _decode()
+    values = torch.randn([12, 4], device=DEV)
+    classes = torch.randint(0, cols, [12, 4], device=DEV)
+    tt = t.clone().requires_grad_(True)
+    loss = decode.distill_rows(tt, values, classes, live=torch.tensor(live.astype(np.uint8), device=DEV))
+    loss.sum().backward()
+    assert torch.isfinite(loss).all() and torch.isfinite(tt.grad.float()).all()
+    dead = torch.tensor(~live, device=DEV)
+    assert (loss[dead] == 0).all() and (tt.grad[dead] == 0).all() and (loss[~dead] > 0).all()
+
+
+@pytest.mark.parametrize("cols", [785, 9001])
+def test_nan_and_infinite_logits_and_classes_outside_the_row(cols):
+    decode = _decode()
+    t, z = _logits(6, cols, "f32", "peaked", 8)
+    t[1, 70] = float("nan")
+    t[2, 70] = float("inf")
+    tokens = torch.tensor([3, 3, 3, -1, cols, 2 ** 32 + 3], device=DEV)
+    t.requires_grad_(True)
+    out = decode.token_logprobs(t, tokens, top=5)
+    assert torch.isnan(out.entropy[1:3]).all() and torch.isfinite(out.entropy[[0, 3, 4, 5]]).all()
+    assert torch.isnan(out.logprobs[1:]).all() and torch.isfinite(out.logprobs[0])
+    want = ref.token_logprobs(z, 1.0, None, 5)["top_classes"]
+    got = out.top_classes.cpu().numpy()
+    assert np.array_equal(got[[0, 3, 4, 5]], want[[0, 3, 4, 5]])
+    assert all(len(set(r)) == 5 and (r >= 0).all() and (r < cols).all() for r in got)
+    g, = torch.autograd.grad(out.logprobs, t, torch.tensor([1.0, 1.0, 1.0, 1.0, 0.0, 1.0], device=DEV))
+    assert torch.isfinite(g[0]).all() and torch.isnan(g[1]).all() and torch.isnan(g[3]).all() and torch.isnan(g[5]).all()
+    assert (g[4] == 0).all()  # no gradient arrives at the class that is not there
+    loss = decode.distill_rows(t, torch.zeros([6, 2], device=DEV),
+                               torch.tensor([[0, 1], [0, 1], [0, 1], [-5, 1], [cols, 1], [0, 2 ** 32]], device=DEV))
+    assert torch.isnan(loss[[1, 2, 4, 5]]).all() and torch.isfinite(loss[[0, 3]]).all()
+    g, = torch.autograd.grad(loss, t, torch.ones([6], device=DEV))
+    assert torch.isfinite(g[[0, 3]]).all() and torch.isnan(g[[1, 4, 5]]).all()
+
+
+def _check_distill(t, z, values, classes, T, tail, dtype, seed=0):
+    decode = _decode()
+    rows = z.shape[0]
+    g = np.random.RandomState(seed).randn(rows).astype(np.float32)
+    t = t.detach().requires_grad_(True)
+    loss = decode.distill_rows(t, torch.tensor(values, device=DEV), torch.tensor(classes, device=DEV), temperature=T,
+                               tail=tail)
+    want = ref.distill(z, values.astype(np.float64), classes, T, tail, g.astype(np.float64), dtype)
+    ref.close(_f64(loss), want["loss"], want["loss_tol"])
+    dz, = torch.autograd.grad(loss, t, torch.tensor(g, device=DEV))
+    assert dz.dtype == t.dtype and dz.shape == t.shape
+    ref.close(_f64(dz), want["dlogits"], want["dlogits_tol"])
+
+
+def _teacher(z, k, T, tail, seed):
+    """(values float32, classes int32) of a teacher near the student's own rows."""
+    rs = np.random.RandomState(seed)
+    t = np.where(np.isfinite(z), z, -50.0) + rs.randn(*z.shape)
+    classes = np.argsort(-t, axis=1, kind="stable")[:, :k].astype(np.int32)
+    logp = ref.softmax(t, T)[0]
+    v = np.take_along_axis(logp if tail else t, classes, axis=1)
+    return v.astype(np.float32), classes
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols,k", [(1, 1, 1), (3, 2, 1), (2, 7, 7), (5, 8, 3), (4, 64, 64), (4, 65, 64), (6, 513, 20),
+                                         (33, 784, 5), (33, 785, 64), (2, 1025, 100), (3, 2047, 64), (3, 2048, 16),
+                                         (3, 2049, 65), (2, 4097, 1024), (2, 8191, 3), (2, 8193, 64), (2, 16385, 20),
+                                         (1, 50177, 64), (2, 131071, 32)])
+def test_distillation_over_sizes(rows, cols, k, dtype, tail):
+    t, z = _logits(rows, cols, dtype, "peaked", rows * 5 + cols)
+    values, classes = _teacher(z, k, 1.7, tail, cols)
+    _check_distill(t, z, values, classes, 1.7, tail, dtype, seed=cols)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [30, 785, 5000, 20000])
+def test_distillation_with_absent_and_repeated_classes_and_masked_students(cols, dtype, tail):
+    t, z = _logits(8, cols, dtype, "masked", cols)
+    t[0], z[0] = 0.25, 0.25
+    k = 11
+    values, classes = _teacher(z, k, 1.0, tail, cols)
+    if tail:
+        values = values - 0.5                       # some mass left
+    classes[1, 4:] = -1                             # fewer entries than places
+    classes[2, :] = -7                              # none
+    classes[3, 5] = classes[3, 2]                   # a class twice
+    classes[4, :] = classes[4, 0]                   # one class in every place
+    if tail:
+        values[4, :] = values[4, :] - 3
+    values[5, 3] = -np.inf                          # an entry without mass
+    order = np.random.RandomState(1).permutation(k)
+    values[6], classes[6] = values[6, order], classes[6, order]
+    _check_distill(t, z, values, classes, 0.8, tail, dtype)
+
+
+@pytest.mark.parametrize("cols", [40, 9000])
+def test_distillation_where_nothing_is_left(cols):
+    """A student row without probability, a student that rules the teacher's class out, a teacher that names every class
+    of the student's, a remaining mass with no class to stand on."""
+    decode = _decode()
+    z = torch.randn([4, cols], device=DEV)
+    z[0] = float("-inf")
+    z[1, 5] = float("-inf")
+    classes = torch.tensor([[1, 2], [5, 6], [1, 2], [1, 2]], device=DEV)
+    z[2] = float("-inf")
+    z[2, 1:3] = 0.5
+    values = torch.log(torch.tensor([[0.5, 0.25]] * 4, device=DEV))
+    z.requires_grad_(True)
+    loss = decode.distill_rows(z, values, classes, tail=True)
+    assert loss[0] == float("inf") and loss[1] == float("inf") and loss[2] == float("inf") and torch.isfinite(loss[3])
+    g, = torch.autograd.grad(loss, z, torch.ones([4], device=DEV))
+    assert (g[0] == 0).all() and torch.isfinite(g).all()
+    loss = decode.distill_rows(z, values, classes)
+    assert loss[0] == float("inf") and loss[1] == float("inf") and torch.isfinite(loss[2:]).all()
+    g, = torch.autograd.grad(loss, z, torch.ones([4], device=DEV))
+    assert torch.isfinite(g).all() and (g[2, 3:] == 0).all()
+
+
+def test_a_student_mass_below_the_floats_keeps_its_logarithm():
+    """The classes outside the entries lie 200 nats down: their mass is no float, its logarithm is."""
+    decode = _decode()
+    for cols in (700, 9000):
+        z = torch.full([1, cols], -200.0, device=DEV)
+        z[0, 3] = 0.0
+        z.requires_grad_(True)
+        values = torch.log(torch.tensor([[0.75]], device=DEV))
+        loss = decode.distill_rows(z, values, torch.tensor([[3]], device=DEV), tail=True)
+        want = 0.75 * np.log(0.75) + 0.25 * (np.log(0.25) - (np.log(cols - 1) - 200.0))
+        # terms of 50 nats: 0.25 * 200 * 4 u and the logarithms' own steps
+        assert abs(float(loss.detach()) - want) < 64 * 2.0 ** -24 * 60
+        g, = torch.autograd.grad(loss, z, torch.ones([1], device=DEV))
+        assert abs(float(g[0, 3]) - 0.25) < 1e-6 and torch.allclose(g[0, :3], torch.tensor(-0.25 / (cols - 1), device=DEV),
+                                                                    rtol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols,width", [(785, 792), (785, 786), (9000, 9001), (50, 64)])
+def test_rows_apart_are_read_in_place(cols, width, dtype):
+    decode = _decode()
+    wide = torch.full([40, width], float("nan"), dtype=DT[dtype], device=DEV)
+    dense = torch.randn([40, cols], device=DEV).to(DT[dtype])
+    wide[:, :cols] = dense
+    tok = torch.randint(0, cols, [40], device=DEV)
+    a = dense.clone().requires_grad_(True)
+    values, classes = torch.topk(dense.float(), 6, dim=1)
+    for view in (wide[:, :cols], wide[::2, :cols], wide[3:, :cols]):
+        sel = slice(0, None, 2) if view.shape[0] == 20 else slice(40 - view.shape[0], None)
+        v = view.detach().requires_grad_(True)
+        x, y = decode.token_logprobs(v, tok[sel], top=6), decode.token_logprobs(a[sel], tok[sel], top=6)
+        assert all(torch.equal(p, q) for p, q in zip(x, y))
+        gx, = torch.autograd.grad(x.logprobs.sum() + x.entropy.sum() + x.top_logprobs.sum(), v)
+        gy, = torch.autograd.grad(y.logprobs.sum() + y.entropy.sum() + y.top_logprobs.sum(), a)
+        assert gx.shape == v.shape and torch.equal(gx, gy[sel])
+        for tail in (False, True):
+            x = decode.distill_rows(v, values[sel], classes[sel], tail=tail)
+            y = decode.distill_rows(a[sel], values[sel], classes[sel], tail=tail)
+            assert torch.equal(x, y)
+            assert torch.equal(torch.autograd.grad(x.sum(), v)[0], torch.autograd.grad(y.sum(), a)[0][sel])
+
+
+def test_shapes_types_and_orders_of_the_arguments():
+    """Leading axes, a single row, transposed and expanded logits, half and double precision, int64 and strided
+    arguments: the same numbers as the plain call."""
+    decode = _decode()
+    z = torch.randn([6, 4, 300], device=DEV)
+    tok = torch.randint(0, 300, [6, 4], device=DEV)
+    out = decode.token_logprobs(z, tok, top=3)
+    assert out.logprobs.shape == (6, 4) and out.entropy.shape == (6, 4) and out.top_classes.shape == (6, 4, 3)
+    flat = decode.token_logprobs(z.reshape(24, 300), tok.reshape(24).to(torch.int32), top=3)
+    assert torch.equal(out.logprobs.reshape(24), flat.logprobs)
+    tr = decode.token_logprobs(z.transpose(0, 1), tok.transpose(0, 1), top=3)
+    assert torch.equal(tr.top_logprobs.transpose(0, 1), out.top_logprobs)
+    one = decode.token_logprobs(z[2, 3], tok[2, 3], top=3)
+    assert one.logprobs.shape == () and torch.equal(one.logprobs, out.logprobs[2, 3]) and one.top_classes.shape == (3,)
+    row = z[:1, 0].expand(5, 300)
+    ex = decode.token_logprobs(row, tok[0, 0].expand(5))
+    assert torch.equal(ex.logprobs, out.logprobs[0, 0].expand(5))
+    none = decode.token_logprobs(z[:0], tok[:0], top=2)
+    assert none.logprobs.shape == (0, 4) and none.top_classes.shape == (0, 4, 2)
+    for half in (torch.float16, torch.float64):
+        h = z.to(half).requires_grad_(True)
+        a, b = decode.token_logprobs(h, tok), decode.token_logprobs(h.detach().float(), tok)
+        assert torch.equal(a.logprobs, b.logprobs)
+        g, = torch.autograd.grad(a.logprobs.sum(), h)
+        assert g.dtype == half and g.shape == h.shape
+    v, c = torch.topk(z, 7, dim=-1)
+    a = decode.distill_rows(z, v, c)
+    assert a.shape == (6, 4)
+    b = decode.distill_rows(z.transpose(0, 1), v.transpose(0, 1), c.to(torch.int32).transpose(0, 1))
+    assert torch.equal(a, b.transpose(0, 1))
+    assert torch.equal(decode.distill_rows(z[0, 0], v[0, 0], c[0, 0]), a[0, 0])
+    live = torch.rand([6, 4], device=DEV) < 0.5
+    m = decode.distill_mean(z, v, c, live=live)
+    want = a[live].double().mean()
+    assert abs(float(m) - float(want)) <= 1e-6 * float(want)
+    assert float(decode.distill_mean(z, v, c, live=torch.zeros_like(live))) == 0.0
+    assert abs(float(decode.distill_mean(z, v, c)) - float(a.double().mean())) <= 1e-6 * float(a.double().mean())
+
+
+def test_second_derivatives_are_refused_and_only_some_outputs_may_carry_gradients():
+    decode = _decode()
+    z = torch.randn([3, 50], device=DEV, requires_grad=True)
+    tok = torch.tensor([1, 2, 3], device=DEV)
+    out = decode.token_logprobs(z, tok, top=4)
+    g1, = torch.autograd.grad(out.logprobs.sum(), z, retain_graph=True, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g1.sum().backward()
+    g2, = torch.autograd.grad(out.entropy.sum(), z, retain_graph=True)
+    g3, = torch.autograd.grad(out.top_logprobs[:, 1].sum(), z, retain_graph=True)
+    both, = torch.autograd.grad(out.logprobs.sum() + out.entropy.sum() + out.top_logprobs[:, 1].sum(), z)
+    assert torch.allclose(both, g1.detach() + g2 + g3, rtol=0, atol=8 * 2.0 ** -24)
+    assert not out.top_classes.requires_grad
+    with pytest.raises(ValueError):
+        decode.token_logprobs(z, tok.cpu())
+    with pytest.raises(ValueError):
+        decode.distill_rows(z, torch.zeros([3, 2]), torch.zeros([3, 2], dtype=torch.int32, device=DEV))
+
+
+def test_the_gradient_of_long_rows_against_differences():
+    """A directional difference of the float64 definition along the direction the kernel's gradient gives."""
+    t, z = _logits(2, 6000, "f32", "peaked", 4)
+    decode = _decode()
+    t.requires_grad_(True)
+    tokens = np.array([5, 4000])
+    out = decode.token_logprobs(t, torch.tensor(tokens, device=DEV))
+    g, = torch.autograd.grad(out.logprobs.sum() + 0.5 * out.entropy.sum(), t)
+    g = _f64(g)
+    f = lambda y: sum((lambda r: r["logprobs"] + 0.5 * r["entropy"])(ref.token_logprobs(y, 1.0, tokens))).sum()
+    h = 1e-4
+    diff = (f(z + h * g) - f(z - h * g)) / (2 * h)
+    assert abs(diff - (g * g).sum()) < 1e-5 * (g * g).sum()  # the kernel's relative error plus h^2
+    values, classes = _teacher(z, 9, 1.0, True, 3)
+    loss = decode.distill_rows(t, torch.tensor(values, device=DEV), torch.tensor(classes, device=DEV), tail=True)
+    g = _f64(torch.autograd.grad(loss.sum(), t)[0])
+    f = lambda y: ref.distill(y, values.astype(np.float64), classes, 1.0, True)["loss"].sum()
+    diff = (f(z + h * g) - f(z - h * g)) / (2 * h)
+    assert abs(diff - (g * g).sum()) < 1e-5 * (g * g).sum() + 1e-9
+
+
+@pytest.mark.parametrize("cols", [785, 20000])
+def test_a_teacher_through_both_operators(cols):
+    """The run a user makes: the teacher's best classes, the student's loss against them, its gradient - and the
+    divergence vanishing where the student is the teacher."""
+    decode = _decode()
+    rows, k, T = 24, 16, 2.0
+    for dtype in ("f32", "bf16"):
+        teacher, zt = _logits(rows, cols, dtype, "peaked", 21)
+        student, zs = _logits(rows, cols, dtype, "peaked", 22)
+        live = np.arange(rows) % 5 != 3
+        lv = torch.tensor(live, device=DEV)
+        best = decode.token_logprobs(teacher, top=k, temperature=T, live=lv)
+        student.requires_grad_(True)
+        loss = decode.distill_rows(student, best.top_logprobs, best.top_classes, temperature=T, tail=True, live=lv)
+        dz, = torch.autograd.grad(loss, student, torch.full([rows], 0.5, device=DEV))
+        values, classes = _f64(best.top_logprobs), best.top_classes.cpu().numpy()
+        want = ref.distill(zs, values, classes, T, True, np.full([rows], 0.5), dtype)
+        ref.close(_f64(loss)[live], want["loss"][live], want["loss_tol"][live])
+        ref.close(_f64(dz)[live], want["dlogits"][live], want["dlogits_tol"][live])
+        assert (_f64(loss)[~live] == 0).all() and (_f64(dz)[~live] == 0).all()
+        same = decode.distill_rows(teacher, best.top_logprobs, best.top_classes, temperature=T, tail=True, live=lv)
+        w = ref.distill(zt, values, classes, T, True)
+        ref.close(_f64(same)[live], w["loss"][live], w["loss_tol"][live])
+        assert float(same.abs().max()) < 1e-4
+
+
+def test_on_another_stream_and_the_same_bits_each_time():
+    decode = _decode()
+    for cols in (785, 30000):
+        z = torch.randn([50, cols], device=DEV)
+        tok = torch.randint(0, cols, [50], device=DEV)
+        v, c = torch.topk(z, 12, dim=1)
+        torch.cuda.synchronize()
+
+        def once():
+            y = z.detach().requires_grad_(True)
+            o = decode.token_logprobs(y, tok, top=12)
+            d = decode.distill_rows(y, v, c, tail=False)
+            g, = torch.autograd.grad((o.logprobs.sum() + o.entropy.sum() + d.sum()), y)
+            return [o.logprobs.detach(), o.entropy.detach(), o.top_logprobs.detach(), o.top_classes, d.detach(), g]
+        first = once()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            second = once()
+        third = once()  # (at the same time as the second, on the default stream)
+        torch.cuda.synchronize()
+        for a, b, d in zip(first, second, third):
+            assert torch.equal(a, b) and torch.equal(a, d)
+
+
+@pytest.mark.parametrize("rows,cols", [(12, 785), (3, 50177)])
+def test_captured_and_replayed(rows, cols):
+    """Forward and backward of both operators as two graphs that live at once: replays after new inputs, with eager work
+    between them, give the eager results bit for bit."""
+    decode = _decode()
+    z = torch.randn([rows, cols], device=DEV)
+    tok = torch.randint(0, cols, [rows], device=DEV)
+    up = torch.randn([rows], device=DEV)
+
+    def work(y):
+        y = y.detach().requires_grad_(True)
+        o = decode.token_logprobs(y, tok, top=8)
+        g, = torch.autograd.grad((o.logprobs, o.entropy), y, (up, up))
+        return [o.logprobs.detach(), o.entropy.detach(), o.top_logprobs.detach(), o.top_classes, g]
+
+    def work2(y, best):
+        y = (y * 0.5).detach().requires_grad_(True)
+        d = decode.distill_rows(y, best[2], best[3], tail=True)
+        g, = torch.autograd.grad(d, y, up)
+        return [d.detach(), g]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # (library handles and the allocator's pools, outside the capture)
+        work2(z, work(z))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        out1 = work(z)
+    with torch.cuda.graph(g2):
+        out2 = work2(z, out1)
+    for n in range(4):
+        z.copy_(torch.randn([rows, cols], device=DEV) * (n + 1))
+        eager1 = work(z)
+        eager2 = work2(z, eager1)
+        g1.replay()
+        if n == 2:
+            torch.cuda.synchronize()
+        g2.replay()
+        for a, b in zip(out1 + out2, eager1 + eager2):
+            assert torch.equal(a, b)
+
+
+def test_rows_past_two_to_the_thirty_one_elements():
+    """Offsets that do not fit 32 bits: the last rows of 2.2e9 bf16 elements."""
+    decode = _decode()
+    rows, cols = 2200, 1000003
+    z = torch.zeros([rows, cols], dtype=torch.bfloat16, device=DEV)
+    z[-2:] = torch.randn([2, cols], device=DEV).to(torch.bfloat16) * 3
+    tail = z[-2:].clone()
+    tok = torch.full([rows], cols - 1, device=DEV)
+    z.requires_grad_(True)
+    out = decode.token_logprobs(z, tok, top=3)
+    small = decode.token_logprobs(tail, tok[-2:], top=3)
+    for a, b in zip(out, small):
+        assert torch.equal(a[-2:], b)
+    assert (out.top_classes[0] == torch.arange(3, device=DEV)).all()
+    g, = torch.autograd.grad(out.logprobs.sum(), z)
+    tail.requires_grad_(True)
+    gs, = torch.autograd.grad(decode.token_logprobs(tail, tok[-2:]).logprobs.sum(), tail)
+    assert torch.equal(g[-2:], gs)
+    del g, gs, out
+    v, c = small.top_logprobs, small.top_classes
+    live = torch.zeros([rows], dtype=torch.bool, device=DEV)
+    live[-2:] = True
+    loss = decode.distill_rows(z, v[:1].expand(rows, 3), c[:1].expand(rows, 3), tail=True, live=live)
+    g, = torch.autograd.grad(loss.sum(), z)
+    ls = decode.distill_rows(tail, v[:1].expand(2, 3), c[:1].expand(2, 3), tail=True)
+    gs, = torch.autograd.grad(ls.sum(), tail)
+    assert torch.equal(loss[-2:].detach(), ls.detach()) and torch.equal(g[-2:], gs) and not g[:-2].any()
