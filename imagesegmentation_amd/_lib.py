@@ -72,11 +72,13 @@ SIGNATURES = {
     "isg_copy_channel_slice": (_int, [_vp, _vp, _vp, _vp, _int, _ll, _ll, _ll, _vp]),
     "isg_a3c_loss_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _vp, _vp]),
     "isg_a3c_loss_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _vp, _vp]),
+    "isg_token_logprobs_workspace_bytes": (_ll, [_int, _int, _int]),
     "isg_token_logprobs_fwd": (_int, [_vp, _ll, _vp, _int, _vp, _int, _int, _int, _f32, _int, _vp, _vp, _vp, _vp, _vp,
-                                      _vp]),
-    "isg_token_logprobs_bwd": (_int, [_vp, _ll, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _f32, _int,
                                       _vp, _vp]),
-    "isg_distill_fwd": (_int, [_vp, _ll, _vp, _vp, _int, _vp, _int, _int, _int, _int, _f32, _int, _vp, _vp, _vp]),
+    "isg_token_logprobs_bwd": (_int, [_vp, _ll, _vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _f32, _int, _vp,
+                                      _vp]),
+    "isg_distill_workspace_bytes": (_ll, [_int, _int]),
+    "isg_distill_fwd": (_int, [_vp, _ll, _vp, _vp, _int, _vp, _int, _int, _int, _int, _f32, _int, _vp, _vp, _vp, _vp]),
     "isg_distill_bwd": (_int, [_vp, _ll, _vp, _vp, _int, _vp, _vp, _int, _int, _int, _int, _f32, _int, _vp, _vp]),
     "isg_rollout_record": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp, _vp, _vp]),
     "isg_gae": (_int, [_vp, _vp, _vp, _vp, _int, _int, _f64, _f64, _vp, _vp, _vp]),
@@ -158,3 +160,10 @@ def ptr(t):
 def current_stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+def stream_of(t):
+    """The current stream of a tensor's device, as the C entries take it (a fifth of ``current_stream``'s time, which a
+    call from an autograd thread pays six-fold)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(t.device.index)

@@ -6,7 +6,17 @@
 // every term of H has one sign, so a confident row loses nothing to cancellation, and z_c - m comes first, so that
 // rows of the type's lowest value are uniform rows and not overflows.  A class at -inf has no probability and adds
 // nothing (its x is kept from meeting 0 * inf by a lower bound far below the smallest float).  All sums are float.
+//
+// Layout.  A row is read once, into registers: up to 2,048 classes by one wave (four rows to a workgroup, no barrier),
+// longer ones in chunks of 2,048 to 8,192 by a workgroup each, whose partial results (maximum, sums, best classes) a
+// second launch joins.  Loads are 16 bytes a lane at whatever alignment the row has (rows of 785 bf16 logits start on
+// any even address); the last vector of a row is the row's last 16 bytes, and what it repeats of its neighbour is
+// blanked.
 #include <hip/hip_bf16.h>
+
+#include <math.h>
+
+#include <type_traits>
 
 #include "isg_common.h"
 
@@ -18,72 +28,188 @@ constexpr int kThreads = 256;
 constexpr int kMaxTop = ISG_TOP_MAX;          // classes kept per row
 constexpr int kMaxEntries = ISG_DISTILL_MAX;  // a teacher's classes per row
 constexpr int kMaxCols = ISG_CLASSES_MAX;     // class axis
+constexpr int kWaveCols = 2048;               // classes one wave holds (32 registers a lane)
+constexpr int kCandidates = 256;              // alternatives in question per wave; a workgroup holds four times as many
 
-template <typename T>
-__device__ __forceinline__ float ld(const T* p, long long i) {
-    return (float)p[i];
+typedef unsigned long long u64;
+
+// ---- across the lanes of a wave: data-parallel moves inside the vector unit (six instructions, no LDS) -------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float old, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
 }
-
+__device__ __forceinline__ float last_lane(float v) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    v = fmaxf(v, dpp<0x111, 0xf>(v, v));  // row_shr:1, 2, 4, 8
+    v = fmaxf(v, dpp<0x112, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x114, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x118, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x142, 0xa>(v, v));  // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
+    v = fmaxf(v, dpp<0x143, 0xc>(v, v));
+    return last_lane(v);
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    v += dpp<0x111, 0xf>(0.0f, v);
+    v += dpp<0x112, 0xf>(0.0f, v);
+    v += dpp<0x114, 0xf>(0.0f, v);
+    v += dpp<0x118, 0xf>(0.0f, v);
+    v += dpp<0x142, 0xa>(0.0f, v);
+    v += dpp<0x143, 0xc>(0.0f, v);
+    return last_lane(v);
+}
+// sum of the lanes up to and including this one
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
     return v;
+}
+__device__ __forceinline__ u64 wave_max_key(u64 k) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const u64 other = __shfl_xor(k, o);
+        k = other > k ? other : k;
+    }
+    return k;
 }
 
-// the value over a workgroup of kThreads, in a fixed order; `red` is kThreads / 64 floats of LDS
-__device__ float block_max(float v, float* red) {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-    for (int w = 1; w < kThreads / 64; ++w) v = fmaxf(v, red[w]);
-    return v;
+// W waves that share a row: LDS written by one lane is there for the others
+template <int W>
+__device__ __forceinline__ void together() {
+    if constexpr (W == 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
+    }
 }
-__device__ float block_sum(float v, float* red) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-    for (int w = 1; w < kThreads / 64; ++w) v += red[w];
-    return v;
+
+__device__ __forceinline__ float ld(const float* p, long long i) { return p[i]; }
+__device__ __forceinline__ float ld(const __hip_bfloat16* p, long long i) { return (float)p[i]; }
+
+// N logits from any address, as floats (N sizeof(T) is 2 to 16 bytes: one load)
+template <int N>
+__device__ __forceinline__ void load_vector(const float* p, float* v) {
+    __builtin_memcpy(v, p, N * 4);
 }
+template <int N>
+__device__ __forceinline__ void load_vector(const __hip_bfloat16* p, float* v) {
+    if constexpr (N == 1) {
+        v[0] = (float)p[0];
+    } else {
+        unsigned w[N / 2];
+        __builtin_memcpy(w, p, N * 2);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+// (floats to bf16 round to nearest even, by the chip's own conversion)
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <int N>
+__device__ __forceinline__ void store_vector(float* p, const float* v) {
+    __builtin_memcpy(p, v, N * 4);
+}
+template <int N>
+__device__ __forceinline__ void store_vector(__hip_bfloat16* p, const float* v) {
+    if constexpr (N == 1) {
+        const __bf16 b = (__bf16)v[0];
+        __builtin_memcpy(p, &b, 2);
+    } else {
+        bf16x2 w[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) w[i] = __builtin_convertvector(f32x2{v[2 * i], v[2 * i + 1]}, bf16x2);
+        __builtin_memcpy(p, w, N * 2);
+    }
+}
+
+// Where the elements of a thread lie in its row: NE of them in vectors of VE, `threads` vectors of a slot side by side.
+// A vector that would end behind the row is the row's last VE elements; `blank` of them belong to its neighbour.
+template <typename T, int W, int NE>
+struct Span {
+    static constexpr int VE = NE < 16 / (int)sizeof(T) ? NE : 16 / (int)sizeof(T);
+    static constexpr int NV = NE / VE;
+    static constexpr int kCols = W * 64 * NE;  // of one unit (a wave or a workgroup)
+    int base, cols, lane;                      // lane: of the unit's W * 64
+
+    __device__ __forceinline__ Span(int base_, int cols_, int lane_) : base(base_), cols(cols_), lane(lane_) {}
+    __device__ __forceinline__ int start(int slot) const { return base + (slot * W * 64 + lane) * VE; }
+    __device__ __forceinline__ bool full(int slot) const { return base + (slot + 1) * W * 64 * VE <= cols; }  // (uniform)
+    __device__ __forceinline__ bool empty(int slot) const { return base + slot * W * 64 * VE >= cols; }       // (uniform)
+    __device__ __forceinline__ int offset(int slot) const {
+        const int s = start(slot);
+        return s < cols - VE ? s : cols - VE;
+    }
+    // the class of element e, or -1 where it is not this thread's
+    __device__ __forceinline__ int cls(int e) const {
+        const int s = start(e / VE), i = offset(e / VE) + e % VE;
+        return i >= s ? i : -1;
+    }
+    // thread and element of a class inside the unit
+    __device__ __forceinline__ void locate(int c, int& thread, int& e) const {
+        const int l = c - base, vec = l / VE, s = base + vec * VE;
+        const int over = s + VE - cols;
+        thread = vec % (W * 64);
+        e = vec / (W * 64) * VE + l % VE + (over > 0 ? over : 0);
+    }
+    // the elements; those that are not this thread's as -inf (BLANK) or as whatever class lies there
+    template <bool BLANK>
+    __device__ __forceinline__ void load(const T* z, float (&v)[NE]) const {
+#pragma unroll
+        for (int t = 0; t < NV; ++t) {
+            if (full(t)) {
+                load_vector<VE>(z + start(t), v + t * VE);
+            } else if (!empty(t)) {
+                const int s = start(t), o = offset(t);
+                load_vector<VE>(z + o, v + t * VE);
+                if constexpr (BLANK) {
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) v[t * VE + j] = o + j >= s ? v[t * VE + j] : -INFINITY;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) v[t * VE + j] = -INFINITY;
+            }
+        }
+    }
+    // a slot's gradients; the row's last vector repeats values of its neighbour, which is no harm inside the unit
+    __device__ __forceinline__ void store(T* d, int t, const float* o) const {
+        const int s = start(t), at = offset(t);
+        if (full(t)) {
+            store_vector<VE>(d + s, o);
+        } else if (s < cols) {
+            if (at >= base) {
+                store_vector<VE>(d + at, o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VE; ++j)
+                    if (at + j >= s) store_vector<1>(d + at + j, o + j);
+            }
+        }
+    }
+};
 
 // a class index stored as 4 or 8 bytes
 __device__ __forceinline__ long long class_at(const void* p, int bytes, long long i) {
     return bytes == 8 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
 }
 
-// Order of the alternatives as one integer: larger logits first (-0 equals 0, NaN last), equal ones by class.
+// Order of the alternatives as one integer: larger logits first (-0 equals 0, NaN below -inf), equal ones by class;
+// 0 is no class.
 __device__ __forceinline__ unsigned order_bits(float v) {
     const unsigned b = __float_as_uint(v + 0.0f);
-    if (v != v) return 0u;
+    if (v != v) return 1u;
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ unsigned long long order_key(float v, int c) {
-    return ((unsigned long long)order_bits(v) << 32) | (unsigned)~c;
+__device__ __forceinline__ float order_value(unsigned k) {
+    return k == 1u ? NAN : __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long k) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor(k, o);
-        k = other > k ? other : k;
-    }
-    return k;
-}
-
-// x = (z - m) log2(e) / T and its power; u_term is 2^x x with 0 for a class without probability
-__device__ __forceinline__ void power(float z, float m, float c, float& e, float& u_term) {
-    const float x = (z - m) * c;
-    e = exp2f(x);
-    u_term = e * fmaxf(x, -1000.0f);
-}
+__device__ __forceinline__ u64 order_key(float v, int c) { return c < 0 ? 0ull : ((u64)order_bits(v) << 32) | (unsigned)~c; }
 
 // log p of a logit; a row without any probability (log2 s = +inf) gives -inf.  In nats throughout: at T = 1 the
 // type's lowest value has a finite logarithm, its binary one would overflow.
@@ -91,114 +217,370 @@ __device__ __forceinline__ float log_prob(float z, float m, float inv_t, float l
     return (z - m) * inv_t - kLn2 * l2s;
 }
 
-// ---- token_logprobs ------------------------------------------------------------------------------------------------
-// One workgroup per row: a pass for the maximum, one for the sums, one per kept class.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(
-    const T* __restrict__ logits, long long row_stride, const void* __restrict__ tokens, int token_bytes,
-    const unsigned char* __restrict__ live, int cols, float c, float inv_t, int top, float* __restrict__ logprobs,
-    float* __restrict__ entropy, float* __restrict__ top_logprobs, int* __restrict__ top_classes,
-    float* __restrict__ stats) {
-    __shared__ float red[kThreads / 64];
-    __shared__ unsigned long long redk[kThreads / 64];
-    const long long row = blockIdx.x;
-    const int tid = threadIdx.x;
-    if (live && !live[row]) {
-        if (tid == 0) {
-            if (logprobs) logprobs[row] = 0.0f;
-            entropy[row] = 0.0f;
-            if (stats) stats[4 * row] = 0.0f, stats[4 * row + 1] = 0.0f, stats[4 * row + 2] = 0.0f, stats[4 * row + 3] = 0.0f;
-        }
-        for (int j = tid; j < top; j += kThreads) top_logprobs[row * top + j] = 0.0f, top_classes[row * top + j] = -1;
-        return;
+// ---- the `top` first keys of a unit ----------------------------------------------------------------------------------
+// The k-th largest of the threads' group maxima is a lower bound of the k-th largest element (k groups hold one at
+// least as large), so the elements not below it are few more than k: k + k^2 / (2 groups) for values in any order.
+// The bound is found to 16 bits by bisection - one comparison a group and a count of the wave's mask per bit, the
+// scalar unit's work -, the elements above it are put side by side in LDS, and each one's place is the number of keys
+// above its own.  Bounds that no finite logit supports and more ties than fit go one class at a time instead.
+template <int W>
+struct TopShared {
+    u64 cand[4 * kCandidates];   // W = 1: a quarter for each wave
+    unsigned group[W == 1 ? 1 : kThreads];
+    unsigned count;
+    u64 best[4];
+};
+
+template <int W, int NE, typename Key, typename Reload, typename Emit>
+__device__ __forceinline__ void select_top(const float (&v)[NE], int k, TopShared<W>& sh, Key key, Reload reload, Emit emit) {
+    constexpr int Q = W == 1 ? (NE < 4 ? NE : 4) : 1;
+    constexpr int kCap = W == 1 ? kCandidates : 4 * kCandidates;
+    const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
+    u64* cand = sh.cand + (W == 1 ? (threadIdx.x >> 6) * kCandidates : 0);
+    float gm[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        gm[q] = v[q];
+#pragma unroll
+        for (int e = q + Q; e < NE; e += Q) gm[q] = fmaxf(gm[q], v[e]);
     }
-    const T* z = logits + row * row_stride;
-    float m = -INFINITY;
-    for (int i = tid; i < cols; i += kThreads) m = fmaxf(m, ld(z, i));
-    m = block_max(m, red);
-    if (m == -INFINITY) m = 0.0f;  // no class has probability (or all are NaN): 2^-inf sums to nothing
-    float s = 0.0f, u = 0.0f;
-    for (int i = tid; i < cols; i += kThreads) {
-        float e, ut;
-        power(ld(z, i), m, c, e, ut);
-        s += e, u += ut;
-    }
-    s = block_sum(s, red);
-    u = block_sum(u, red);
-    const float l2s = s == 0.0f ? INFINITY : log2f(s);
-    const float H = s == 0.0f ? 0.0f : kLn2 * (l2s - u / s);
-    if (tid == 0) {
-        if (tokens) {
-            const long long a = class_at(tokens, token_bytes, row);
-            logprobs[row] = a >= 0 && a < cols ? log_prob(ld(z, a), m, inv_t, l2s) : NAN;
+    unsigned bound = 0;
+    if constexpr (W == 1) {
+        if (k > 16) {  // (several groups a lane: fewer elements to each)
+            unsigned g[Q];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) g[q] = order_bits(gm[q]) >> 16;
+            for (int bit = 15; bit >= 0; --bit) {
+                const unsigned t = bound | (1u << bit);
+                int n = 0;
+#pragma unroll
+                for (int q = 0; q < Q; ++q) n += __builtin_popcountll(__ballot(g[q] >= t));
+                if (n >= k) bound = t;
+            }
+        } else {
+            float lm = gm[0];
+#pragma unroll
+            for (int q = 1; q < Q; ++q) lm = fmaxf(lm, gm[q]);
+            const unsigned g = order_bits(lm) >> 16;
+            for (int bit = 15; bit >= 0; --bit) {
+                const unsigned t = bound | (1u << bit);
+                if (__builtin_popcountll(__ballot(g >= t)) >= k) bound = t;
+            }
         }
-        entropy[row] = H;
-        if (stats) stats[4 * row] = m, stats[4 * row + 1] = l2s, stats[4 * row + 2] = H, stats[4 * row + 3] = 0.0f;
-    }
-    unsigned long long last = ~0ull;
-    for (int j = 0; j < top; ++j) {
-        unsigned long long best = 0;
-        for (int i = tid; i < cols; i += kThreads) {
-            const unsigned long long k = order_key(ld(z, i), i);
-            if (k < last && k > best) best = k;
+    } else {
+        if (tid == 0) sh.count = 0;
+        sh.group[tid] = order_bits(gm[0]) >> 16;
+        together<W>();
+        unsigned g[W];
+#pragma unroll
+        for (int q = 0; q < W; ++q) g[q] = sh.group[q * 64 + lane];
+        for (int bit = 15; bit >= 0; --bit) {
+            const unsigned t = bound | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int q = 0; q < W; ++q) n += __builtin_popcountll(__ballot(g[q] >= t));
+            if (n >= k) bound = t;
         }
-        best = wave_max_key(best);
-        __syncthreads();
-        if ((tid & 63) == 0) redk[tid >> 6] = best;
-        __syncthreads();
-        for (int w = 0; w < kThreads / 64; ++w) best = redk[w] > best ? redk[w] : best;
-        last = best;
-        if (tid == 0) {
-            const int cls = (int)~(unsigned)best;
-            top_logprobs[row * top + j] = log_prob(ld(z, cls), m, inv_t, l2s);
-            top_classes[row * top + j] = cls;
+    }
+    int total = kCap + 1;
+    if (bound > 0x7fu) {  // (0x7f begins the key of -inf)
+        const float low = order_value(bound << 16);
+        unsigned hit = 0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) hit |= (v[e] >= low ? 1u : 0u) << e;
+        const int mine = __builtin_popcount(hit);
+        int at;
+        if constexpr (W == 1) {
+            const int upto = wave_scan(mine);
+            total = __builtin_amdgcn_readlane(upto, 63);
+            at = upto - mine;
+        } else {
+            at = mine ? (int)atomicAdd(&sh.count, (unsigned)mine) : 0;
+            together<W>();
+            total = (int)sh.count;
+        }
+        if (total <= kCap) {
+            while (hit) {
+                const int e = __builtin_ctz(hit);
+                hit &= hit - 1;
+                cand[at++] = reload(e);
+            }
+            together<W>();
+            for (int r = tid; r < total; r += W * 64) {
+                const u64 own = cand[r];
+                int place = 0;
+                for (int o = 0; o < total; ++o) place += cand[o] > own ? 1 : 0;
+                if (place < k) emit(place, own);
+            }
+        }
+    }
+    if (total > kCap) {
+        u64 last = ~0ull;
+        for (int j = 0; j < k; ++j) {
+            u64 best = 0;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                const u64 x = key(e);
+                if (x < last && x > best) best = x;
+            }
+            best = wave_max_key(best);
+            if constexpr (W > 1) {
+                together<W>();
+                if (lane == 0) sh.best[tid >> 6] = best;
+                together<W>();
+#pragma unroll
+                for (int w = 0; w < W; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+            }
+            last = best;
+            if (tid == 0) emit(j, best);
+            if (best == 0) {  // (fewer classes than are asked for: the last part of a split row)
+                for (int o = j + 1 + tid; o < k; o += W * 64) emit(o, 0ull);
+                break;
+            }
         }
     }
 }
 
-// dlogits[c] = 1/T ([c = a] g_a + sum_j [c = i_j] g_j - p_c (g_a + sum_j g_j) - g_H p_c (log p_c + H)): the dense part
-// is written first, the few classes with a gradient of their own are written again behind it.
+// maximum, sum of powers and sum of powers times exponents of a part of a row
+struct Sums {
+    float m, s, u;
+};
+
+// The sums over a unit's elements.  A unit without any probability has m = -inf and s = 0.
+template <int W, int NE>
+__device__ __forceinline__ Sums unit_sums(const float (&v)[NE], float c, float (*red)[4]) {
+    float m = v[0];
+#pragma unroll
+    for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
+    m = wave_max(m);
+    const float mz = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+        const float x = (v[e] - mz) * c, p = __builtin_amdgcn_exp2f(x);
+        s += p;
+        u += p * fmaxf(x, -1000.0f);
+    }
+    s = wave_sum(s), u = wave_sum(u);
+    if constexpr (W == 1) return Sums{m, s, u};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane == 0) red[wave][0] = m, red[wave][1] = s, red[wave][2] = u;
+    together<W>();
+    Sums r{red[0][0], 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 1; w < W; ++w) r.m = fmaxf(r.m, red[w][0]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const float sw = red[w][1];
+        if (sw == 0.0f) continue;
+        const float d = (red[w][0] - r.m) * c, f = __builtin_amdgcn_exp2f(d);
+        r.s += f * sw;
+        r.u += f * (red[w][2] + fmaxf(d, -1000.0f) * sw);
+    }
+    return r;
+}
+
+// What a row's results follow from.  `c_rel`: by how much log2(e) / T exceeds the float c, relative; the logarithm of
+// the sum moves with the exponents' scale as their mean does, u / s.
+struct RowStats {
+    float m, l2s, H;
+};
+__device__ __forceinline__ RowStats row_stats(const Sums& t, float c_rel) {
+    RowStats r;
+    r.m = t.m == -INFINITY ? 0.0f : t.m;
+    const float mean = t.u / t.s;
+    r.l2s = t.s == 0.0f ? INFINITY : __builtin_amdgcn_logf(t.s) + c_rel * mean;
+    r.H = t.s == 0.0f ? 0.0f : kLn2 * (r.l2s - mean);
+    return r;
+}
+
+struct LogprobsArgs {
+    const void* tokens;
+    const unsigned char* live;
+    float* logprobs;
+    float* entropy;
+    float* top_logprobs;
+    int* top_classes;
+    float* stats;
+    Sums* part;      // [rows][splits]
+    u64* part_keys;  // [rows][splits][top]
+    long long row_stride, units;
+    int token_bytes, cols, splits, top;
+    float c, inv_t, c_rel;
+};
+
+// a dead row's outputs
+template <int W>
+__device__ __forceinline__ void dead_row(const LogprobsArgs& a, long long row, int tid) {
+    if (tid == 0) {
+        if (a.logprobs) a.logprobs[row] = 0.0f;
+        a.entropy[row] = 0.0f;
+        if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(0.0f, INFINITY, 0.0f, 0.0f);
+    }
+    for (int j = tid; j < a.top; j += W * 64) a.top_logprobs[row * a.top + j] = 0.0f, a.top_classes[row * a.top + j] = -1;
+}
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(
-    const T* __restrict__ logits, long long row_stride, const void* __restrict__ tokens, int token_bytes,
-    const unsigned char* __restrict__ live, const int* __restrict__ top_classes, const float* __restrict__ stats,
-    const float* __restrict__ dlogprobs, const float* __restrict__ dentropy, const float* __restrict__ dtop, int cols,
-    float c, float inv_t, int top, T* __restrict__ dlogits) {
-    __shared__ float red[kThreads / 64];
-    const long long row = blockIdx.x;
-    const int tid = threadIdx.x;
-    T* d = dlogits + row * cols;
-    const float m = stats[4 * row], l2s = stats[4 * row + 1], H = stats[4 * row + 2];
-    if ((live && !live[row]) || l2s == INFINITY) {  // dead, or no class has probability: nothing to move
-        for (int i = tid; i < cols; i += kThreads) d[i] = (T)0.0f;
+__device__ __forceinline__ void row_outputs(const LogprobsArgs& a, const T* z, long long row, const RowStats& r) {
+    if (a.tokens) {
+        const long long t = class_at(a.tokens, a.token_bytes, row);
+        a.logprobs[row] = t >= 0 && t < a.cols ? log_prob(ld(z, t), r.m, a.inv_t, r.l2s) : NAN;
+    }
+    a.entropy[row] = r.H;
+    if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(r.m, r.l2s, r.H, 0.0f);
+}
+
+__device__ __forceinline__ long long block_index() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
+// ---- token_logprobs ------------------------------------------------------------------------------------------------
+template <typename T, int W, int NE, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restrict__ logits, LogprobsArgs a) {
+    __shared__ float red[W][4];
+    __shared__ typename std::conditional<TOP, TopShared<W>, char>::type shared;
+    const int tid = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
+    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+    if (unit >= a.units) return;
+    const long long row = a.splits == 1 ? unit : unit / a.splits;
+    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    if (a.live && !a.live[row]) {
+        if (a.splits == 1) dead_row<W>(a, row, tid);
         return;
     }
-    const T* z = logits + row * row_stride;
-    const float ga = dlogprobs ? dlogprobs[row] : 0.0f, gh = dentropy ? dentropy[row] : 0.0f;
-    const long long a = dlogprobs ? class_at(tokens, token_bytes, row) : -1;
-    float g = 0.0f;
-    if (dtop)
-        for (int j = tid; j < top; j += kThreads) g += dtop[row * top + j];
-    g = dtop ? block_sum(g, red) : 0.0f;
-    g += ga;
-    if (dlogprobs && ga != 0.0f && (a < 0 || a >= cols)) g = NAN;  // a class the row does not have
-    auto dense = [&](int i, float& p) {
-        const float x = (ld(z, i) - m) * c - l2s;
-        p = exp2f(x);
-        return -p * (g + gh * (kLn2 * fmaxf(x, -1000.0f) + H));
-    };
-    for (int i = tid; i < cols; i += kThreads) {
-        float p;
-        d[i] = (T)(inv_t * dense(i, p));
+    const T* z = logits + row * a.row_stride;
+    const Span<T, W, NE> span(split * Span<T, W, NE>::kCols, a.cols, tid);
+    float v[NE];
+    span.template load<true>(z, v);
+    const Sums t = unit_sums<W, NE>(v, a.c, red);
+    RowStats r;
+    if (a.splits == 1) {
+        r = row_stats(t, a.c_rel);
+        if (tid == 0) row_outputs(a, z, row, r);
+    } else if (tid == 0) {
+        a.part[unit] = t;
     }
-    __syncthreads();
-    const int entries = (dtop ? top : 0) + 1;
-    for (int j = tid; j < entries; j += kThreads) {
-        const long long i = j + 1 < entries ? (long long)top_classes[row * top + j] : a;
-        if (i < 0 || i >= cols) continue;
-        float own = i == a ? ga : 0.0f, p;
-        for (int k = 0; k + 1 < entries; ++k) own += top_classes[row * top + k] == i ? dtop[row * top + k] : 0.0f;
-        d[i] = (T)(inv_t * (dense((int)i, p) + own));
+    if constexpr (TOP) {
+        const auto key = [&](int e) { return order_key(v[e], span.cls(e)); };
+        const auto reload = [&](int e) {
+            const int i = span.cls(e);
+            return order_key(ld(z, i), i);
+        };
+        if (a.splits == 1)
+            select_top<W, NE>(v, a.top, shared, key, reload, [&](int place, u64 k) {
+                a.top_logprobs[row * a.top + place] = log_prob(order_value((unsigned)(k >> 32)), r.m, a.inv_t, r.l2s);
+                a.top_classes[row * a.top + place] = (int)~(unsigned)k;
+            });
+        else
+            select_top<W, NE>(v, a.top, shared, key, reload, [&](int place, u64 k) { a.part_keys[unit * a.top + place] = k; });
+    }
+}
+
+// Joins the parts of a row: one unit of W waves, NE keys a thread.
+template <typename T, int W, int NE>
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __restrict__ logits, LogprobsArgs a) {
+    __shared__ TopShared<W> shared;
+    const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
+    const long long row = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+    if (row >= a.units) return;
+    if (a.live && !a.live[row]) {
+        dead_row<W>(a, row, tid);
+        return;
+    }
+    // (every wave for itself)
+    const Sums* part = a.part + row * a.splits;
+    float m = -INFINITY;
+    for (int i = lane; i < a.splits; i += 64) m = fmaxf(m, part[i].m);
+    Sums t{wave_max(m), 0.0f, 0.0f};
+    for (int i = lane; i < a.splits; i += 64) {
+        const Sums p = part[i];
+        if (p.s == 0.0f) continue;
+        const float d = (p.m - t.m) * a.c, f = __builtin_amdgcn_exp2f(d);
+        t.s += f * p.s;
+        t.u += f * (p.u + fmaxf(d, -1000.0f) * p.s);
+    }
+    t.s = wave_sum(t.s), t.u = wave_sum(t.u);
+    const RowStats r = row_stats(t, a.c_rel);
+    if (tid == 0) row_outputs(a, logits + row * a.row_stride, row, r);
+    if (a.top == 0) return;
+    const int n = a.splits * a.top;
+    const u64* keys = a.part_keys + row * n;
+    u64 k[NE];
+    float v[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+        const int i = e * W * 64 + tid;
+        k[e] = i < n ? keys[i] : 0ull;
+        v[e] = k[e] ? order_value((unsigned)(k[e] >> 32)) : -INFINITY;
+    }
+    select_top<W, NE>(
+        v, a.top, shared, [&](int e) { return k[e]; }, [&](int e) { return keys[e * W * 64 + tid]; },
+        [&](int place, u64 key) {
+            a.top_logprobs[row * a.top + place] = log_prob(order_value((unsigned)(key >> 32)), r.m, a.inv_t, r.l2s);
+            a.top_classes[row * a.top + place] = (int)~(unsigned)key;
+        });
+}
+
+// dlogits[c] = 1/T ([c = a] g_a + sum_j [c = i_j] g_j - p_c (g_a + sum_j g_j) - g_H p_c (log p_c + H)): the dense part
+// is written first, the few classes with a gradient of their own are written again behind it by the same unit.
+struct LogprobsBwdArgs {
+    const void* tokens;
+    const int* top_classes;
+    const float* stats;
+    const float* dlogprobs;
+    const float* dentropy;
+    const float* dtop;
+    long long row_stride, units;
+    int token_bytes, cols, splits, top;
+    float c, inv_t;
+};
+
+template <typename T, int W, int NE>
+__global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restrict__ logits, LogprobsBwdArgs a,
+                                                               T* __restrict__ dlogits) {
+    const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
+    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+    if (unit >= a.units) return;
+    const long long row = a.splits == 1 ? unit : unit / a.splits;
+    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    using S = Span<T, W, NE>;
+    const S span(split * S::kCols, a.cols, tid);
+    T* d = dlogits + row * a.cols;
+    const float m = a.stats[4 * row], l2s = a.stats[4 * row + 1], H = a.stats[4 * row + 2];
+    const bool zero = l2s == INFINITY;  // a dead row, or no class has probability: nothing to move
+    const T* z = logits + row * a.row_stride;
+    float v[NE];
+    if (!zero) span.template load<false>(z, v);
+    const float ga = a.dlogprobs ? a.dlogprobs[row] : 0.0f, gh = a.dentropy ? a.dentropy[row] : 0.0f;
+    const long long tok = a.dlogprobs ? class_at(a.tokens, a.token_bytes, row) : -1;
+    // (every wave for itself; top <= 64: one alternative a lane)
+    float gt = 0.0f;
+    int ti = -1;
+    if (a.dtop && lane < a.top) gt = a.dtop[row * a.top + lane], ti = a.top_classes[row * a.top + lane];
+    float g = a.dtop ? wave_sum(gt) + ga : ga;
+    if (a.dlogprobs && ga != 0.0f && (tok < 0 || tok >= a.cols)) g = NAN;  // a class the row does not have
+    const auto dense = [&](float zi) {
+        const float x = (zi - m) * a.c - l2s;
+        return -__builtin_amdgcn_exp2f(x) * (g + gh * (kLn2 * fmaxf(x, -1000.0f) + H));
+    };
+#pragma unroll
+    for (int t = 0; t < S::NV; ++t) {
+        if (span.empty(t)) break;
+        float o[S::VE];
+#pragma unroll
+        for (int j = 0; j < S::VE; ++j) o[j] = zero ? 0.0f : a.inv_t * dense(v[t * S::VE + j]);
+        span.store(d, t, o);
+    }
+    if (zero) return;
+    together<W>();
+    if (tid >= 64) return;
+    const int lo = span.base, hi = span.base + S::kCols < a.cols ? span.base + S::kCols : a.cols;
+    const bool both = __ballot(ti >= 0 && ti == tok) != 0;
+    if (ti >= lo && ti < hi) {
+        const float o = a.inv_t * (dense(ld(z, ti)) + gt + (ti == tok ? ga : 0.0f));
+        store_vector<1>(d + ti, &o);
+    }
+    if (lane == 0 && !both && tok >= lo && tok < hi) {
+        const float o = a.inv_t * (dense(ld(z, tok)) + ga);
+        store_vector<1>(d + tok, &o);
     }
 }
 
@@ -209,147 +591,400 @@ struct DistillStats {
     float mb, lb, coef, total, m, l2s, mv, lv;
 };
 
+// maximum and sum of powers of a row's classes outside the teacher's entries, and of the entries' own classes
+struct DistillPart {
+    float m, s, me, se;
+};
+
+struct DistillArgs {
+    const float* values;
+    const void* classes;
+    const unsigned char* live;
+    float* loss;
+    DistillStats* stats;
+    DistillPart* part;  // [rows][splits]
+    long long row_stride, units;
+    int class_bytes, cols, splits, k, tail;
+    float c, c_lo, inv_t;
+};
+
+// 2^((z - m) (c + c_lo)): log2(e) / T to twice a float's digits, as a rounded c shifts every exponent the same way
+__device__ __forceinline__ float power(float z, float m, float c, float c_lo) {
+    const float d = z - m;
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c_lo, d * c));
+}
+
 // A remaining mass that rounding alone can leave of the entries' log-probabilities (k of them, each good to 2^-24 of
 // its size): where the student has no class outside the entries it is no mass, anything above it has nowhere to go.
 constexpr float kNoMass = 1e-5f;
 
-constexpr int kMarkCols = 32768;  // columns marked at a time (4 KB of bits)
+// (m, s) of two disjoint parts
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float c, float c_lo) {
+    const float n = fmaxf(m, m2);
+    const float a = s == 0.0f ? 0.0f : s * power(m, n, c, c_lo), b = s2 == 0.0f ? 0.0f : s2 * power(m2, n, c, c_lo);
+    m = n, s = a + b;
+}
 
-// One workgroup per row.  loss = sum_j q_j (log q_j - log p_(i_j)), and with `tail` the mass outside the entries as one
-// more class: + q_r (log q_r - log p_r), where p_r is summed over those classes themselves (1 - sum would cancel).
+__device__ __forceinline__ void distill_dead(const DistillArgs& a, long long row) {
+    a.loss[row] = 0.0f;
+    if (a.stats) a.stats[row] = DistillStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, INFINITY, 0.0f, 0.0f};
+}
+
+// whether an earlier entry names the class as well
+__device__ bool named_before(const DistillArgs& a, long long row, int j, long long cls) {
+    for (int o = 0; o < j; ++o)
+        if (class_at(a.classes, a.class_bytes, row * a.k + o) == cls) return true;
+    return false;
+}
+
+// The loss of a row from its sums, by one wave.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_fwd_kernel(
-    const T* __restrict__ logits, long long row_stride, const float* __restrict__ values,
-    const void* __restrict__ classes, int class_bytes, const unsigned char* __restrict__ live, int cols, int k, float c,
-    float inv_t, int tail, float* __restrict__ loss, DistillStats* __restrict__ stats) {
-    __shared__ float red[kThreads / 64];
-    __shared__ unsigned marks[kMarkCols / 32];
-    const long long row = blockIdx.x;
-    const int tid = threadIdx.x;
-    if (live && !live[row]) {
-        if (tid == 0) {
-            loss[row] = 0.0f;
-            if (stats) stats[row] = DistillStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, INFINITY, 0.0f, 0.0f};
-        }
-        return;
-    }
-    const T* z = logits + row * row_stride;
-    const float* v = values + row * k;
-    float m = -INFINITY;
-    for (int i = tid; i < cols; i += kThreads) m = fmaxf(m, ld(z, i));
-    m = block_max(m, red);
-    if (m == -INFINITY) m = 0.0f;
+__device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z, long long row, const DistillPart& t) {
+    const int lane = threadIdx.x & 63;
+    const float* v = a.values + row * a.k;
+    float m = t.m, s = t.s;
+    if (a.tail) merge(m, s, t.me, t.se, a.c, a.c_lo);
+    m = m == -INFINITY ? 0.0f : m;
+    const float l2s = s == 0.0f ? INFINITY : __builtin_amdgcn_logf(s);
     // the teacher's distribution over its entries
-    float mv = 0.0f, lv = 0.0f, bad = 0.0f;
-    const float cv = tail ? kLog2e : c;
-    if (!tail) {
+    const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? (float)(1.4426950408889634074 - (double)kLog2e) : a.c_lo;
+    float mv = 0.0f, lv = 0.0f, bad = 0.0f, sv = 0.0f;
+    if (!a.tail) {
         mv = -INFINITY;
-        for (int j = tid; j < k; j += kThreads)
-            if (class_at(classes, class_bytes, row * k + j) >= 0) mv = fmaxf(mv, v[j]);
-        mv = block_max(mv, red);
+        for (int j = lane; j < a.k; j += 64)
+            if (class_at(a.classes, a.class_bytes, row * a.k + j) >= 0) mv = fmaxf(mv, v[j]);
+        mv = wave_max(mv);
         if (mv == -INFINITY) mv = 0.0f;
     }
-    float sv = 0.0f;
-    for (int j = tid; j < k; j += kThreads) {
-        const long long i = class_at(classes, class_bytes, row * k + j);
-        if (i >= 0) sv += exp2f((v[j] - mv) * cv);
-        if (i >= cols) bad = 1.0f;
+    for (int j = lane; j < a.k; j += 64) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i >= 0) sv += power(v[j], mv, cv, cv_lo);
+        if (i >= a.cols) bad = 1.0f;
     }
-    sv = block_sum(sv, red);
-    bad = block_max(bad, red);
-    if (!tail) lv = sv == 0.0f ? INFINITY : log2f(sv);
-    const float qsum = tail ? sv : (sv == 0.0f ? 0.0f : 1.0f);
-    float qr = tail ? fmaxf(1.0f - sv, 0.0f) : 0.0f;
-    // the student's sums: over every class, and over the classes outside the entries
-    float s = 0.0f, mr = -INFINITY, sr = 0.0f;
-    for (int base = 0; base < cols; base += kMarkCols) {
-        const int end = base + kMarkCols < cols ? base + kMarkCols : cols;
-        if (tail) {
-            __syncthreads();
-            for (int i = tid; i < kMarkCols / 32; i += kThreads) marks[i] = 0u;
-            __syncthreads();
-            for (int j = tid; j < k; j += kThreads) {
-                const long long i = class_at(classes, class_bytes, row * k + j);
-                if (i >= base && i < end) atomicOr(&marks[(i - base) >> 5], 1u << ((i - base) & 31));
-            }
-            __syncthreads();
-        }
-        for (int i = base + tid; i < end; i += kThreads) {
-            const float zi = ld(z, i);
-            s += exp2f((zi - m) * c);
-            if (tail && !(marks[(i - base) >> 5] >> ((i - base) & 31) & 1u)) {
-                if (zi > mr) sr = sr * exp2f((mr - zi) * c) + 1.0f, mr = zi;
-                else if (zi != -INFINITY) sr += exp2f((zi - mr) * c);
-            }
-        }
-    }
-    s = block_sum(s, red);
-    const float l2s = s == 0.0f ? INFINITY : log2f(s);
-    float lr = INFINITY;
-    if (tail) {
-        const float gm = block_max(mr, red);
-        const float scale = mr == -INFINITY ? 0.0f : exp2f((mr - gm) * c);
-        sr = block_sum(sr * scale, red);
-        mr = gm == -INFINITY ? 0.0f : gm;
-        lr = sr == 0.0f ? INFINITY : log2f(sr);
-    }
+    sv = wave_sum(sv);
+    if (!a.tail) lv = sv == 0.0f ? INFINITY : __builtin_amdgcn_logf(sv);
+    const float qsum = a.tail ? sv : (sv == 0.0f ? 0.0f : 1.0f);
+    float qr = a.tail ? fmaxf(1.0f - sv, 0.0f) : 0.0f;
     float l = 0.0f;
-    for (int j = tid; j < k; j += kThreads) {
-        const long long i = class_at(classes, class_bytes, row * k + j);
-        if (i < 0 || i >= cols) continue;
-        const float q = exp2f((v[j] - mv) * cv - lv);
-        const float lq = (v[j] - mv) * (tail ? 1.0f : inv_t) - kLn2 * lv;
-        if (q != 0.0f) l += q * (lq - log_prob(ld(z, i), m, inv_t, l2s));
+    for (int j = lane; j < a.k; j += 64) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < 0 || i >= a.cols) continue;
+        const float q = power(v[j], mv, cv, cv_lo) * __builtin_amdgcn_exp2f(-lv);
+        const float lq = (v[j] - mv) * (a.tail ? 1.0f : a.inv_t) - kLn2 * lv;
+        if (q != 0.0f) l += q * (lq - log_prob(ld(z, i), m, a.inv_t, l2s));
     }
-    l = block_sum(l, red);
-    if (tid == 0) {
+    l = wave_sum(l);
+    bad = wave_max(bad);
+    if (lane == 0) {
         float coef = qsum, mb = m, lb = l2s;
-        if (tail) {
-            const float lpr = (mr - m) * c + lr - l2s;  // log2 of the student's mass outside
-            const bool none = lr == INFINITY;
+        if (a.tail) {
+            const bool none = t.s == 0.0f;
+            const float mr = t.m == -INFINITY ? 0.0f : t.m, lr = none ? INFINITY : __builtin_amdgcn_logf(t.s);
             if (none && qr <= kNoMass) qr = 0.0f;
-            if (qr > 0.0f) l += none ? INFINITY : qr * kLn2 * (log2f(qr) - lpr);
-            coef = none ? 0.0f : (qsum + qr) * exp2f(lpr) - qr;
+            // log2 of the student's mass outside
+            const float lpr = __builtin_fmaf(mr - m, a.c_lo, (mr - m) * a.c) + (lr - l2s);
+            if (qr > 0.0f) l += none ? INFINITY : qr * kLn2 * (__builtin_amdgcn_logf(qr) - lpr);
+            coef = none ? 0.0f : (qsum + qr) * __builtin_amdgcn_exp2f(lpr) - qr;
             mb = mr, lb = lr;
         }
         if (bad != 0.0f) l = NAN, coef = NAN;
-        loss[row] = l;
-        if (stats) stats[row] = DistillStats{mb, lb, coef, qsum + qr, m, l2s, mv, lv};
+        a.loss[row] = l;
+        if (a.stats) a.stats[row] = DistillStats{mb, lb, coef, qsum + qr, m, l2s, mv, lv};
+    }
+}
+
+// loss = sum_j q_j (log q_j - log p_(i_j)), and with TAIL the mass outside the entries as one more class:
+// + q_r (log q_r - log p_r), where p_r is summed over those classes themselves (1 - sum would cancel).  For that every
+// thread gets one bit per element of its own that an entry names, through LDS, and blanks those elements; the entries'
+// own classes are summed from a second look at them.
+template <typename T, int W, int NE, bool TAIL>
+__global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restrict__ logits, DistillArgs a) {
+    __shared__ DistillPart red[W];
+    __shared__ unsigned marks[TAIL ? kThreads : 1];
+    __shared__ unsigned repeated;
+    const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
+    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+    if (unit >= a.units) return;
+    const long long row = a.splits == 1 ? unit : unit / a.splits;
+    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    if (a.live && !a.live[row]) {
+        if (tid == 0 && a.splits == 1) distill_dead(a, row);
+        return;
+    }
+    const T* z = logits + row * a.row_stride;
+    using S = Span<T, W, NE>;
+    const S span(split * S::kCols, a.cols, tid);
+    float v[NE];
+    span.template load<true>(z, v);
+    DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    if constexpr (TAIL) {
+        unsigned* mine = marks + (W == 1 ? threadIdx.x - lane : 0);
+        mine[tid] = 0u;
+        if (W > 1 && tid == 0) repeated = 0u;
+        together<W>();
+        const int hi = span.base + S::kCols < a.cols ? span.base + S::kCols : a.cols;
+        bool twice = false;
+        for (int j = tid; j < a.k; j += W * 64) {
+            const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+            if (i < span.base || i >= hi) continue;
+            int thread, e;
+            span.locate((int)i, thread, e);
+            twice |= (atomicOr(&mine[thread], 1u << e) >> e & 1u) != 0;
+        }
+        if constexpr (W == 1) {
+            twice = __ballot(twice) != 0;
+        } else {
+            if (twice) repeated = 1u;
+        }
+        together<W>();
+        if constexpr (W > 1) twice = repeated != 0;
+        const unsigned hit = mine[tid];
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] = hit >> e & 1u ? -INFINITY : v[e];
+        for (int j = tid; j < a.k; j += W * 64) {
+            const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+            if (i < span.base || i >= hi) continue;
+            if (twice && named_before(a, row, j, i)) continue;
+            const float zi = ld(z, i);
+            merge(t.me, t.se, zi, zi == -INFINITY ? 0.0f : 1.0f, a.c, a.c_lo);
+        }
+        const float m = wave_max(t.me);
+        t.se = wave_sum(t.se == 0.0f ? 0.0f : t.se * power(t.me, m, a.c, a.c_lo));
+        t.me = m;
+    }
+    float m = v[0];
+#pragma unroll
+    for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
+    t.m = wave_max(m);
+    const float mz = t.m == -INFINITY ? 0.0f : t.m;
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s += power(v[e], mz, a.c, a.c_lo);
+    t.s = wave_sum(s);
+    if constexpr (W > 1) {
+        if (lane == 0) red[threadIdx.x >> 6] = t;
+        together<W>();
+        if (tid >= 64) return;
+        t = red[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            merge(t.m, t.s, red[w].m, red[w].s, a.c, a.c_lo);
+            if constexpr (TAIL) merge(t.me, t.se, red[w].me, red[w].se, a.c, a.c_lo);
+        }
+    }
+    if (a.splits == 1)
+        distill_finish(a, z, row, t);
+    else if (lane == 0)
+        a.part[unit] = t;
+}
+
+// Joins the parts of a row: one wave.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void distill_join_kernel(const T* __restrict__ logits, DistillArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long row = block_index() * 4 + (threadIdx.x >> 6);
+    if (row >= a.units) return;
+    if (a.live && !a.live[row]) {
+        if (lane == 0) distill_dead(a, row);
+        return;
+    }
+    DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    for (int i = lane; i < a.splits; i += 64) {
+        const DistillPart p = a.part[row * a.splits + i];
+        merge(t.m, t.s, p.m, p.s, a.c, a.c_lo);
+        merge(t.me, t.se, p.me, p.se, a.c, a.c_lo);
+    }
+    const float m = wave_max(t.m), me = wave_max(t.me);
+    t.s = wave_sum(t.s == 0.0f ? 0.0f : t.s * power(t.m, m, a.c, a.c_lo));
+    t.se = wave_sum(t.se == 0.0f ? 0.0f : t.se * power(t.me, me, a.c, a.c_lo));
+    t.m = m, t.me = me;
+    distill_finish(a, logits + row * a.row_stride, row, t);
+}
+
+struct DistillBwdArgs {
+    const float* values;
+    const void* classes;
+    const DistillStats* stats;
+    const float* dloss;
+    long long row_stride, units;
+    int class_bytes, cols, splits, k, tail;
+    float c, inv_t;
+};
+
+template <typename T, int W, int NE>
+__global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restrict__ logits, DistillBwdArgs a,
+                                                              T* __restrict__ dlogits) {
+    __shared__ unsigned marks[kThreads];
+    __shared__ unsigned repeated;
+    const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
+    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+    if (unit >= a.units) return;
+    const long long row = a.splits == 1 ? unit : unit / a.splits;
+    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    using S = Span<T, W, NE>;
+    const S span(split * S::kCols, a.cols, tid);
+    T* d = dlogits + row * a.cols;
+    const DistillStats st = a.stats[row];
+    const bool zero = st.l2s == INFINITY;  // a dead row, or no class has probability
+    const T* z = logits + row * a.row_stride;
+    float v[NE];
+    if (!zero) span.template load<false>(z, v);
+    const float g = a.dloss[row] * a.inv_t;
+    // (no class outside the entries has probability: lb = +inf, and the powers come out as 0 from a finite mb)
+    const float gc = g * st.coef;
+#pragma unroll
+    for (int t = 0; t < S::NV; ++t) {
+        if (span.empty(t)) break;
+        float o[S::VE];
+#pragma unroll
+        for (int j = 0; j < S::VE; ++j)
+            o[j] = zero ? 0.0f : gc * __builtin_amdgcn_exp2f((v[t * S::VE + j] - st.mb) * a.c - st.lb);
+        span.store(d, t, o);
+    }
+    if (zero || st.coef != st.coef) return;  // (NaN: an entry the row does not have; the whole row is)
+    // the entries' classes once more, behind the dense part
+    const int lo = span.base, hi = span.base + S::kCols < a.cols ? span.base + S::kCols : a.cols;
+    unsigned* mine = marks + (W == 1 ? threadIdx.x - lane : 0);
+    mine[tid] = 0u;
+    if (W > 1 && tid == 0) repeated = 0u;
+    together<W>();
+    bool twice = false;
+    for (int j = tid; j < a.k; j += W * 64) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < lo || i >= hi) continue;
+        int thread, e;
+        span.locate((int)i, thread, e);
+        twice |= (atomicOr(&mine[thread], 1u << e) >> e & 1u) != 0;
+    }
+    if constexpr (W == 1) {
+        twice = __ballot(twice) != 0;
+    } else {
+        if (twice) repeated = 1u;
+        together<W>();
+        twice = repeated != 0;
+    }
+    const float cv = a.tail ? kLog2e : a.c;
+    for (int j = tid; j < a.k; j += W * 64) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < lo || i >= hi) continue;
+        float q = __builtin_amdgcn_exp2f((a.values[row * a.k + j] - st.mv) * cv - st.lv);
+        if (twice) {  // (every place of the class writes the same sum)
+            q = 0.0f;
+            for (int o = 0; o < a.k; ++o)
+                if (class_at(a.classes, a.class_bytes, row * a.k + o) == i)
+                    q += __builtin_amdgcn_exp2f((a.values[row * a.k + o] - st.mv) * cv - st.lv);
+        }
+        const float p = __builtin_amdgcn_exp2f((ld(z, i) - st.m) * a.c - st.l2s);
+        const float o = g * (st.total * p - q);
+        store_vector<1>(d + i, &o);
+    }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------
+// How a row is cut: one wave for up to kWaveCols classes; beyond, workgroups of 256 threads with 32, 16 or 8 classes a
+// thread - the most that still leaves kUnits workgroups (four for each of the 256 CUs) for few rows.
+constexpr long long kUnits = 1024;
+constexpr int kMaxSplits = kMaxCols / (kThreads * 32);
+struct Cut {
+    int waves, ne, splits;
+};
+Cut cut_rows(long long rows, int cols) {
+    if (cols <= kWaveCols) {
+        int ne = 1;
+        while (64 * ne < cols) ne *= 2;
+        if (ne == 32 && cols <= 64 * 24) ne = 24;
+        return Cut{1, ne, 1};
+    }
+    for (int ne = 8;; ne *= 2) {
+        const int splits = (cols + kThreads * ne - 1) / (kThreads * ne);
+        const int half = (cols + kThreads * 2 * ne - 1) / (kThreads * 2 * ne);
+        if (ne == 32 || (splits <= kMaxSplits && rows * half < kUnits)) return Cut{4, ne, splits};
+    }
+}
+
+dim3 grid_of(long long units, int waves) {
+    const long long blocks = waves == 1 ? (units + 3) / 4 : units;
+    const long long x = blocks < (1 << 20) ? blocks : (1 << 20);
+    return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+
+// F::template run<W, NE>(...) for a cut
+template <typename F, typename... A>
+void with_cut(const Cut& cut, A&&... args) {
+    if (cut.waves == 4) {
+        if (cut.ne == 8) F::template run<4, 8>(args...);
+        else if (cut.ne == 16) F::template run<4, 16>(args...);
+        else F::template run<4, 32>(args...);
+    } else {
+        switch (cut.ne) {
+            case 1: F::template run<1, 1>(args...); break;
+            case 2: F::template run<1, 2>(args...); break;
+            case 4: F::template run<1, 4>(args...); break;
+            case 8: F::template run<1, 8>(args...); break;
+            case 16: F::template run<1, 16>(args...); break;
+            case 24: F::template run<1, 24>(args...); break;
+            default: F::template run<1, 32>(args...);
+        }
     }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
-    const T* __restrict__ logits, long long row_stride, const float* __restrict__ values,
-    const void* __restrict__ classes, int class_bytes, const DistillStats* __restrict__ stats,
-    const float* __restrict__ dloss, int cols, int k, float c, float inv_t, int tail, T* __restrict__ dlogits) {
-    const long long row = blockIdx.x;
-    const int tid = threadIdx.x;
-    T* d = dlogits + row * cols;
-    const DistillStats st = stats[row];
-    if (st.l2s == INFINITY) {  // dead, or no class has probability
-        for (int i = tid; i < cols; i += kThreads) d[i] = (T)0.0f;
-        return;
+struct LogprobsFwd {
+    template <int W, int NE>
+    static void run(const void* logits, const LogprobsArgs& a, hipStream_t s) {
+        if (a.top > 0)
+            hipLaunchKernelGGL((logprobs_fwd_kernel<T, W, NE, true>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                               static_cast<const T*>(logits), a);
+        else
+            hipLaunchKernelGGL((logprobs_fwd_kernel<T, W, NE, false>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                               static_cast<const T*>(logits), a);
     }
-    const T* z = logits + row * row_stride;
-    const float g = dloss[row] * inv_t;
-    for (int i = tid; i < cols; i += kThreads) {
-        // (no class outside the entries has probability: lb = +inf and the product is 0)
-        const float p = st.lb == INFINITY ? 0.0f : exp2f((ld(z, i) - st.mb) * c - st.lb);
-        d[i] = (T)(g * (st.coef * p));
+};
+template <typename T>
+struct LogprobsJoin {
+    template <int W, int NE>
+    static void run(const void* logits, const LogprobsArgs& a, hipStream_t s) {
+        hipLaunchKernelGGL((logprobs_join_kernel<T, W, NE>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits), a);
     }
-    __syncthreads();
-    const float cv = tail ? kLog2e : c;
-    if (st.coef != st.coef) return;  // an entry the row does not have: the row is NaN
-    for (int j = tid; j < k; j += kThreads) {
-        const long long i = class_at(classes, class_bytes, row * k + j);
-        if (i < 0 || i >= cols) continue;
-        float q = 0.0f;
-        for (int o = 0; o < k; ++o)
-            if (class_at(classes, class_bytes, row * k + o) == i) q += exp2f((values[row * k + o] - st.mv) * cv - st.lv);
-        const float p = exp2f((ld(z, i) - st.m) * c - st.l2s);
-        d[i] = (T)(g * (st.total * p - q));
+};
+template <typename T>
+struct LogprobsBwd {
+    template <int W, int NE>
+    static void run(const void* logits, const LogprobsBwdArgs& a, void* dlogits, hipStream_t s) {
+        hipLaunchKernelGGL((logprobs_bwd_kernel<T, W, NE>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits), a, static_cast<T*>(dlogits));
     }
+};
+template <typename T>
+struct DistillFwd {
+    template <int W, int NE>
+    static void run(const void* logits, const DistillArgs& a, hipStream_t s) {
+        if (a.tail)
+            hipLaunchKernelGGL((distill_fwd_kernel<T, W, NE, true>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                               static_cast<const T*>(logits), a);
+        else
+            hipLaunchKernelGGL((distill_fwd_kernel<T, W, NE, false>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                               static_cast<const T*>(logits), a);
+    }
+};
+template <typename T>
+struct DistillBwd {
+    template <int W, int NE>
+    static void run(const void* logits, const DistillBwdArgs& a, void* dlogits, hipStream_t s) {
+        hipLaunchKernelGGL((distill_bwd_kernel<T, W, NE>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits), a, static_cast<T*>(dlogits));
+    }
+};
+
+// The keys of a row's parts: one wave while they fit its registers.
+Cut cut_keys(int n) {
+    if (n <= 64 * 32) {
+        int ne = 4;
+        while (64 * ne < n) ne *= 2;
+        return Cut{1, ne, 1};
+    }
+    return Cut{4, n <= kThreads * 16 ? 16 : 32, 1};
 }
 
 int check_call(const char* who, long long row_stride, int rows, int cols, int dtype, float temperature) {
@@ -366,75 +1001,116 @@ int check_bytes(const char* who, const void* classes, int bytes) {
     return ISG_OK;
 }
 
-}  // namespace
-
-extern "C" int isg_token_logprobs_fwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
-                                      const unsigned char* live, int rows, int cols, int dtype, float temperature,
-                                      int top, float* logprobs, float* entropy, float* top_logprobs,
-                                      int32_t* top_classes, float* stats, void* stream) {
-    const char* who = "isg_token_logprobs_fwd";
-    int rc = check_call(who, row_stride, rows, cols, dtype, temperature);
-    if (rc != ISG_OK) return rc;
-    rc = check_bytes(who, tokens, token_bytes);
-    if (rc != ISG_OK) return rc;
+int check_top(const char* who, int top, int cols) {
     ISG_REQUIRE(top >= 0 && top <= kMaxTop && top <= cols, ISG_EINVAL, "%s: top=%d of %d classes (at most %d)", who, top, cols,
                 kMaxTop);
-    if (rows == 0) return ISG_OK;
-    ISG_REQUIRE(logits && entropy && (!tokens || logprobs) && (top == 0 || (top_logprobs && top_classes)), ISG_EINVAL,
-                "%s: null pointer", who);
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const float c = kLog2e / temperature, inv_t = 1.0f / temperature;
-    if (dtype == ISG_F32)
-        hipLaunchKernelGGL(logprobs_fwd_kernel<float>, dim3(rows), dim3(kThreads), 0, s, static_cast<const float*>(logits),
-                           row_stride, tokens, token_bytes, live, cols, c, inv_t, top, logprobs, entropy, top_logprobs, top_classes,
-                           stats);
-    else
-        hipLaunchKernelGGL(logprobs_fwd_kernel<__hip_bfloat16>, dim3(rows), dim3(kThreads), 0, s,
-                           static_cast<const __hip_bfloat16*>(logits), row_stride, tokens, token_bytes, live, cols, c, inv_t, top,
-                           logprobs, entropy, top_logprobs, top_classes, stats);
-    return isg::check_launch("logprobs_fwd_kernel");
+    return ISG_OK;
 }
 
-extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
-                                      const unsigned char* live, const int32_t* top_classes, const float* stats,
-                                      const float* dlogprobs, const float* dentropy, const float* dtop_logprobs, int rows,
-                                      int cols, int dtype, float temperature, int top, void* dlogits, void* stream) {
-    const char* who = "isg_token_logprobs_bwd";
-    int rc = check_call(who, row_stride, rows, cols, dtype, temperature);
-    if (rc != ISG_OK) return rc;
-    rc = check_bytes(who, tokens, token_bytes);
-    if (rc != ISG_OK) return rc;
-    ISG_REQUIRE(top >= 0 && top <= kMaxTop && top <= cols, ISG_EINVAL, "%s: top=%d of %d classes (at most %d)", who, top, cols,
-                kMaxTop);
-    if (rows == 0) return ISG_OK;
-    ISG_REQUIRE(logits && stats && dlogits && (!dlogprobs || tokens) && (!dtop_logprobs || (top > 0 && top_classes)),
-                ISG_EINVAL, "%s: null pointer", who);
-    ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const float c = kLog2e / temperature, inv_t = 1.0f / temperature;
-    if (dtype == ISG_F32)
-        hipLaunchKernelGGL(logprobs_bwd_kernel<float>, dim3(rows), dim3(kThreads), 0, s, static_cast<const float*>(logits),
-                           row_stride, tokens, token_bytes, live, top_classes, stats, dlogprobs, dentropy, dtop_logprobs,
-                           cols, c, inv_t, top, static_cast<float*>(dlogits));
-    else
-        hipLaunchKernelGGL(logprobs_bwd_kernel<__hip_bfloat16>, dim3(rows), dim3(kThreads), 0, s,
-                           static_cast<const __hip_bfloat16*>(logits), row_stride, tokens, token_bytes, live, top_classes,
-                           stats, dlogprobs, dentropy, dtop_logprobs, cols, c, inv_t, top,
-                           static_cast<__hip_bfloat16*>(dlogits));
-    return isg::check_launch("logprobs_bwd_kernel");
-}
-
-namespace {
 int check_entries(const char* who, int k, int tail) {
     ISG_REQUIRE(k >= 1 && k <= kMaxEntries, ISG_EINVAL, "%s: k=%d classes of the teacher (1 to %d)", who, k, kMaxEntries);
     ISG_REQUIRE(tail == 0 || tail == 1, ISG_EINVAL, "%s: tail=%d", who, tail);
     return ISG_OK;
 }
+
+// log2(e) / T as the float below it and what is missing, which is positive (an infinite distance times both parts is an
+// infinity of one sign)
+void scale_of(float temperature, float& c, float& c_lo, float& inv_t) {
+    const double exact = 1.4426950408889634074 / (double)temperature;
+    c = (float)exact;
+    if ((double)c >= exact) c = nextafterf(c, 0.0f);
+    c_lo = (float)(exact - (double)c);
+    inv_t = (float)(1.0 / (double)temperature);
+}
+
 }  // namespace
+
+extern "C" long long isg_token_logprobs_workspace_bytes(int rows, int cols, int top) {
+    if (rows < 0 || cols < 1 || cols > kMaxCols || top < 0 || top > kMaxTop) return -1;
+    const Cut cut = cut_rows(rows, cols);
+    return cut.splits == 1 ? 0 : (long long)rows * cut.splits * ((long long)sizeof(Sums) + 8 * top) + 8;
+}
+
+extern "C" int isg_token_logprobs_fwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
+                                      const unsigned char* live, int rows, int cols, int dtype, float temperature,
+                                      int top, float* logprobs, float* entropy, float* top_logprobs,
+                                      int32_t* top_classes, float* stats, void* workspace, void* stream) {
+    const char* who = "isg_token_logprobs_fwd";
+    int rc = check_call(who, row_stride, rows, cols, dtype, temperature);
+    if (rc != ISG_OK) return rc;
+    rc = check_bytes(who, tokens, token_bytes);
+    if (rc != ISG_OK) return rc;
+    rc = check_top(who, top, cols);
+    if (rc != ISG_OK) return rc;
+    if (rows == 0) return ISG_OK;
+    ISG_REQUIRE(logits && entropy && (!tokens || logprobs) && (top == 0 || (top_logprobs && top_classes)), ISG_EINVAL,
+                "%s: null pointer", who);
+    const Cut cut = cut_rows(rows, cols);
+    ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
+    ISG_REQUIRE(((uintptr_t)workspace | (uintptr_t)stats) % 8 == 0 && (uintptr_t)stats % 16 == 0, ISG_EINVAL,
+                "%s: workspace and stats must be aligned to 8 and 16 bytes", who);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    LogprobsArgs a{};
+    a.tokens = tokens, a.live = live, a.logprobs = tokens ? logprobs : nullptr, a.entropy = entropy;
+    a.top_logprobs = top_logprobs, a.top_classes = top_classes, a.stats = stats;
+    a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
+    a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.top = top;
+    float c_lo;
+    scale_of(temperature, a.c, c_lo, a.inv_t);
+    a.c_rel = c_lo / a.c;
+    if (cut.splits > 1) {
+        a.part_keys = static_cast<u64*>(workspace);
+        a.part = reinterpret_cast<Sums*>(a.part_keys + a.units * top);
+    }
+    if (dtype == ISG_F32) with_cut<LogprobsFwd<float>>(cut, logits, a, s);
+    else with_cut<LogprobsFwd<__hip_bfloat16>>(cut, logits, a, s);
+    rc = isg::check_launch("logprobs_fwd_kernel");
+    if (rc != ISG_OK || cut.splits == 1) return rc;
+    a.units = rows;
+    const Cut join = cut_keys(cut.splits * top);
+    if (dtype == ISG_F32) with_cut<LogprobsJoin<float>>(join, logits, a, s);
+    else with_cut<LogprobsJoin<__hip_bfloat16>>(join, logits, a, s);
+    return isg::check_launch("logprobs_join_kernel");
+}
+
+extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
+                                      const int32_t* top_classes, const float* stats, const float* dlogprobs,
+                                      const float* dentropy, const float* dtop_logprobs, int rows, int cols, int dtype,
+                                      float temperature, int top, void* dlogits, void* stream) {
+    const char* who = "isg_token_logprobs_bwd";
+    int rc = check_call(who, row_stride, rows, cols, dtype, temperature);
+    if (rc != ISG_OK) return rc;
+    rc = check_bytes(who, tokens, token_bytes);
+    if (rc != ISG_OK) return rc;
+    rc = check_top(who, top, cols);
+    if (rc != ISG_OK) return rc;
+    if (rows == 0) return ISG_OK;
+    ISG_REQUIRE(logits && stats && dlogits && (!dlogprobs || tokens) && (!dtop_logprobs || (top > 0 && top_classes)),
+                ISG_EINVAL, "%s: null pointer", who);
+    ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
+    const Cut cut = cut_rows(rows, cols);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    LogprobsBwdArgs a{};
+    a.tokens = tokens, a.top_classes = top_classes, a.stats = stats;
+    a.dlogprobs = dlogprobs, a.dentropy = dentropy, a.dtop = dtop_logprobs;
+    a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
+    a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.top = top;
+    float c_lo;
+    scale_of(temperature, a.c, c_lo, a.inv_t);
+    if (dtype == ISG_F32) with_cut<LogprobsBwd<float>>(cut, logits, a, dlogits, s);
+    else with_cut<LogprobsBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
+    return isg::check_launch("logprobs_bwd_kernel");
+}
+
+extern "C" long long isg_distill_workspace_bytes(int rows, int cols) {
+    if (rows < 0 || cols < 1 || cols > kMaxCols) return -1;
+    const Cut cut = cut_rows(rows, cols);
+    return cut.splits == 1 ? 0 : (long long)rows * cut.splits * (long long)sizeof(DistillPart);
+}
 
 extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const float* values, const void* classes,
                                int class_bytes, const unsigned char* live, int rows, int cols, int k, int dtype,
-                               float temperature, int tail, float* loss, float* stats, void* stream) {
+                               float temperature, int tail, float* loss, float* stats, void* workspace, void* stream) {
     const char* who = "isg_distill_fwd";
     int rc = check_call(who, row_stride, rows, cols, dtype, temperature);
     if (rc != ISG_OK) return rc;
@@ -444,17 +1120,27 @@ extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const f
     if (rc != ISG_OK) return rc;
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && loss, ISG_EINVAL, "%s: null pointer", who);
+    const Cut cut = cut_rows(rows, cols);
+    ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const float c = kLog2e / temperature, inv_t = 1.0f / temperature;
-    DistillStats* st = reinterpret_cast<DistillStats*>(stats);
+    DistillArgs a{};
+    a.values = values, a.classes = classes, a.live = live, a.loss = loss;
+    a.stats = reinterpret_cast<DistillStats*>(stats), a.part = static_cast<DistillPart*>(workspace);
+    a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
+    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.k = k, a.tail = tail;
+    scale_of(temperature, a.c, a.c_lo, a.inv_t);
+    if (dtype == ISG_F32) with_cut<DistillFwd<float>>(cut, logits, a, s);
+    else with_cut<DistillFwd<__hip_bfloat16>>(cut, logits, a, s);
+    rc = isg::check_launch("distill_fwd_kernel");
+    if (rc != ISG_OK || cut.splits == 1) return rc;
+    a.units = rows;
     if (dtype == ISG_F32)
-        hipLaunchKernelGGL(distill_fwd_kernel<float>, dim3(rows), dim3(kThreads), 0, s, static_cast<const float*>(logits),
-                           row_stride, values, classes, class_bytes, live, cols, k, c, inv_t, tail, loss, st);
+        hipLaunchKernelGGL(distill_join_kernel<float>, grid_of(rows, 1), dim3(kThreads), 0, s,
+                           static_cast<const float*>(logits), a);
     else
-        hipLaunchKernelGGL(distill_fwd_kernel<__hip_bfloat16>, dim3(rows), dim3(kThreads), 0, s,
-                           static_cast<const __hip_bfloat16*>(logits), row_stride, values, classes, class_bytes, live, cols,
-                           k, c, inv_t, tail, loss, st);
-    return isg::check_launch("distill_fwd_kernel");
+        hipLaunchKernelGGL(distill_join_kernel<__hip_bfloat16>, grid_of(rows, 1), dim3(kThreads), 0, s,
+                           static_cast<const __hip_bfloat16*>(logits), a);
+    return isg::check_launch("distill_join_kernel");
 }
 
 extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const float* values, const void* classes,
@@ -470,16 +1156,15 @@ extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const f
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && stats && dloss && dlogits, ISG_EINVAL, "%s: null pointer", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
+    const Cut cut = cut_rows(rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const float c = kLog2e / temperature, inv_t = 1.0f / temperature;
-    const DistillStats* st = reinterpret_cast<const DistillStats*>(stats);
-    if (dtype == ISG_F32)
-        hipLaunchKernelGGL(distill_bwd_kernel<float>, dim3(rows), dim3(kThreads), 0, s, static_cast<const float*>(logits),
-                           row_stride, values, classes, class_bytes, st, dloss, cols, k, c, inv_t, tail,
-                           static_cast<float*>(dlogits));
-    else
-        hipLaunchKernelGGL(distill_bwd_kernel<__hip_bfloat16>, dim3(rows), dim3(kThreads), 0, s,
-                           static_cast<const __hip_bfloat16*>(logits), row_stride, values, classes, class_bytes, st, dloss,
-                           cols, k, c, inv_t, tail, static_cast<__hip_bfloat16*>(dlogits));
+    DistillBwdArgs a{};
+    a.values = values, a.classes = classes, a.stats = reinterpret_cast<const DistillStats*>(stats), a.dloss = dloss;
+    a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
+    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.k = k, a.tail = tail;
+    float c_lo;
+    scale_of(temperature, a.c, c_lo, a.inv_t);
+    if (dtype == ISG_F32) with_cut<DistillBwd<float>>(cut, logits, a, dlogits, s);
+    else with_cut<DistillBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
     return isg::check_launch("distill_bwd_kernel");
 }

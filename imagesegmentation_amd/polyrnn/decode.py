@@ -220,24 +220,51 @@ def _temperature(value, what):
 def _on_device(t):
     """The kernels launch on the current device's stream: for a tensor of another device that one is made current."""
     if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _here
     return torch.cuda.device(t.device)
+
+
+_here = contextlib.nullcontext()
+
+
+_ONE_UNIT_CLASSES = 2048  # rows up to here take no workspace
 
 
 def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
     rows, cols, stride = geometry
-    new = lambda shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=z.device)
-    logp = new([rows]) if tokens is not None else None
-    entropy = new([rows])
-    top_logp, top_cls = (new([rows, top]), new([rows, top], torch.int32)) if top else (None, None)
-    stats = new([rows, 4]) if keep else None
+    lib, dev = _lib.lib(), z.device
+    f32 = torch.float32
+    entropy = torch.empty([rows], dtype=f32, device=dev)
+    logp = torch.empty([rows], dtype=f32, device=dev) if tokens is not None else None
+    top_logp = top_cls = stats = space = None
+    if top:
+        top_logp = torch.empty([rows, top], dtype=f32, device=dev)
+        top_cls = torch.empty([rows, top], dtype=torch.int32, device=dev)
+    if keep:
+        stats = torch.empty([rows, 4], dtype=f32, device=dev)
+    if cols > _ONE_UNIT_CLASSES:
+        space = torch.empty([lib.isg_token_logprobs_workspace_bytes(rows, cols, top)], dtype=torch.uint8, device=dev)
     with _on_device(z):
-        rc = _lib.lib().isg_token_logprobs_fwd(
+        rc = lib.isg_token_logprobs_fwd(
             z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4, _lib.ptr(live),
-            rows, cols, dtype_code(z.dtype), temperature, top, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(top_logp),
-            _lib.ptr(top_cls), _lib.ptr(stats), _lib.current_stream())
-    _lib.check(rc, "isg_token_logprobs_fwd")
+            rows, cols, dtype_code(z.dtype), temperature, top, _lib.ptr(logp), entropy.data_ptr(), _lib.ptr(top_logp),
+            _lib.ptr(top_cls), _lib.ptr(stats), _lib.ptr(space), _lib.stream_of(z))
+    if rc:
+        _lib.check(rc, "isg_token_logprobs_fwd")
     return logp, entropy, top_logp, top_cls, stats
+
+
+def _like_input(dz, shape, dtype):
+    """A gradient [rows, classes] in the logits' shape and type."""
+    if dz.shape != shape:
+        dz = dz.reshape(shape)
+    return dz if dz.dtype == dtype else dz.to(dtype)
+
+
+def _float_gradient(g):
+    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -246,7 +273,7 @@ class _TokenLogprobs(torch.autograd.Function):
         z, rows, cols, stride = _class_rows(logits, "token_logprobs")
         logp, entropy, top_logp, top_cls, stats = _logprobs_forward(z, (rows, cols, stride), tokens, live, top,
                                                                     temperature, True)
-        ctx.save_for_backward(z, tokens, live, top_cls, stats)
+        ctx.save_for_backward(z, tokens, top_cls, stats)
         ctx.call = (rows, cols, stride, top, temperature)
         ctx.shape, ctx.in_dtype = logits.shape, logits.dtype
         if top_cls is not None:
@@ -259,18 +286,18 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, dlogp, dentropy, dtop, _):
         if dlogp is None and dentropy is None and dtop is None:
             return None, None, None, None, None
-        z, tokens, live, top_cls, stats = ctx.saved_tensors
+        z, tokens, top_cls, stats = ctx.saved_tensors
         rows, cols, stride, top, temperature = ctx.call
-        f32 = lambda t: None if t is None else t.to(torch.float32).contiguous()
-        dlogp, dentropy, dtop = f32(dlogp), f32(dentropy), f32(dtop)
+        dlogp, dentropy, dtop = _float_gradient(dlogp), _float_gradient(dentropy), _float_gradient(dtop)
         dz = torch.empty([rows, cols], dtype=z.dtype, device=z.device)
         with _on_device(z):
             rc = _lib.lib().isg_token_logprobs_bwd(
                 z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4,
-                _lib.ptr(live), _lib.ptr(top_cls), _lib.ptr(stats), _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(dtop),
-                rows, cols, dtype_code(z.dtype), temperature, top, _lib.ptr(dz), _lib.current_stream())
-        _lib.check(rc, "isg_token_logprobs_bwd")
-        return dz.reshape(ctx.shape).to(ctx.in_dtype), None, None, None, None
+                _lib.ptr(top_cls), stats.data_ptr(), _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(dtop), rows, cols,
+                dtype_code(z.dtype), temperature, top, dz.data_ptr(), _lib.stream_of(z))
+        if rc:
+            _lib.check(rc, "isg_token_logprobs_bwd")
+        return _like_input(dz, ctx.shape, ctx.in_dtype), None, None, None, None
 
 
 def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
@@ -313,13 +340,18 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
 # ---- distillation -----------------------------------------------------------------------------------------------------
 def _distill_forward(z, geometry, values, classes, live, temperature, tail, keep):
     rows, cols, stride = geometry
-    loss = torch.empty([rows], dtype=torch.float32, device=z.device)
-    stats = torch.empty([rows, 8], dtype=torch.float32, device=z.device) if keep else None
+    lib, dev = _lib.lib(), z.device
+    loss = torch.empty([rows], dtype=torch.float32, device=dev)
+    stats = torch.empty([rows, 8], dtype=torch.float32, device=dev) if keep else None
+    space = None
+    if cols > _ONE_UNIT_CLASSES:
+        space = torch.empty([lib.isg_distill_workspace_bytes(rows, cols)], dtype=torch.uint8, device=dev)
     with _on_device(z):
-        rc = _lib.lib().isg_distill_fwd(z.data_ptr(), stride, _lib.ptr(values), _lib.ptr(classes), classes.element_size(),
-                                        _lib.ptr(live), rows, cols, values.shape[-1], dtype_code(z.dtype), temperature,
-                                        tail, _lib.ptr(loss), _lib.ptr(stats), _lib.current_stream())
-    _lib.check(rc, "isg_distill_fwd")
+        rc = lib.isg_distill_fwd(z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(), classes.element_size(),
+                                 _lib.ptr(live), rows, cols, values.shape[-1], dtype_code(z.dtype), temperature, tail,
+                                 loss.data_ptr(), _lib.ptr(stats), _lib.ptr(space), _lib.stream_of(z))
+    if rc:
+        _lib.check(rc, "isg_distill_fwd")
     return loss, stats
 
 
@@ -338,15 +370,16 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, dloss):
         z, values, classes, stats = ctx.saved_tensors
         rows, cols, stride, temperature, tail = ctx.call
-        g = dloss.to(torch.float32).contiguous()
+        g = _float_gradient(dloss)
         dz = torch.empty([rows, cols], dtype=z.dtype, device=z.device)
         with _on_device(z):
-            rc = _lib.lib().isg_distill_bwd(z.data_ptr(), stride, _lib.ptr(values), _lib.ptr(classes),
-                                            classes.element_size(), _lib.ptr(stats), _lib.ptr(g), rows, cols,
-                                            values.shape[-1], dtype_code(z.dtype), temperature, tail, _lib.ptr(dz),
-                                            _lib.current_stream())
-        _lib.check(rc, "isg_distill_bwd")
-        return dz.reshape(ctx.shape).to(ctx.in_dtype), None, None, None, None, None
+            rc = _lib.lib().isg_distill_bwd(z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(),
+                                            classes.element_size(), stats.data_ptr(), g.data_ptr(), rows, cols,
+                                            values.shape[-1], dtype_code(z.dtype), temperature, tail, dz.data_ptr(),
+                                            _lib.stream_of(z))
+        if rc:
+            _lib.check(rc, "isg_distill_bwd")
+        return _like_input(dz, ctx.shape, ctx.in_dtype), None, None, None, None, None
 
 
 def distill_rows(logits, teacher_values, teacher_classes, temperature=1.0, tail=False, live=None):

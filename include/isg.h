@@ -379,23 +379,26 @@ int isg_a3c_loss_bwd(const void* logits, const float* vf, const int32_t* actions
  *   entropy[r]  = -sum_c p_c log p_c
  *   top_classes / top_logprobs [r][top]: the classes of the `top` largest logits in falling order, equal logits by
  *     class (lowest first, NaN last), and their log-probabilities
- *   stats float [r][4] (may be NULL): what isg_token_logprobs_bwd reads.
+ *   stats float [r][4] (may be NULL; 16-byte aligned): what isg_token_logprobs_bwd reads.
  * A logit of -inf is a class without probability; a row of nothing else has log-probability -inf everywhere, entropy 0
  * and a zero gradient.  live uint8 [rows] (may be NULL): rows with 0 are not read, their outputs are 0 (classes -1)
  * and their gradient is 0.  logits `dtype` with rows row_stride >= cols elements apart; tokens are int32 or int64
  * (token_bytes 4 or 8).  0 <= top <= ISG_TOP_MAX, cols <= ISG_CLASSES_MAX, temperature in [1e-30, 1e30].
+ * workspace: device scratch of isg_token_logprobs_workspace_bytes(rows, cols, top) bytes, 8-byte aligned (0 bytes up to
+ * 2,048 classes: may be NULL), in use until the call's work on the stream is done.
  * isg_token_logprobs_bwd: dlogits `dtype` [rows][cols] (dense, not the logits themselves) from the gradients of the
- * three outputs (float; each may be NULL: no gradient arrives there).  No atomics: the same call gives the same bits. */
+ * three outputs (float; each may be NULL: no gradient arrives there).  The same call gives the same bits. */
 #define ISG_TOP_MAX 64
 #define ISG_CLASSES_MAX (1 << 20)
+long long isg_token_logprobs_workspace_bytes(int rows, int cols, int top);
 int isg_token_logprobs_fwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
                            const unsigned char* live, int rows, int cols, int dtype, float temperature, int top,
                            float* logprobs, float* entropy, float* top_logprobs, int32_t* top_classes, float* stats,
-                           void* stream);
+                           void* workspace, void* stream);
 int isg_token_logprobs_bwd(const void* logits, long long row_stride, const void* tokens, int token_bytes,
-                           const unsigned char* live, const int32_t* top_classes, const float* stats,
-                           const float* dlogprobs, const float* dentropy, const float* dtop_logprobs, int rows, int cols,
-                           int dtype, float temperature, int top, void* dlogits, void* stream);
+                           const int32_t* top_classes, const float* stats, const float* dlogprobs, const float* dentropy,
+                           const float* dtop_logprobs, int rows, int cols, int dtype, float temperature, int top,
+                           void* dlogits, void* stream);
 
 /* Distillation from a teacher's k most probable classes (no counterpart in the reference, whose nets train on labels
  * only, polyrnn/Model.py:98-100): the divergence of p = softmax(z / temperature) from the teacher's q,
@@ -408,13 +411,15 @@ int isg_token_logprobs_bwd(const void* logits, long long row_stride, const void*
  * values float [rows][k]; classes int32 or int64 (class_bytes) [rows][k]: a negative class is no entry (fewer than k
  * alternatives), one the row does not have (>= cols) makes loss and gradient of the row NaN, a class given twice takes
  * both masses.  A row without entries has loss 0 and no gradient.  live, row_stride, temperature: as above; k <=
- * ISG_DISTILL_MAX.  stats float [rows][8] (may be NULL without a backward pass).
+ * ISG_DISTILL_MAX.  stats float [rows][8] (may be NULL without a backward pass); workspace as above, of
+ * isg_distill_workspace_bytes(rows, cols) bytes.
  * isg_distill_bwd: dlogits `dtype` [rows][cols] (dense, not the logits themselves) from dloss float [rows]; the values
  * take no gradient. */
 #define ISG_DISTILL_MAX 1024
+long long isg_distill_workspace_bytes(int rows, int cols);
 int isg_distill_fwd(const void* logits, long long row_stride, const float* values, const void* classes, int class_bytes,
                     const unsigned char* live, int rows, int cols, int k, int dtype, float temperature, int tail,
-                    float* loss, float* stats, void* stream);
+                    float* loss, float* stats, void* workspace, void* stream);
 int isg_distill_bwd(const void* logits, long long row_stride, const float* values, const void* classes, int class_bytes,
                     const float* stats, const float* dloss, int rows, int cols, int k, int dtype, float temperature,
                     int tail, void* dlogits, void* stream);

@@ -54,20 +54,21 @@ ONE, TWO = ctypes.c_void_p(4096), ctypes.c_void_p(8192)  # never read: every cal
 
 
 def _fwd(logits=ONE, stride=100, tokens=ONE, tb=4, rows=2, cols=100, dtype=1, T=1.0, top=0, out=ONE, ent=ONE, tl=ONE,
-         tc=ONE):
+         tc=ONE, ws=None, stats=None):
     return _lib.lib().isg_token_logprobs_fwd(logits, stride, tokens, tb, None, rows, cols, dtype, T, top, out, ent, tl, tc,
-                                             None, None)
+                                             stats, ws, None)
 
 
 def _bwd(logits=ONE, stride=100, tokens=ONE, tb=4, tc=ONE, stats=ONE, gl=ONE, gt=None, rows=2, cols=100, dtype=1, T=1.0,
          top=0, out=TWO):
-    return _lib.lib().isg_token_logprobs_bwd(logits, stride, tokens, tb, None, tc, stats, gl, None, gt, rows, cols, dtype, T,
-                                             top, out, None)
+    return _lib.lib().isg_token_logprobs_bwd(logits, stride, tokens, tb, tc, stats, gl, None, gt, rows, cols, dtype, T, top,
+                                             out, None)
 
 
-def _dfwd(logits=ONE, stride=100, values=ONE, classes=ONE, cb=4, rows=2, cols=100, k=4, dtype=1, T=1.0, tail=0, loss=ONE):
+def _dfwd(logits=ONE, stride=100, values=ONE, classes=ONE, cb=4, rows=2, cols=100, k=4, dtype=1, T=1.0, tail=0, loss=ONE,
+          ws=None):
     return _lib.lib().isg_distill_fwd(logits, stride, values, classes, cb, None, rows, cols, k, dtype, T, tail, loss, None,
-                                      None)
+                                      ws, None)
 
 
 def _dbwd(logits=ONE, stride=100, values=ONE, classes=ONE, cb=4, stats=ONE, g=ONE, rows=2, cols=100, k=4, dtype=1, T=1.0,
@@ -93,6 +94,9 @@ def test_entry_points_refuse_what_is_their_own():
     assert _fwd(top=65) == -1 and _fwd(top=-1) == -1 and _fwd(cols=8, top=9) == -1 and b"top" in err()
     assert _fwd(tb=2) == -1 and b"bytes" in err()
     assert _fwd(out=None) == -1 and _fwd(ent=None) == -1 and _fwd(top=3, tl=None) == -1 and _fwd(top=3, tc=None) == -1
+    assert _fwd(cols=50177, stride=50177) == -1 and b"workspace" in err()
+    assert _dfwd(cols=50177, stride=50177) == -1 and b"workspace" in err()
+    assert _fwd(stats=ctypes.c_void_p(4100)) == -1 and b"aligned" in err()
     assert _bwd(top=65) == -1 and _bwd(tokens=None) == -1 and _bwd(stats=None) == -1
     assert _bwd(gt=ONE) == -1 and _bwd(gt=ONE, top=3, tc=None) == -1  # gradients of alternatives there are none of
     assert _bwd(out=ONE) == -1 and b"alias" in err()
@@ -100,6 +104,18 @@ def test_entry_points_refuse_what_is_their_own():
     assert _dfwd(values=None) == -1 and _dfwd(classes=None) == -1 and _dfwd(loss=None) == -1
     assert _dbwd(k=0) == -1 and _dbwd(stats=None) == -1 and _dbwd(g=None) == -1 and _dbwd(out=None) == -1
     assert _dbwd(out=ONE) == -1 and b"alias" in err()
+
+
+def test_workspaces_cover_the_parts_of_a_split_row():
+    lib = _lib.lib()
+    size, dsize = lib.isg_token_logprobs_workspace_bytes, lib.isg_distill_workspace_bytes
+    assert size(1000, 2048, 64) == 0 and size(4096, 8192, 64) == 0 and size(0, 50177, 5) >= 0
+    for rows, cols in ((1, 2049), (1, 50177), (300, 8193), (5000, 131071), (2, 1 << 20), (100000, 1 << 20)):
+        for top in (0, 20, 64):  # at least 32 classes a thread of 256, at most one part per 2,048 classes
+            assert size(rows, cols, top) <= rows * -(-cols // 2048) * (12 + 8 * top) + 8
+            assert size(rows, cols, top) >= rows * (cols > 8192) * -(-cols // 8192) * (12 + 8 * top)
+        assert dsize(rows, cols) <= rows * -(-cols // 2048) * 16
+    assert size(-1, 10, 0) == -1 and size(1, (1 << 20) + 1, 0) == -1 and size(1, 10, 65) == -1 and dsize(1, 0) == -1
 
 
 def test_python_calls_refuse_what_they_cannot_take():
