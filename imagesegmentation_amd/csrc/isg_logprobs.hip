@@ -646,6 +646,9 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
     if (a.tail) merge(m, s, t.me, t.se, a.c, a.c_lo);
     m = m == -INFINITY ? 0.0f : m;
     const float l2s = s == 0.0f ? INFINITY : __builtin_amdgcn_logf(s);
+    // (log s as a whole number of ln 2 and the logarithm of a fraction: added one after the other to a difference of the
+    // same size it loses a rounding of that difference, not one of its own that every entry of the row would share)
+    const float s_exp = (float)__builtin_amdgcn_frexp_expf(s), s_log = kLn2 * __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s));
     // the teacher's distribution over its entries
     const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? (float)(1.4426950408889634074 - (double)kLog2e) : a.c_lo;
     float mv = 0.0f, lv = 0.0f, bad = 0.0f, sv = 0.0f;
@@ -671,7 +674,8 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
         if (i < 0 || i >= a.cols) continue;
         const float q = power(v[j], mv, cv, cv_lo) * __builtin_amdgcn_exp2f(-lv);
         const float lq = (v[j] - mv) * (a.tail ? 1.0f : a.inv_t) - kLn2 * lv;
-        if (q != 0.0f) l += q * (lq - log_prob(ld(z, i), m, a.inv_t, l2s));
+        const float d = lq - (ld(z, i) - m) * a.inv_t;  // log q - log p - log s
+        if (q != 0.0f) l += s == 0.0f ? INFINITY : q * (__builtin_fmaf(s_exp, kLn2, d) + s_log);
     }
     l = wave_sum(l);
     bad = wave_max(bad);
@@ -681,10 +685,11 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
             const bool none = t.s == 0.0f;
             const float mr = t.m == -INFINITY ? 0.0f : t.m, lr = none ? INFINITY : __builtin_amdgcn_logf(t.s);
             if (none && qr <= kNoMass) qr = 0.0f;
-            // log2 of the student's mass outside
-            const float lpr = __builtin_fmaf(mr - m, a.c_lo, (mr - m) * a.c) + (lr - l2s);
+            // the student's mass outside; its logarithm from the logarithms where it is no normal float
+            const float pr = t.s * power(mr, m, a.c, a.c_lo) / s;
+            const float lpr = pr > 1e-30f ? __builtin_amdgcn_logf(pr) : (mr - m) * a.c + (lr - l2s);
             if (qr > 0.0f) l += none ? INFINITY : qr * kLn2 * (__builtin_amdgcn_logf(qr) - lpr);
-            coef = none ? 0.0f : (qsum + qr) * __builtin_amdgcn_exp2f(lpr) - qr;
+            coef = none ? 0.0f : (qsum + qr) * pr - qr;
             mb = mr, lb = lr;
         }
         if (bad != 0.0f) l = NAN, coef = NAN;

@@ -203,7 +203,7 @@ def _row_argument(t, shape, kinds, device, what):
     """A per-row tensor of one of the ``kinds`` in the rows' shape, contiguous."""
     if not torch.is_tensor(t) or t.dtype not in kinds:
         raise TypeError("%s must be a tensor of %s" % (what, " or ".join(str(k).replace("torch.", "") for k in kinds)))
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError("%s must have the shape %s, not %s" % (what, tuple(shape), tuple(t.shape)))
     if t.device != device:
         raise ValueError("%s lives on %s, the logits on %s" % (what, t.device, device))
@@ -228,6 +228,8 @@ _here = contextlib.nullcontext()
 
 
 _ONE_UNIT_CLASSES = 2048  # rows up to here take no workspace
+_ROW_CLASSES = (torch.int32, torch.int64)
+_ROW_MASKS = (torch.bool, torch.uint8)
 
 
 def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
@@ -235,7 +237,7 @@ def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
     lib, dev = _lib.lib(), z.device
     f32 = torch.float32
     entropy = torch.empty([rows], dtype=f32, device=dev)
-    logp = torch.empty([rows], dtype=f32, device=dev) if tokens is not None else None
+    logp = torch.empty_like(entropy) if tokens is not None else None
     top_logp = top_cls = stats = space = None
     if top:
         top_logp = torch.empty([rows, top], dtype=f32, device=dev)
@@ -254,17 +256,28 @@ def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
     return logp, entropy, top_logp, top_cls, stats
 
 
-def _like_input(dz, shape, dtype):
-    """A gradient [rows, classes] in the logits' shape and type."""
-    if dz.shape != shape:
-        dz = dz.reshape(shape)
-    return dz if dz.dtype == dtype else dz.to(dtype)
+# Backward passes run on autograd's own thread, where every line of Python costs two to three times what it does in the
+# caller's: what they pass to the library is put together in the forward pass, and their checks are the forward's.
+def _gradient_like(z, shape):
+    """The tensor a gradient is written into: the logits' shape, dense."""
+    if z.is_contiguous():
+        return torch.empty_like(z)
+    return torch.empty(shape, dtype=z.dtype, device=z.device)
 
 
 def _float_gradient(g):
     if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
         return g
     return g.to(torch.float32).contiguous()
+
+
+def _first_derivative_only(function):
+    """As ``once_differentiable``, at no cost where no graph of the backward pass is asked for."""
+    guarded = once_differentiable(function)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else function(ctx, *grads)
+    return backward
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -274,30 +287,30 @@ class _TokenLogprobs(torch.autograd.Function):
         logp, entropy, top_logp, top_cls, stats = _logprobs_forward(z, (rows, cols, stride), tokens, live, top,
                                                                     temperature, True)
         ctx.save_for_backward(z, tokens, top_cls, stats)
-        ctx.call = (rows, cols, stride, top, temperature)
-        ctx.shape, ctx.in_dtype = logits.shape, logits.dtype
+        ctx.first = (z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4,
+                     _lib.ptr(top_cls), stats.data_ptr())
+        ctx.last = (rows, cols, dtype_code(z.dtype), temperature, top)
+        ctx.shape, ctx.in_dtype, ctx.device = logits.shape, logits.dtype, z.device.index
         if top_cls is not None:
             ctx.mark_non_differentiable(top_cls)
         ctx.set_materialize_grads(False)
         return logp, entropy, top_logp, top_cls
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative_only
     def backward(ctx, dlogp, dentropy, dtop, _):
         if dlogp is None and dentropy is None and dtop is None:
             return None, None, None, None, None
-        z, tokens, top_cls, stats = ctx.saved_tensors
-        rows, cols, stride, top, temperature = ctx.call
+        z = ctx.saved_tensors[0]  # (all of them are checked for changes in place)
         dlogp, dentropy, dtop = _float_gradient(dlogp), _float_gradient(dentropy), _float_gradient(dtop)
-        dz = torch.empty([rows, cols], dtype=z.dtype, device=z.device)
-        with _on_device(z):
-            rc = _lib.lib().isg_token_logprobs_bwd(
-                z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4,
-                _lib.ptr(top_cls), stats.data_ptr(), _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(dtop), rows, cols,
-                dtype_code(z.dtype), temperature, top, dz.data_ptr(), _lib.stream_of(z))
+        dz = _gradient_like(z, ctx.shape)
+        rc = _lib.lib().isg_token_logprobs_bwd(
+            *ctx.first, None if dlogp is None else dlogp.data_ptr(), None if dentropy is None else dentropy.data_ptr(),
+            None if dtop is None else dtop.data_ptr(), *ctx.last, dz.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(ctx.device))
         if rc:
             _lib.check(rc, "isg_token_logprobs_bwd")
-        return _like_input(dz, ctx.shape, ctx.in_dtype), None, None, None, None
+        return dz if dz.dtype == ctx.in_dtype else dz.to(ctx.in_dtype), None, None, None, None
 
 
 def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
@@ -320,9 +333,9 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
         raise ValueError("token_logprobs: top %d of %d classes (0 to %d)" % (top, logits.shape[-1], TOP_MAX))
     temperature = _temperature(temperature, "token_logprobs")
     if tokens is not None:
-        tokens = _row_argument(tokens, lead, (torch.int32, torch.int64), logits.device, "token_logprobs: tokens")
+        tokens = _row_argument(tokens, lead, _ROW_CLASSES, logits.device, "token_logprobs: tokens")
     if live is not None:
-        live = _row_argument(live, lead, (torch.bool, torch.uint8), logits.device, "token_logprobs: live")
+        live = _row_argument(live, lead, _ROW_MASKS, logits.device, "token_logprobs: live")
     if torch.is_grad_enabled() and logits.requires_grad:
         logp, entropy, top_logp, top_cls = _TokenLogprobs.apply(logits, tokens, live, top, temperature)
     else:
@@ -361,25 +374,23 @@ class _Distill(torch.autograd.Function):
         z, rows, cols, stride = _class_rows(logits, "distill_rows")
         loss, stats = _distill_forward(z, (rows, cols, stride), values, classes, live, temperature, tail, True)
         ctx.save_for_backward(z, values, classes, stats)
-        ctx.call = (rows, cols, stride, temperature, tail)
-        ctx.shape, ctx.in_dtype = logits.shape, logits.dtype
+        ctx.first = (z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(), classes.element_size(),
+                     stats.data_ptr())
+        ctx.last = (rows, cols, values.shape[-1], dtype_code(z.dtype), temperature, tail)
+        ctx.shape, ctx.in_dtype, ctx.device = logits.shape, logits.dtype, z.device.index
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative_only
     def backward(ctx, dloss):
-        z, values, classes, stats = ctx.saved_tensors
-        rows, cols, stride, temperature, tail = ctx.call
+        z = ctx.saved_tensors[0]
         g = _float_gradient(dloss)
-        dz = torch.empty([rows, cols], dtype=z.dtype, device=z.device)
-        with _on_device(z):
-            rc = _lib.lib().isg_distill_bwd(z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(),
-                                            classes.element_size(), stats.data_ptr(), g.data_ptr(), rows, cols,
-                                            values.shape[-1], dtype_code(z.dtype), temperature, tail, dz.data_ptr(),
-                                            _lib.stream_of(z))
+        dz = _gradient_like(z, ctx.shape)
+        rc = _lib.lib().isg_distill_bwd(*ctx.first, g.data_ptr(), *ctx.last, dz.data_ptr(),
+                                        torch._C._cuda_getCurrentRawStream(ctx.device))
         if rc:
             _lib.check(rc, "isg_distill_bwd")
-        return _like_input(dz, ctx.shape, ctx.in_dtype), None, None, None, None, None
+        return dz if dz.dtype == ctx.in_dtype else dz.to(ctx.in_dtype), None, None, None, None, None
 
 
 def distill_rows(logits, teacher_values, teacher_classes, temperature=1.0, tail=False, live=None):
@@ -405,13 +416,14 @@ def distill_rows(logits, teacher_values, teacher_classes, temperature=1.0, tail=
     k = teacher_values.shape[-1] if teacher_values.dim() else 0
     if not 1 <= k <= DISTILL_MAX:
         raise ValueError("distill_rows: %d classes of the teacher (1 to %d)" % (k, DISTILL_MAX))
-    values = teacher_values.detach()
-    values = _row_argument(values if values.dtype == torch.float32 else values.float(), lead + (k,), (torch.float32,),
-                           logits.device, "distill_rows: teacher_values")
-    classes = _row_argument(teacher_classes, lead + (k,), (torch.int32, torch.int64), logits.device,
-                            "distill_rows: teacher_classes")
+    values = teacher_values.detach() if teacher_values.requires_grad else teacher_values
+    if values.dtype != torch.float32:
+        values = values.float()
+    shape = lead + (k,)
+    values = _row_argument(values, shape, (torch.float32,), logits.device, "distill_rows: teacher_values")
+    classes = _row_argument(teacher_classes, shape, _ROW_CLASSES, logits.device, "distill_rows: teacher_classes")
     if live is not None:
-        live = _row_argument(live, lead, (torch.bool, torch.uint8), logits.device, "distill_rows: live")
+        live = _row_argument(live, lead, _ROW_MASKS, logits.device, "distill_rows: live")
     if torch.is_grad_enabled() and logits.requires_grad:
         loss = _Distill.apply(logits, values, classes, live, temperature, int(bool(tail)))
     else:
