@@ -30,6 +30,8 @@ constexpr int kMaxEntries = ISG_DISTILL_MAX;  // a teacher's classes per row
 constexpr int kMaxCols = ISG_CLASSES_MAX;     // class axis
 constexpr int kWaveCols = 2048;               // classes one wave holds (32 registers a lane)
 constexpr int kCandidates = 256;              // alternatives in question per wave; a workgroup holds four times as many
+constexpr int kListMax = 1024;                // alternatives a workgroup collects along its part of a row
+constexpr int kListTrim = 256;                // ... before it goes back to the best
 
 typedef unsigned long long u64;
 
@@ -135,7 +137,7 @@ struct Span {
     static constexpr int VE = NE < 16 / (int)sizeof(T) ? NE : 16 / (int)sizeof(T);
     static constexpr int NV = NE / VE;
     static constexpr int kCols = W * 64 * NE;  // of one unit (a wave or a workgroup)
-    int base, cols, lane;                      // lane: of the unit's W * 64
+    int base, cols, lane;                      // cols: where the unit ends; lane: of its W * 64
 
     __device__ __forceinline__ Span(int base_, int cols_, int lane_) : base(base_), cols(cols_), lane(lane_) {}
     __device__ __forceinline__ int start(int slot) const { return base + (slot * W * 64 + lane) * VE; }
@@ -145,7 +147,7 @@ struct Span {
         const int s = start(slot);
         return s < cols - VE ? s : cols - VE;
     }
-    // the class of element e, or -1 where it is not this thread's
+    // the class of element e, or -1 where it is not this thread's (or another unit's)
     __device__ __forceinline__ int cls(int e) const {
         const int s = start(e / VE), i = offset(e / VE) + e % VE;
         return i >= s ? i : -1;
@@ -175,6 +177,26 @@ struct Span {
 #pragma unroll
                 for (int j = 0; j < VE; ++j) v[t * VE + j] = -INFINITY;
             }
+        }
+    }
+    // the same in two halves, for loads that are on their way while other elements are worked on
+    static constexpr int kWords = NE * (int)sizeof(T) / 4;
+    __device__ __forceinline__ void fetch(const T* z, unsigned (&raw)[kWords]) const {
+#pragma unroll
+        for (int t = 0; t < NV; ++t) __builtin_memcpy(raw + t * (kWords / NV), z + offset(t), 16);
+    }
+    __device__ __forceinline__ void unpack(const unsigned (&raw)[kWords], float (&v)[NE]) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[i]);
+            else v[2 * i] = __uint_as_float(raw[i] << 16), v[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+        }
+        if (base + kCols <= cols) return;
+#pragma unroll
+        for (int t = 0; t < NV; ++t) {
+            const int s = start(t), o = offset(t);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) v[t * VE + j] = o + j >= s ? v[t * VE + j] : -INFINITY;
         }
     }
     // a slot's gradients; the row's last vector repeats values of its neighbour, which is no harm inside the unit
@@ -209,7 +231,7 @@ __device__ __forceinline__ unsigned order_bits(float v) {
 __device__ __forceinline__ float order_value(unsigned k) {
     return k == 1u ? NAN : __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-__device__ __forceinline__ u64 order_key(float v, int c) { return c < 0 ? 0ull : ((u64)order_bits(v) << 32) | (unsigned)~c; }
+__device__ __forceinline__ u64 order_key(float v, int c) { return ((u64)order_bits(v) << 32) | (unsigned)~c; }
 
 // log p of a logit; a row without any probability (log2 s = +inf) gives -inf.  In nats throughout: at T = 1 the
 // type's lowest value has a finite logarithm, its binary one would overflow.
@@ -231,8 +253,8 @@ struct TopShared {
     u64 best[4];
 };
 
-template <int W, int NE, typename Key, typename Reload, typename Emit>
-__device__ __forceinline__ void select_top(const float (&v)[NE], int k, TopShared<W>& sh, Key key, Reload reload, Emit emit) {
+template <int W, int NE, typename Reload, typename Emit>
+__device__ __forceinline__ void select_top(const float (&v)[NE], int k, TopShared<W>& sh, Reload reload, Emit emit) {
     constexpr int Q = W == 1 ? (NE < 4 ? NE : 4) : 1;
     constexpr int kCap = W == 1 ? kCandidates : 4 * kCandidates;
     const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
@@ -318,9 +340,9 @@ __device__ __forceinline__ void select_top(const float (&v)[NE], int k, TopShare
         u64 last = ~0ull;
         for (int j = 0; j < k; ++j) {
             u64 best = 0;
-#pragma unroll
+#pragma unroll 1
             for (int e = 0; e < NE; ++e) {
-                const u64 x = key(e);
+                const u64 x = reload(e);
                 if (x < last && x > best) best = x;
             }
             best = wave_max_key(best);
@@ -346,9 +368,15 @@ struct Sums {
     float m, s, u;
 };
 
-// The sums over a unit's elements.  A unit without any probability has m = -inf and s = 0.
-template <int W, int NE>
-__device__ __forceinline__ Sums unit_sums(const float (&v)[NE], float c, float (*red)[4]) {
+__device__ __forceinline__ void add_power(float z, float m, float c, float& s, float& u) {
+    const float x = (z - m) * c, p = __builtin_amdgcn_exp2f(x);
+    s += p;
+    u += p * fmaxf(x, -1000.0f);
+}
+
+// A part without any probability has m = -inf and s = 0.
+template <int NE>
+__device__ __forceinline__ Sums wave_sums(const float (&v)[NE], float c) {
     float m = v[0];
 #pragma unroll
     for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
@@ -356,28 +384,22 @@ __device__ __forceinline__ Sums unit_sums(const float (&v)[NE], float c, float (
     const float mz = m == -INFINITY ? 0.0f : m;
     float s = 0.0f, u = 0.0f;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-        const float x = (v[e] - mz) * c, p = __builtin_amdgcn_exp2f(x);
-        s += p;
-        u += p * fmaxf(x, -1000.0f);
+    for (int e = 0; e < NE; ++e) add_power(v[e], mz, c, s, u);
+    return Sums{m, wave_sum(s), wave_sum(u)};
+}
+
+__device__ __forceinline__ void merge_sums(Sums& t, const Sums& p, float c) {
+    const float m = fmaxf(t.m, p.m);
+    Sums r{m, 0.0f, 0.0f};
+    if (t.s != 0.0f) {
+        const float d = (t.m - m) * c, f = __builtin_amdgcn_exp2f(d);
+        r.s = f * t.s, r.u = f * (t.u + fmaxf(d, -1000.0f) * t.s);
     }
-    s = wave_sum(s), u = wave_sum(u);
-    if constexpr (W == 1) return Sums{m, s, u};
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane == 0) red[wave][0] = m, red[wave][1] = s, red[wave][2] = u;
-    together<W>();
-    Sums r{red[0][0], 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 1; w < W; ++w) r.m = fmaxf(r.m, red[w][0]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const float sw = red[w][1];
-        if (sw == 0.0f) continue;
-        const float d = (red[w][0] - r.m) * c, f = __builtin_amdgcn_exp2f(d);
-        r.s += f * sw;
-        r.u += f * (red[w][2] + fmaxf(d, -1000.0f) * sw);
+    if (p.s != 0.0f) {
+        const float d = (p.m - m) * c, f = __builtin_amdgcn_exp2f(d);
+        r.s += f * p.s, r.u += f * (p.u + fmaxf(d, -1000.0f) * p.s);
     }
-    return r;
+    t = r;
 }
 
 // What a row's results follow from.  `c_rel`: by how much log2(e) / T exceeds the float c, relative; the logarithm of
@@ -405,7 +427,7 @@ struct LogprobsArgs {
     Sums* part;      // [rows][splits]
     u64* part_keys;  // [rows][splits][top]
     long long row_stride, units;
-    int token_bytes, cols, splits, top;
+    int token_bytes, cols, splits, per, top;  // a row is cut into `splits` parts of `per` classes
     float c, inv_t, c_rel;
 };
 
@@ -430,27 +452,163 @@ __device__ __forceinline__ void row_outputs(const LogprobsArgs& a, const T* z, l
     if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(r.m, r.l2s, r.H, 0.0f);
 }
 
+__device__ __forceinline__ void row_alternative(const LogprobsArgs& a, long long row, const RowStats& r, int place, u64 key) {
+    a.top_logprobs[row * a.top + place] = log_prob(order_value((unsigned)(key >> 32)), r.m, a.inv_t, r.l2s);
+    a.top_classes[row * a.top + place] = (int)~(unsigned)key;
+}
+
 __device__ __forceinline__ long long block_index() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
 
 // ---- token_logprobs ------------------------------------------------------------------------------------------------
-template <typename T, int W, int NE, bool TOP>
+// A row of up to kWaveCols classes: one wave.
+template <typename T, int NE, bool TOP>
 __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restrict__ logits, LogprobsArgs a) {
-    __shared__ float red[W][4];
-    __shared__ typename std::conditional<TOP, TopShared<W>, char>::type shared;
-    const int tid = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
-    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
+    __shared__ typename std::conditional<TOP, TopShared<1>, char>::type shared;
+    const int lane = threadIdx.x & 63;
+    const long long row = block_index() * 4 + (threadIdx.x >> 6);
+    if (row >= a.units) return;
+    if (a.live && !a.live[row]) {
+        dead_row<1>(a, row, lane);
+        return;
+    }
+    const T* z = logits + row * a.row_stride;
+    const Span<T, 1, NE> span(0, a.cols, lane);
+    float v[NE];
+    span.template load<true>(z, v);
+    const RowStats r = row_stats(wave_sums(v, a.c), a.c_rel);
+    if (lane == 0) row_outputs(a, z, row, r);
+    if constexpr (TOP)
+        select_top<1, NE>(
+            v, a.top, shared,
+            [&](int e) {
+                const int i = span.cls(e);
+                return i < 0 ? 0ull : order_key(ld(z, i), i);
+            },
+            [&](int place, u64 k) { row_alternative(a, row, r, place, k); });
+}
+
+// What a workgroup has found of a part of a row's best classes so far.
+struct TopList {
+    u64 keys[kListMax];  // in no order beyond the first `top` after a prune
+    u64 sorted[kMaxTop];
+    int count;
+};
+
+// The k first keys of the list, in order, to its front.  Uniform over the workgroup; returns the new count.
+__device__ __forceinline__ int prune(TopList& list, int count, int k) {
+    for (int r = threadIdx.x; r < count; r += kThreads) {
+        const u64 own = list.keys[r];
+        int place = 0;
+#pragma unroll 4
+        for (int o = 0; o < count; ++o) place += list.keys[o] > own ? 1 : 0;
+        if (place < k) list.sorted[place] = own;
+    }
+    __syncthreads();
+    const int n = count < k ? count : k;
+    for (int r = threadIdx.x; r < n; r += kThreads) list.keys[r] = list.sorted[r];
+    __syncthreads();
+    return n;
+}
+
+// A part of a longer row: a workgroup walks over it, kThreads * NE classes at a time, the next ones being loaded
+// meanwhile.  Every wave keeps its own maximum and its lanes their own sums until the end.  Of the best classes the
+// first step finds its k by select_top; what a later step has above the k-th of the list joins the list, which is cut
+// back to k when it has grown to kListTrim.  Steps that would overrun it (rising rows) go through select_top as well.
+template <typename T, int NE, bool TOP>
+__global__ __launch_bounds__(kThreads, 8) void logprobs_stream_kernel(const T* __restrict__ logits, LogprobsArgs a) {
+    __shared__ float red[4][4];
+    __shared__ typename std::conditional<TOP, TopShared<4>, char>::type shared;
+    __shared__ typename std::conditional<TOP, TopList, char>::type list;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const long long unit = block_index();
     if (unit >= a.units) return;
     const long long row = a.splits == 1 ? unit : unit / a.splits;
     const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
     if (a.live && !a.live[row]) {
-        if (a.splits == 1) dead_row<W>(a, row, tid);
+        if (a.splits == 1) dead_row<4>(a, row, tid);
         return;
     }
     const T* z = logits + row * a.row_stride;
-    const Span<T, W, NE> span(split * Span<T, W, NE>::kCols, a.cols, tid);
-    float v[NE];
-    span.template load<true>(z, v);
-    const Sums t = unit_sums<W, NE>(v, a.c, red);
+    using S = Span<T, 4, NE>;
+    const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
+    unsigned raw[S::kWords];
+    S(lo, hi, tid).fetch(z, raw);
+    Sums t{-INFINITY, 0.0f, 0.0f};  // (m of the wave; s, u of the lane)
+    int count = 0;
+    float low = -INFINITY;   // what a further class has to exceed
+    bool trusted = false;    // ... where the list holds k real classes
+    for (int base = lo; base < hi; base += S::kCols) {
+        const S span(base, hi, tid);
+        float v[NE];
+        span.unpack(raw, v);
+        if (base + S::kCols < hi) S(base + S::kCols, hi, tid).fetch(z, raw);
+        float m = v[0];
+#pragma unroll
+        for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
+        const float lane_max = m;
+        m = wave_max(m);
+        if (m > t.m) {  // (uniform in the wave)
+            if (t.m != -INFINITY) {
+                const float d = (t.m - m) * a.c, f = __builtin_amdgcn_exp2f(d);
+                t.u = f * (t.u + fmaxf(d, -1000.0f) * t.s);
+                t.s *= f;
+            }
+            t.m = m;
+        }
+        const float mz = t.m == -INFINITY ? 0.0f : t.m;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) add_power(v[e], mz, a.c, t.s, t.u);
+        if constexpr (TOP) {
+            const auto reload = [&](int e) {
+                const int i = span.cls(e);
+                return i < 0 ? 0ull : order_key(ld(z, i), i);
+            };
+            bool select = !trusted;
+            if (trusted) {
+                unsigned hit = 0;
+                if (__ballot(lane_max > low)) {
+#pragma unroll
+                    for (int e = 0; e < NE; ++e) hit |= (v[e] > low ? 1u : 0u) << e;
+                }
+                if (tid == 0) list.count = count;
+                __syncthreads();
+                int at = 0;
+                const int mine = __builtin_popcount(hit);
+                if (mine) at = atomicAdd(&list.count, mine);
+                if (at + mine <= kListMax)
+                    while (hit) {
+                        const int e = __builtin_ctz(hit);
+                        hit &= hit - 1;
+                        list.keys[at++] = reload(e);
+                    }
+                __syncthreads();
+                const int total = list.count;
+                select = total > kListMax;
+                if (!select) count = total;
+            }
+            if (select) {
+                if (count > a.top) count = prune(list, count, a.top);
+                select_top<4, NE>(
+                    v, a.top, shared, reload,
+                    [&](int place, u64 k) { list.keys[count + place] = k; });
+                __syncthreads();
+                count += a.top;
+            }
+            if (select || count > kListTrim) {
+                count = prune(list, count, a.top);
+                const unsigned kth = (unsigned)(list.keys[a.top - 1] >> 32);
+                trusted = count == a.top && kth > 1u;  // (0: fewer classes than that so far; 1: NaN)
+                low = order_value(kth);
+            }
+        }
+    }
+    // the waves' sums
+    t.s = wave_sum(t.s), t.u = wave_sum(t.u);
+    if (lane == 0) red[tid >> 6][0] = t.m, red[tid >> 6][1] = t.s, red[tid >> 6][2] = t.u;
+    __syncthreads();
+    t = Sums{red[0][0], red[0][1], red[0][2]};
+#pragma unroll
+    for (int w = 1; w < 4; ++w) merge_sums(t, Sums{red[w][0], red[w][1], red[w][2]}, a.c);
     RowStats r;
     if (a.splits == 1) {
         r = row_stats(t, a.c_rel);
@@ -459,18 +617,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restr
         a.part[unit] = t;
     }
     if constexpr (TOP) {
-        const auto key = [&](int e) { return order_key(v[e], span.cls(e)); };
-        const auto reload = [&](int e) {
-            const int i = span.cls(e);
-            return order_key(ld(z, i), i);
-        };
-        if (a.splits == 1)
-            select_top<W, NE>(v, a.top, shared, key, reload, [&](int place, u64 k) {
-                a.top_logprobs[row * a.top + place] = log_prob(order_value((unsigned)(k >> 32)), r.m, a.inv_t, r.l2s);
-                a.top_classes[row * a.top + place] = (int)~(unsigned)k;
-            });
-        else
-            select_top<W, NE>(v, a.top, shared, key, reload, [&](int place, u64 k) { a.part_keys[unit * a.top + place] = k; });
+        if (count > a.top) count = prune(list, count, a.top);
+        for (int j = tid; j < a.top; j += kThreads) {
+            const u64 k = j < count ? list.keys[j] : 0ull;
+            if (a.splits == 1) row_alternative(a, row, r, j, k);
+            else a.part_keys[unit * a.top + j] = k;
+        }
     }
 }
 
@@ -487,36 +639,30 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
     }
     // (every wave for itself)
     const Sums* part = a.part + row * a.splits;
-    float m = -INFINITY;
-    for (int i = lane; i < a.splits; i += 64) m = fmaxf(m, part[i].m);
-    Sums t{wave_max(m), 0.0f, 0.0f};
-    for (int i = lane; i < a.splits; i += 64) {
-        const Sums p = part[i];
-        if (p.s == 0.0f) continue;
-        const float d = (p.m - t.m) * a.c, f = __builtin_amdgcn_exp2f(d);
-        t.s += f * p.s;
-        t.u += f * (p.u + fmaxf(d, -1000.0f) * p.s);
-    }
+    Sums t{-INFINITY, 0.0f, 0.0f};
+    for (int i = lane; i < a.splits; i += 64) merge_sums(t, part[i], a.c);
+    const float m = wave_max(t.m);
+    merge_sums(t, Sums{m, 0.0f, 0.0f}, a.c);  // (to the common maximum)
     t.s = wave_sum(t.s), t.u = wave_sum(t.u);
     const RowStats r = row_stats(t, a.c_rel);
     if (tid == 0) row_outputs(a, logits + row * a.row_stride, row, r);
     if (a.top == 0) return;
     const int n = a.splits * a.top;
     const u64* keys = a.part_keys + row * n;
-    u64 k[NE];
     float v[NE];
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
         const int i = e * W * 64 + tid;
-        k[e] = i < n ? keys[i] : 0ull;
-        v[e] = k[e] ? order_value((unsigned)(k[e] >> 32)) : -INFINITY;
+        const unsigned k = i < n ? (unsigned)(keys[i] >> 32) : 0u;
+        v[e] = k ? order_value(k) : -INFINITY;
     }
     select_top<W, NE>(
-        v, a.top, shared, [&](int e) { return k[e]; }, [&](int e) { return keys[e * W * 64 + tid]; },
-        [&](int place, u64 key) {
-            a.top_logprobs[row * a.top + place] = log_prob(order_value((unsigned)(key >> 32)), r.m, a.inv_t, r.l2s);
-            a.top_classes[row * a.top + place] = (int)~(unsigned)key;
-        });
+        v, a.top, shared,
+        [&](int e) {
+            const int i = e * W * 64 + tid;
+            return i < n ? keys[i] : 0ull;
+        },
+        [&](int place, u64 key) { row_alternative(a, row, r, place, key); });
 }
 
 // dlogits[c] = 1/T ([c = a] g_a + sum_j [c = i_j] g_j - p_c (g_a + sum_j g_j) - g_H p_c (log p_c + H)): the dense part
@@ -529,7 +675,7 @@ struct LogprobsBwdArgs {
     const float* dentropy;
     const float* dtop;
     long long row_stride, units;
-    int token_bytes, cols, splits, top;
+    int token_bytes, cols, splits, per, top;
     float c, inv_t;
 };
 
@@ -542,7 +688,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restr
     const long long row = a.splits == 1 ? unit : unit / a.splits;
     const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
     using S = Span<T, W, NE>;
-    const S span(split * S::kCols, a.cols, tid);
+    const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
+    const S span(lo, hi, tid);
     T* d = dlogits + row * a.cols;
     const float m = a.stats[4 * row], l2s = a.stats[4 * row + 1], H = a.stats[4 * row + 2];
     const bool zero = l2s == INFINITY;  // a dead row, or no class has probability: nothing to move
@@ -572,7 +719,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restr
     if (zero) return;
     together<W>();
     if (tid >= 64) return;
-    const int lo = span.base, hi = span.base + S::kCols < a.cols ? span.base + S::kCols : a.cols;
     const bool both = __ballot(ti >= 0 && ti == tok) != 0;
     if (ti >= lo && ti < hi) {
         const float o = a.inv_t * (dense(ld(z, ti)) + gt + (ti == tok ? ga : 0.0f));
@@ -604,8 +750,8 @@ struct DistillArgs {
     DistillStats* stats;
     DistillPart* part;  // [rows][splits]
     long long row_stride, units;
-    int class_bytes, cols, splits, k, tail;
-    float c, c_lo, inv_t;
+    int class_bytes, cols, splits, per, k, tail;
+    float c, c_lo, c_near, inv_t;
 };
 
 // 2^((z - m) (c + c_lo)): log2(e) / T to twice a float's digits, as a rounded c shifts every exponent the same way
@@ -614,9 +760,17 @@ __device__ __forceinline__ float power(float z, float m, float c, float c_lo) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c_lo, d * c));
 }
 
+// ... of the many classes of a row: of bf16 logits by the nearest float alone (x is off by 2^-25 of itself at most)
+template <typename T>
+__device__ __forceinline__ float power_of(const DistillArgs& a, float z, float m) {
+    return sizeof(T) == 4 ? power(z, m, a.c, a.c_lo) : __builtin_amdgcn_exp2f((z - m) * a.c_near);
+}
+
 // A remaining mass that rounding alone can leave of the entries' log-probabilities (k of them, each good to 2^-24 of
 // its size): where the student has no class outside the entries it is no mass, anything above it has nowhere to go.
 constexpr float kNoMass = 1e-5f;
+
+constexpr int kMarkCols = 131072;  // classes a workgroup's part may have: one bit each (16 KB)
 
 // (m, s) of two disjoint parts
 __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float c, float c_lo) {
@@ -700,62 +854,69 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
 
 // loss = sum_j q_j (log q_j - log p_(i_j)), and with TAIL the mass outside the entries as one more class:
 // + q_r (log q_r - log p_r), where p_r is summed over those classes themselves (1 - sum would cancel).  For that every
-// thread gets one bit per element of its own that an entry names, through LDS, and blanks those elements; the entries'
-// own classes are summed from a second look at them.
-template <typename T, int W, int NE, bool TAIL>
+// class an entry names is marked in LDS and blanked when its thread comes to it; the entries' own classes are summed
+// from a second look at them.
+
+// The sums (me, se) over the classes the entries name in [lo, hi), each once; mark(class) says whether it was marked
+// before.  W waves share the entries; the result is the wave's.
+template <int W, typename T, typename Mark>
+__device__ __forceinline__ void mark_entries(const DistillArgs& a, const T* z, long long row, int lo, int hi, unsigned* repeated,
+                                             DistillPart& t, Mark mark) {
+    const int tid = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
+    bool twice = false;
+    for (int j = tid; j < a.k; j += W * 64) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i >= lo && i < hi) twice |= mark((int)i);
+    }
+    if constexpr (W == 1) {
+        twice = __ballot(twice) != 0;
+        together<W>();
+    } else {
+        if (twice) *repeated = 1u;
+        together<W>();
+        twice = *repeated != 0;
+    }
+    for (int j = tid; j < a.k; j += W * 64) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < lo || i >= hi) continue;
+        if (twice && named_before(a, row, j, i)) continue;
+        const float zi = ld(z, i);
+        merge(t.me, t.se, zi, zi == -INFINITY ? 0.0f : 1.0f, a.c, a.c_lo);
+    }
+    const float m = wave_max(t.me);
+    t.se = wave_sum(t.se == 0.0f ? 0.0f : t.se * power(t.me, m, a.c, a.c_lo));
+    t.me = m;
+}
+
+// A row of up to kWaveCols classes: one wave.
+template <typename T, int NE, bool TAIL>
 __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restrict__ logits, DistillArgs a) {
-    __shared__ DistillPart red[W];
     __shared__ unsigned marks[TAIL ? kThreads : 1];
-    __shared__ unsigned repeated;
-    const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
-    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
-    if (unit >= a.units) return;
-    const long long row = a.splits == 1 ? unit : unit / a.splits;
-    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    const int lane = threadIdx.x & 63;
+    const long long row = block_index() * 4 + (threadIdx.x >> 6);
+    if (row >= a.units) return;
     if (a.live && !a.live[row]) {
-        if (tid == 0 && a.splits == 1) distill_dead(a, row);
+        if (lane == 0) distill_dead(a, row);
         return;
     }
     const T* z = logits + row * a.row_stride;
-    using S = Span<T, W, NE>;
-    const S span(split * S::kCols, a.cols, tid);
+    using S = Span<T, 1, NE>;
+    const S span(0, a.cols, lane);
     float v[NE];
     span.template load<true>(z, v);
     DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
     if constexpr (TAIL) {
-        unsigned* mine = marks + (W == 1 ? threadIdx.x - lane : 0);
-        mine[tid] = 0u;
-        if (W > 1 && tid == 0) repeated = 0u;
-        together<W>();
-        const int hi = span.base + S::kCols < a.cols ? span.base + S::kCols : a.cols;
-        bool twice = false;
-        for (int j = tid; j < a.k; j += W * 64) {
-            const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-            if (i < span.base || i >= hi) continue;
+        unsigned* mine = marks + (threadIdx.x - lane);
+        mine[lane] = 0u;
+        together<1>();
+        mark_entries<1>(a, z, row, 0, a.cols, nullptr, t, [&](int i) {
             int thread, e;
-            span.locate((int)i, thread, e);
-            twice |= (atomicOr(&mine[thread], 1u << e) >> e & 1u) != 0;
-        }
-        if constexpr (W == 1) {
-            twice = __ballot(twice) != 0;
-        } else {
-            if (twice) repeated = 1u;
-        }
-        together<W>();
-        if constexpr (W > 1) twice = repeated != 0;
-        const unsigned hit = mine[tid];
+            span.locate(i, thread, e);
+            return (atomicOr(&mine[thread], 1u << e) >> e & 1u) != 0;
+        });
+        const unsigned hit = mine[lane];
 #pragma unroll
         for (int e = 0; e < NE; ++e) v[e] = hit >> e & 1u ? -INFINITY : v[e];
-        for (int j = tid; j < a.k; j += W * 64) {
-            const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-            if (i < span.base || i >= hi) continue;
-            if (twice && named_before(a, row, j, i)) continue;
-            const float zi = ld(z, i);
-            merge(t.me, t.se, zi, zi == -INFINITY ? 0.0f : 1.0f, a.c, a.c_lo);
-        }
-        const float m = wave_max(t.me);
-        t.se = wave_sum(t.se == 0.0f ? 0.0f : t.se * power(t.me, m, a.c, a.c_lo));
-        t.me = m;
     }
     float m = v[0];
 #pragma unroll
@@ -764,18 +925,83 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
     const float mz = t.m == -INFINITY ? 0.0f : t.m;
     float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) s += power(v[e], mz, a.c, a.c_lo);
+    for (int e = 0; e < NE; ++e) s += power_of<T>(a, v[e], mz);
     t.s = wave_sum(s);
-    if constexpr (W > 1) {
-        if (lane == 0) red[threadIdx.x >> 6] = t;
-        together<W>();
-        if (tid >= 64) return;
-        t = red[0];
+    distill_finish(a, z, row, t);
+}
+
+// A part of a longer row, walked over as in logprobs_stream_kernel.  The marks are one bit a class of the part.
+template <typename T, int NE, bool TAIL>
+__global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __restrict__ logits, DistillArgs a) {
+    __shared__ DistillPart red[4];
+    __shared__ unsigned char marks[TAIL ? kMarkCols / 8 : 1] __attribute__((aligned(16)));
+    __shared__ unsigned repeated;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const long long unit = block_index();
+    if (unit >= a.units) return;
+    const long long row = a.splits == 1 ? unit : unit / a.splits;
+    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    if (a.live && !a.live[row]) {
+        if (tid == 0 && a.splits == 1) distill_dead(a, row);
+        return;
+    }
+    const T* z = logits + row * a.row_stride;
+    using S = Span<T, 4, NE>;
+    const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
+    unsigned raw[S::kWords];
+    S(lo, hi, tid).fetch(z, raw);
+    DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    if constexpr (TAIL) {
+        unsigned* words = reinterpret_cast<unsigned*>(marks);
+        for (int i = tid; i < (hi - lo + 31) / 32; i += kThreads) words[i] = 0u;
+        if (tid == 0) repeated = 0u;
+        __syncthreads();
+        mark_entries<4>(a, z, row, lo, hi, &repeated, t, [&](int i) {
+            const int b = i - lo;
+            return (atomicOr(&words[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) != 0;
+        });
+    }
+    float s = 0.0f;
+    for (int base = lo; base < hi; base += S::kCols) {
+        const S span(base, hi, tid);
+        float v[NE];
+        span.unpack(raw, v);
+        if (base + S::kCols < hi) S(base + S::kCols, hi, tid).fetch(z, raw);
+        if constexpr (TAIL) {
 #pragma unroll
-        for (int w = 1; w < W; ++w) {
-            merge(t.m, t.s, red[w].m, red[w].s, a.c, a.c_lo);
-            if constexpr (TAIL) merge(t.me, t.se, red[w].me, red[w].se, a.c, a.c_lo);
+            for (int q = 0; q < S::NV; ++q) {
+                const int first = span.start(q);
+                unsigned bits = 0;
+                if (first < hi) bits = (unsigned)marks[(first - lo) >> 3] >> ((first - lo) & 7);
+                if (__ballot(bits != 0)) {  // (the row's last vector lies `over` classes further down)
+                    const int over = first - span.offset(q);
+                    bits <<= over > 0 && over < S::VE ? over : 0;
+#pragma unroll
+                    for (int j = 0; j < S::VE; ++j) v[q * S::VE + j] = bits >> j & 1u ? -INFINITY : v[q * S::VE + j];
+                }
+            }
         }
+        float m = v[0];
+#pragma unroll
+        for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
+        m = wave_max(m);
+        if (m > t.m) {
+            if (t.m != -INFINITY) s *= power(t.m, m, a.c, a.c_lo);
+            t.m = m;
+        }
+        const float mz = t.m == -INFINITY ? 0.0f : t.m;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) s += power_of<T>(a, v[e], mz);
+    }
+    t.s = wave_sum(s);
+    if (lane == 0) red[tid >> 6] = t;
+    __syncthreads();
+    if (tid >= 64) return;
+    t = red[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        merge(t.m, t.s, red[w].m, red[w].s, a.c, a.c_lo);
+        if constexpr (TAIL) merge(t.me, t.se, red[w].me, red[w].se, a.c, a.c_lo);
     }
     if (a.splits == 1)
         distill_finish(a, z, row, t);
@@ -812,7 +1038,7 @@ struct DistillBwdArgs {
     const DistillStats* stats;
     const float* dloss;
     long long row_stride, units;
-    int class_bytes, cols, splits, k, tail;
+    int class_bytes, cols, splits, per, k, tail;
     float c, inv_t;
 };
 
@@ -827,7 +1053,8 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     const long long row = a.splits == 1 ? unit : unit / a.splits;
     const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
     using S = Span<T, W, NE>;
-    const S span(split * S::kCols, a.cols, tid);
+    const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
+    const S span(lo, hi, tid);
     T* d = dlogits + row * a.cols;
     const DistillStats st = a.stats[row];
     const bool zero = st.l2s == INFINITY;  // a dead row, or no class has probability
@@ -848,7 +1075,6 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     }
     if (zero || st.coef != st.coef) return;  // (NaN: an entry the row does not have; the whole row is)
     // the entries' classes once more, behind the dense part
-    const int lo = span.base, hi = span.base + S::kCols < a.cols ? span.base + S::kCols : a.cols;
     unsigned* mine = marks + (W == 1 ? threadIdx.x - lane : 0);
     mine[tid] = 0u;
     if (W > 1 && tid == 0) repeated = 0u;
@@ -886,24 +1112,38 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
-// How a row is cut: one wave for up to kWaveCols classes; beyond, workgroups of 256 threads with 32, 16 or 8 classes a
-// thread - the most that still leaves kUnits workgroups (four for each of the 256 CUs) for few rows.
-constexpr long long kUnits = 1024;
-constexpr int kMaxSplits = kMaxCols / (kThreads * 32);
+// How a row is cut: one wave for up to kWaveCols classes.  Beyond, the forward passes walk over parts of a row, as many
+// as give kUnits workgroups but of at least kWaveCols classes; the backward passes have nothing to join and take
+// workgroups of at most 32 classes a thread.  Parts are equal, of whole vectors.
+constexpr long long kUnits = 4096;
+constexpr int kMaxSplits = 128;
 struct Cut {
-    int waves, ne, splits;
+    int waves, ne, splits, per;
 };
-Cut cut_rows(long long rows, int cols) {
-    if (cols <= kWaveCols) {
-        int ne = 1;
-        while (64 * ne < cols) ne *= 2;
-        if (ne == 32 && cols <= 64 * 24) ne = 24;
-        return Cut{1, ne, 1};
-    }
+int equal_part(int cols, int splits) { return ((cols + splits - 1) / splits + 7) / 8 * 8; }
+Cut cut_wave(int cols) {
+    int ne = 1;
+    while (64 * ne < cols) ne *= 2;
+    if (ne == 32 && cols <= 64 * 24) ne = 24;
+    return Cut{1, ne, 1, cols};
+}
+Cut cut_forward(long long rows, int cols) {
+    if (cols <= kWaveCols) return cut_wave(cols);
+    long long splits = (kUnits + rows - 1) / (rows > 0 ? rows : 1);
+    const int most = cols / kWaveCols < kMaxSplits ? cols / kWaveCols : kMaxSplits, least = (cols + kMarkCols - 1) / kMarkCols;
+    splits = splits > most ? most : splits;
+    splits = splits < least ? least : splits;
+    const int per = equal_part(cols, (int)splits);
+    return Cut{4, 16, (cols + per - 1) / per, per};
+}
+Cut cut_backward(long long rows, int cols) {
+    if (cols <= kWaveCols) return cut_wave(cols);
     for (int ne = 8;; ne *= 2) {
         const int splits = (cols + kThreads * ne - 1) / (kThreads * ne);
         const int half = (cols + kThreads * 2 * ne - 1) / (kThreads * 2 * ne);
-        if (ne == 32 || (splits <= kMaxSplits && rows * half < kUnits)) return Cut{4, ne, splits};
+        if (ne < 32 && rows * half >= 1024) continue;  // (still four workgroups for each of the 256 CUs)
+        const int per = equal_part(cols, splits);
+        return Cut{4, ne, (cols + per - 1) / per, per};
     }
 }
 
@@ -913,83 +1153,87 @@ dim3 grid_of(long long units, int waves) {
     return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
 
-// F::template run<W, NE>(...) for a cut
+// F::template run<NE>(...) for a wave's cut
 template <typename F, typename... A>
-void with_cut(const Cut& cut, A&&... args) {
-    if (cut.waves == 4) {
-        if (cut.ne == 8) F::template run<4, 8>(args...);
-        else if (cut.ne == 16) F::template run<4, 16>(args...);
-        else F::template run<4, 32>(args...);
-    } else {
-        switch (cut.ne) {
-            case 1: F::template run<1, 1>(args...); break;
-            case 2: F::template run<1, 2>(args...); break;
-            case 4: F::template run<1, 4>(args...); break;
-            case 8: F::template run<1, 8>(args...); break;
-            case 16: F::template run<1, 16>(args...); break;
-            case 24: F::template run<1, 24>(args...); break;
-            default: F::template run<1, 32>(args...);
-        }
+void with_wave(int ne, A&&... args) {
+    switch (ne) {
+        case 1: F::template run<1>(args...); break;
+        case 2: F::template run<2>(args...); break;
+        case 4: F::template run<4>(args...); break;
+        case 8: F::template run<8>(args...); break;
+        case 16: F::template run<16>(args...); break;
+        case 24: F::template run<24>(args...); break;
+        default: F::template run<32>(args...);
     }
 }
 
-template <typename T>
+template <typename T, bool TOP>
 struct LogprobsFwd {
-    template <int W, int NE>
+    template <int NE>
     static void run(const void* logits, const LogprobsArgs& a, hipStream_t s) {
-        if (a.top > 0)
-            hipLaunchKernelGGL((logprobs_fwd_kernel<T, W, NE, true>), grid_of(a.units, W), dim3(kThreads), 0, s,
-                               static_cast<const T*>(logits), a);
-        else
-            hipLaunchKernelGGL((logprobs_fwd_kernel<T, W, NE, false>), grid_of(a.units, W), dim3(kThreads), 0, s,
-                               static_cast<const T*>(logits), a);
-    }
-};
-template <typename T>
-struct LogprobsJoin {
-    template <int W, int NE>
-    static void run(const void* logits, const LogprobsArgs& a, hipStream_t s) {
-        hipLaunchKernelGGL((logprobs_join_kernel<T, W, NE>), grid_of(a.units, W), dim3(kThreads), 0, s,
+        hipLaunchKernelGGL((logprobs_fwd_kernel<T, NE, TOP>), grid_of(a.units, 1), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a);
     }
+    static void launch(const Cut& cut, const void* logits, const LogprobsArgs& a, hipStream_t s) {
+        if (cut.waves == 1)
+            with_wave<LogprobsFwd>(cut.ne, logits, a, s);
+        else
+            hipLaunchKernelGGL((logprobs_stream_kernel<T, 16, TOP>), grid_of(a.units, 4), dim3(kThreads), 0, s,
+                               static_cast<const T*>(logits), a);
+    }
 };
+template <typename T, int W, int NE>
+void launch_join(const void* logits, const LogprobsArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((logprobs_join_kernel<T, W, NE>), grid_of(a.units, W), dim3(kThreads), 0, s,
+                       static_cast<const T*>(logits), a);
+}
 template <typename T>
 struct LogprobsBwd {
-    template <int W, int NE>
+    template <int NE, int W = 1>
     static void run(const void* logits, const LogprobsBwdArgs& a, void* dlogits, hipStream_t s) {
         hipLaunchKernelGGL((logprobs_bwd_kernel<T, W, NE>), grid_of(a.units, W), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a, static_cast<T*>(dlogits));
     }
 };
-template <typename T>
+template <typename T, bool TAIL>
 struct DistillFwd {
-    template <int W, int NE>
+    template <int NE>
     static void run(const void* logits, const DistillArgs& a, hipStream_t s) {
-        if (a.tail)
-            hipLaunchKernelGGL((distill_fwd_kernel<T, W, NE, true>), grid_of(a.units, W), dim3(kThreads), 0, s,
-                               static_cast<const T*>(logits), a);
+        hipLaunchKernelGGL((distill_fwd_kernel<T, NE, TAIL>), grid_of(a.units, 1), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits), a);
+    }
+    static void launch(const Cut& cut, const void* logits, const DistillArgs& a, hipStream_t s) {
+        if (cut.waves == 1)
+            with_wave<DistillFwd>(cut.ne, logits, a, s);
         else
-            hipLaunchKernelGGL((distill_fwd_kernel<T, W, NE, false>), grid_of(a.units, W), dim3(kThreads), 0, s,
+            hipLaunchKernelGGL((distill_stream_kernel<T, 16, TAIL>), grid_of(a.units, 4), dim3(kThreads), 0, s,
                                static_cast<const T*>(logits), a);
     }
 };
 template <typename T>
 struct DistillBwd {
-    template <int W, int NE>
+    template <int NE, int W = 1>
     static void run(const void* logits, const DistillBwdArgs& a, void* dlogits, hipStream_t s) {
         hipLaunchKernelGGL((distill_bwd_kernel<T, W, NE>), grid_of(a.units, W), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a, static_cast<T*>(dlogits));
     }
 };
+template <typename F, typename... A>
+void launch_backward(const Cut& cut, A&&... args) {
+    if (cut.waves == 1) with_wave<F>(cut.ne, args...);
+    else if (cut.ne == 8) F::template run<8, 4>(args...);
+    else if (cut.ne == 16) F::template run<16, 4>(args...);
+    else F::template run<32, 4>(args...);
+}
 
 // The keys of a row's parts: one wave while they fit its registers.
-Cut cut_keys(int n) {
-    if (n <= 64 * 32) {
-        int ne = 4;
-        while (64 * ne < n) ne *= 2;
-        return Cut{1, ne, 1};
-    }
-    return Cut{4, n <= kThreads * 16 ? 16 : 32, 1};
+template <typename T>
+void join_parts(int n, const void* logits, const LogprobsArgs& a, hipStream_t s) {
+    if (n <= 64 * 4) launch_join<T, 1, 4>(logits, a, s);
+    else if (n <= 64 * 8) launch_join<T, 1, 8>(logits, a, s);
+    else if (n <= kThreads * 4) launch_join<T, 4, 4>(logits, a, s);
+    else if (n <= kThreads * 8) launch_join<T, 4, 8>(logits, a, s);
+    else launch_join<T, 4, 32>(logits, a, s);
 }
 
 int check_call(const char* who, long long row_stride, int rows, int cols, int dtype, float temperature) {
@@ -1032,7 +1276,7 @@ void scale_of(float temperature, float& c, float& c_lo, float& inv_t) {
 
 extern "C" long long isg_token_logprobs_workspace_bytes(int rows, int cols, int top) {
     if (rows < 0 || cols < 1 || cols > kMaxCols || top < 0 || top > kMaxTop) return -1;
-    const Cut cut = cut_rows(rows, cols);
+    const Cut cut = cut_forward(rows, cols);
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * ((long long)sizeof(Sums) + 8 * top) + 8;
 }
 
@@ -1050,7 +1294,7 @@ extern "C" int isg_token_logprobs_fwd(const void* logits, long long row_stride, 
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && entropy && (!tokens || logprobs) && (top == 0 || (top_logprobs && top_classes)), ISG_EINVAL,
                 "%s: null pointer", who);
-    const Cut cut = cut_rows(rows, cols);
+    const Cut cut = cut_forward(rows, cols);
     ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     ISG_REQUIRE(((uintptr_t)workspace | (uintptr_t)stats) % 8 == 0 && (uintptr_t)stats % 16 == 0, ISG_EINVAL,
                 "%s: workspace and stats must be aligned to 8 and 16 bytes", who);
@@ -1059,7 +1303,7 @@ extern "C" int isg_token_logprobs_fwd(const void* logits, long long row_stride, 
     a.tokens = tokens, a.live = live, a.logprobs = tokens ? logprobs : nullptr, a.entropy = entropy;
     a.top_logprobs = top_logprobs, a.top_classes = top_classes, a.stats = stats;
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
-    a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.top = top;
+    a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.top = top;
     float c_lo;
     scale_of(temperature, a.c, c_lo, a.inv_t);
     a.c_rel = c_lo / a.c;
@@ -1067,14 +1311,16 @@ extern "C" int isg_token_logprobs_fwd(const void* logits, long long row_stride, 
         a.part_keys = static_cast<u64*>(workspace);
         a.part = reinterpret_cast<Sums*>(a.part_keys + a.units * top);
     }
-    if (dtype == ISG_F32) with_cut<LogprobsFwd<float>>(cut, logits, a, s);
-    else with_cut<LogprobsFwd<__hip_bfloat16>>(cut, logits, a, s);
+    if (dtype == ISG_F32)
+        top > 0 ? LogprobsFwd<float, true>::launch(cut, logits, a, s) : LogprobsFwd<float, false>::launch(cut, logits, a, s);
+    else
+        top > 0 ? LogprobsFwd<__hip_bfloat16, true>::launch(cut, logits, a, s)
+                : LogprobsFwd<__hip_bfloat16, false>::launch(cut, logits, a, s);
     rc = isg::check_launch("logprobs_fwd_kernel");
     if (rc != ISG_OK || cut.splits == 1) return rc;
     a.units = rows;
-    const Cut join = cut_keys(cut.splits * top);
-    if (dtype == ISG_F32) with_cut<LogprobsJoin<float>>(join, logits, a, s);
-    else with_cut<LogprobsJoin<__hip_bfloat16>>(join, logits, a, s);
+    if (dtype == ISG_F32) join_parts<float>(cut.splits * top, logits, a, s);
+    else join_parts<__hip_bfloat16>(cut.splits * top, logits, a, s);
     return isg::check_launch("logprobs_join_kernel");
 }
 
@@ -1093,23 +1339,23 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
     ISG_REQUIRE(logits && stats && dlogits && (!dlogprobs || tokens) && (!dtop_logprobs || (top > 0 && top_classes)),
                 ISG_EINVAL, "%s: null pointer", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
-    const Cut cut = cut_rows(rows, cols);
+    const Cut cut = cut_backward(rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
     LogprobsBwdArgs a{};
     a.tokens = tokens, a.top_classes = top_classes, a.stats = stats;
     a.dlogprobs = dlogprobs, a.dentropy = dentropy, a.dtop = dtop_logprobs;
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
-    a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.top = top;
+    a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.top = top;
     float c_lo;
     scale_of(temperature, a.c, c_lo, a.inv_t);
-    if (dtype == ISG_F32) with_cut<LogprobsBwd<float>>(cut, logits, a, dlogits, s);
-    else with_cut<LogprobsBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
+    if (dtype == ISG_F32) launch_backward<LogprobsBwd<float>>(cut, logits, a, dlogits, s);
+    else launch_backward<LogprobsBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
     return isg::check_launch("logprobs_bwd_kernel");
 }
 
 extern "C" long long isg_distill_workspace_bytes(int rows, int cols) {
     if (rows < 0 || cols < 1 || cols > kMaxCols) return -1;
-    const Cut cut = cut_rows(rows, cols);
+    const Cut cut = cut_forward(rows, cols);
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * (long long)sizeof(DistillPart);
 }
 
@@ -1125,17 +1371,21 @@ extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const f
     if (rc != ISG_OK) return rc;
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && loss, ISG_EINVAL, "%s: null pointer", who);
-    const Cut cut = cut_rows(rows, cols);
+    const Cut cut = cut_forward(rows, cols);
     ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
     DistillArgs a{};
     a.values = values, a.classes = classes, a.live = live, a.loss = loss;
     a.stats = reinterpret_cast<DistillStats*>(stats), a.part = static_cast<DistillPart*>(workspace);
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
-    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.k = k, a.tail = tail;
+    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.k = k, a.tail = tail;
     scale_of(temperature, a.c, a.c_lo, a.inv_t);
-    if (dtype == ISG_F32) with_cut<DistillFwd<float>>(cut, logits, a, s);
-    else with_cut<DistillFwd<__hip_bfloat16>>(cut, logits, a, s);
+    a.c_near = (float)(1.4426950408889634074 / (double)temperature);
+    if (dtype == ISG_F32)
+        tail ? DistillFwd<float, true>::launch(cut, logits, a, s) : DistillFwd<float, false>::launch(cut, logits, a, s);
+    else
+        tail ? DistillFwd<__hip_bfloat16, true>::launch(cut, logits, a, s)
+             : DistillFwd<__hip_bfloat16, false>::launch(cut, logits, a, s);
     rc = isg::check_launch("distill_fwd_kernel");
     if (rc != ISG_OK || cut.splits == 1) return rc;
     a.units = rows;
@@ -1161,15 +1411,15 @@ extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const f
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && stats && dloss && dlogits, ISG_EINVAL, "%s: null pointer", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
-    const Cut cut = cut_rows(rows, cols);
+    const Cut cut = cut_backward(rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
     DistillBwdArgs a{};
     a.values = values, a.classes = classes, a.stats = reinterpret_cast<const DistillStats*>(stats), a.dloss = dloss;
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
-    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.k = k, a.tail = tail;
+    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.k = k, a.tail = tail;
     float c_lo;
     scale_of(temperature, a.c, c_lo, a.inv_t);
-    if (dtype == ISG_F32) with_cut<DistillBwd<float>>(cut, logits, a, dlogits, s);
-    else with_cut<DistillBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
+    if (dtype == ISG_F32) launch_backward<DistillBwd<float>>(cut, logits, a, dlogits, s);
+    else launch_backward<DistillBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
     return isg::check_launch("distill_bwd_kernel");
 }
