@@ -8,10 +8,8 @@
 // nothing (its x is kept from meeting 0 * inf by a lower bound far below the smallest float).  All sums are float.
 //
 // Layout.  A row is read once, into registers: up to 2,048 classes by one wave (four rows to a workgroup, no barrier),
-// longer ones in chunks of 2,048 to 8,192 by a workgroup each, whose partial results (maximum, sums, best classes) a
-// second launch joins.  Loads are 16 bytes a lane at whatever alignment the row has (rows of 785 bf16 logits start on
-// any even address); the last vector of a row is the row's last 16 bytes, and what it repeats of its neighbour is
-// blanked.
+// longer ones by workgroups that walk over equal parts of it, whose results (maximum, sums, best classes) a second
+// launch joins.
 #include <hip/hip_bf16.h>
 
 #include <math.h>
@@ -28,10 +26,11 @@ constexpr int kThreads = 256;
 constexpr int kMaxTop = ISG_TOP_MAX;          // classes kept per row
 constexpr int kMaxEntries = ISG_DISTILL_MAX;  // a teacher's classes per row
 constexpr int kMaxCols = ISG_CLASSES_MAX;     // class axis
-constexpr int kWaveCols = 2048;               // classes one wave holds (32 registers a lane)
+constexpr int kWaveCols = 2048;               // classes one wave holds at most (32 registers a lane)
 constexpr int kCandidates = 256;              // alternatives in question per wave; a workgroup holds four times as many
 constexpr int kListMax = 1024;                // alternatives a workgroup collects along its part of a row
-constexpr int kListTrim = 256;                // ... before it goes back to the best
+constexpr int kListTrim = 256;                // ... before it goes back to the best, of which it may keep
+constexpr int kListKeep = 128;                // this many
 
 typedef unsigned long long u64;
 
@@ -130,60 +129,71 @@ __device__ __forceinline__ void store_vector(__hip_bfloat16* p, const float* v) 
     }
 }
 
-// Where the elements of a thread lie in its row: NE of them in vectors of VE, `threads` vectors of a slot side by side.
-// A vector that would end behind the row is the row's last VE elements; `blank` of them belong to its neighbour.
+// Where the elements of a thread lie in its unit's part [lo, hi) of a row: NE of them in vectors of VE (16 bytes), the
+// vectors of a slot side by side over the unit's W * 64 threads, on 16-byte boundaries of memory from `first` <= lo on.
+// (Two-byte boundaries cost a 16-byte load three to four cache accesses instead of one.)  The part's first and last
+// vector may reach outside; they are read from lo and up to hi instead, and `start` tells which of their elements are
+// this thread's own.
 template <typename T, int W, int NE>
 struct Span {
     static constexpr int VE = NE < 16 / (int)sizeof(T) ? NE : 16 / (int)sizeof(T);
     static constexpr int NV = NE / VE;
-    static constexpr int kCols = W * 64 * NE;  // of one unit (a wave or a workgroup)
-    int base, cols, lane;                      // cols: where the unit ends; lane: of its W * 64
+    static constexpr int kCols = W * 64 * NE;
+    int lo, hi, first, lane;  // lane: of the unit's W * 64
 
-    __device__ __forceinline__ Span(int base_, int cols_, int lane_) : base(base_), cols(cols_), lane(lane_) {}
-    __device__ __forceinline__ int start(int slot) const { return base + (slot * W * 64 + lane) * VE; }
-    __device__ __forceinline__ bool full(int slot) const { return base + (slot + 1) * W * 64 * VE <= cols; }  // (uniform)
-    __device__ __forceinline__ bool empty(int slot) const { return base + slot * W * 64 * VE >= cols; }       // (uniform)
-    __device__ __forceinline__ int offset(int slot) const {
-        const int s = start(slot);
-        return s < cols - VE ? s : cols - VE;
+    // z: the row, whose memory the vectors are aligned in
+    __device__ __forceinline__ Span(const T* z, int lo_, int hi_, int lane_) : lo(lo_), hi(hi_), lane(lane_) {
+        first = lo - (int)(((uintptr_t)z / sizeof(T) + (unsigned)lo) % VE);
     }
-    // the class of element e, or -1 where it is not this thread's (or another unit's)
+    __device__ __forceinline__ void next() { first += kCols; }  // to the following kCols classes
+    __device__ __forceinline__ bool more() const { return first < hi; }
+    __device__ __forceinline__ bool whole() const { return first >= lo && first + kCols <= hi; }  // (uniform)
+    __device__ __forceinline__ bool empty(int slot) const { return first + slot * W * 64 * VE >= hi; }  // (uniform)
+    __device__ __forceinline__ int start(int slot) const { return first + (slot * W * 64 + lane) * VE; }
+    __device__ __forceinline__ int inside(int s) const {
+        s = s < hi - VE ? s : hi - VE;
+        return s > lo ? s : lo;
+    }
+    // the class of element e, or -1 where it is another thread's (or none)
     __device__ __forceinline__ int cls(int e) const {
-        const int s = start(e / VE), i = offset(e / VE) + e % VE;
-        return i >= s ? i : -1;
+        const int s = start(e / VE), i = inside(s) + e % VE;
+        return i >= s && i < s + VE ? i : -1;
     }
-    // thread and element of a class inside the unit
+    // thread and element of a class of the unit
     __device__ __forceinline__ void locate(int c, int& thread, int& e) const {
-        const int l = c - base, vec = l / VE, s = base + vec * VE;
-        const int over = s + VE - cols;
+        const int vec = (c - first) / VE;
         thread = vec % (W * 64);
-        e = vec / (W * 64) * VE + l % VE + (over > 0 ? over : 0);
+        e = vec / (W * 64) * VE + c - inside(first + vec * VE);
     }
     // the elements; those that are not this thread's as -inf (BLANK) or as whatever class lies there
     template <bool BLANK>
     __device__ __forceinline__ void load(const T* z, float (&v)[NE]) const {
 #pragma unroll
         for (int t = 0; t < NV; ++t) {
-            if (full(t)) {
-                load_vector<VE>(z + start(t), v + t * VE);
-            } else if (!empty(t)) {
-                const int s = start(t), o = offset(t);
-                load_vector<VE>(z + o, v + t * VE);
-                if constexpr (BLANK) {
-#pragma unroll
-                    for (int j = 0; j < VE; ++j) v[t * VE + j] = o + j >= s ? v[t * VE + j] : -INFINITY;
-                }
+            if (!empty(t)) {
+                load_vector<VE>(z + inside(start(t)), v + t * VE);
             } else {
 #pragma unroll
                 for (int j = 0; j < VE; ++j) v[t * VE + j] = -INFINITY;
             }
+        }
+        if constexpr (BLANK) blank(v);
+    }
+    __device__ __forceinline__ void blank(float (&v)[NE]) const {
+#pragma unroll
+        for (int t = 0; t < NV; ++t) {
+            const int f = first + t * W * 64 * VE;
+            if (f >= lo && f + W * 64 * VE <= hi) continue;  // (uniform)
+            const int s = start(t), from = s - inside(s);    // own: from <= j < from + VE
+#pragma unroll
+            for (int j = 0; j < VE; ++j) v[t * VE + j] = j >= from && j < from + VE ? v[t * VE + j] : -INFINITY;
         }
     }
     // the same in two halves, for loads that are on their way while other elements are worked on
     static constexpr int kWords = NE * (int)sizeof(T) / 4;
     __device__ __forceinline__ void fetch(const T* z, unsigned (&raw)[kWords]) const {
 #pragma unroll
-        for (int t = 0; t < NV; ++t) __builtin_memcpy(raw + t * (kWords / NV), z + offset(t), 16);
+        for (int t = 0; t < NV; ++t) __builtin_memcpy(raw + t * (kWords / NV), z + inside(start(t)), 16);
     }
     __device__ __forceinline__ void unpack(const unsigned (&raw)[kWords], float (&v)[NE]) const {
 #pragma unroll
@@ -191,28 +201,12 @@ struct Span {
             if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[i]);
             else v[2 * i] = __uint_as_float(raw[i] << 16), v[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
         }
-        if (base + kCols <= cols) return;
-#pragma unroll
-        for (int t = 0; t < NV; ++t) {
-            const int s = start(t), o = offset(t);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) v[t * VE + j] = o + j >= s ? v[t * VE + j] : -INFINITY;
-        }
+        if (!whole()) blank(v);
     }
-    // a slot's gradients; the row's last vector repeats values of its neighbour, which is no harm inside the unit
+    // a slot's gradients (what the outer vectors repeat of their neighbours they repeat with the same values)
     __device__ __forceinline__ void store(T* d, int t, const float* o) const {
-        const int s = start(t), at = offset(t);
-        if (full(t)) {
-            store_vector<VE>(d + s, o);
-        } else if (s < cols) {
-            if (at >= base) {
-                store_vector<VE>(d + at, o);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VE; ++j)
-                    if (at + j >= s) store_vector<1>(d + at + j, o + j);
-            }
-        }
+        const int s = start(t);
+        if (s < hi) store_vector<VE>(d + inside(s), o);
     }
 };
 
@@ -231,6 +225,8 @@ __device__ __forceinline__ unsigned order_bits(float v) {
 __device__ __forceinline__ float order_value(unsigned k) {
     return k == 1u ? NAN : __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+// the next float in that order: v > x where v >= above(x)
+__device__ __forceinline__ float above(float x) { return order_value(order_bits(x) + 1u); }
 __device__ __forceinline__ u64 order_key(float v, int c) { return ((u64)order_bits(v) << 32) | (unsigned)~c; }
 
 // log p of a logit; a row without any probability (log2 s = +inf) gives -inf.  In nats throughout: at T = 1 the
@@ -252,6 +248,23 @@ struct TopShared {
     unsigned count;
     u64 best[4];
 };
+
+__device__ __forceinline__ unsigned group_bound(float lane_max, int k, TopShared<4>& sh) {
+    const int lane = threadIdx.x & 63;
+    sh.group[threadIdx.x] = order_bits(lane_max) >> 16;
+    __syncthreads();
+    unsigned g[4], bound = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) g[q] = sh.group[q * 64 + lane];
+    for (int bit = 15; bit >= 0; --bit) {
+        const unsigned t = bound | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) n += __builtin_popcountll(__ballot(g[q] >= t));
+        if (n >= k) bound = t;
+    }
+    return bound;
+}
 
 template <int W, int NE, typename Reload, typename Emit>
 __device__ __forceinline__ void select_top(const float (&v)[NE], int k, TopShared<W>& sh, Reload reload, Emit emit) {
@@ -291,25 +304,14 @@ __device__ __forceinline__ void select_top(const float (&v)[NE], int k, TopShare
         }
     } else {
         if (tid == 0) sh.count = 0;
-        sh.group[tid] = order_bits(gm[0]) >> 16;
-        together<W>();
-        unsigned g[W];
-#pragma unroll
-        for (int q = 0; q < W; ++q) g[q] = sh.group[q * 64 + lane];
-        for (int bit = 15; bit >= 0; --bit) {
-            const unsigned t = bound | (1u << bit);
-            int n = 0;
-#pragma unroll
-            for (int q = 0; q < W; ++q) n += __builtin_popcountll(__ballot(g[q] >= t));
-            if (n >= k) bound = t;
-        }
+        bound = group_bound(gm[0], k, sh);
     }
     int total = kCap + 1;
     if (bound > 0x7fu) {  // (0x7f begins the key of -inf)
         const float low = order_value(bound << 16);
         unsigned hit = 0;
 #pragma unroll
-        for (int e = 0; e < NE; ++e) hit |= (v[e] >= low ? 1u : 0u) << e;
+        for (int e = NE - 1; e >= 0; --e) hit = hit + hit + (v[e] >= low ? 1u : 0u);
         const int mine = __builtin_popcount(hit);
         int at;
         if constexpr (W == 1) {
@@ -472,7 +474,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restr
         return;
     }
     const T* z = logits + row * a.row_stride;
-    const Span<T, 1, NE> span(0, a.cols, lane);
+    const Span<T, 1, NE> span(z, 0, a.cols, lane);
     float v[NE];
     span.template load<true>(z, v);
     const RowStats r = row_stats(wave_sums(v, a.c), a.c_rel);
@@ -487,35 +489,77 @@ __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restr
             [&](int place, u64 k) { row_alternative(a, row, r, place, k); });
 }
 
-// What a workgroup has found of a part of a row's best classes so far.
+// What a workgroup has found of a part of a row's best classes so far: the k first are among them, in no order.
 struct TopList {
-    u64 keys[kListMax];  // in no order beyond the first `top` after a prune
-    u64 sorted[kMaxTop];
+    u64 keys[kListMax];
+    u64 kept[kListKeep];
     int count;
 };
 
-// The k first keys of the list, in order, to its front.  Uniform over the workgroup; returns the new count.
-__device__ __forceinline__ int prune(TopList& list, int count, int k) {
+// The largest 16-bit prefix that at least k of the n keys (n <= kListMax) reach; uniform, every wave for itself.
+template <int Q>
+__device__ __forceinline__ unsigned prefix_of(const u64* keys, int n, int k) {
+    const int lane = threadIdx.x & 63;
+    unsigned g[Q], bound = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) g[q] = q * 64 + lane < n ? (unsigned)(keys[q * 64 + lane] >> 48) : 0u;
+    for (int bit = 15; bit >= 0; --bit) {
+        const unsigned t = bound | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) c += __builtin_popcountll(__ballot(g[q] >= t));
+        if (c >= k) bound = t;
+    }
+    return bound;
+}
+
+// The k first keys of the list in order, through emit(place, key): the place of a key is the number of keys above it.
+template <typename Emit>
+__device__ __forceinline__ void rank_list(const TopList& list, int count, int k, Emit emit) {
     for (int r = threadIdx.x; r < count; r += kThreads) {
         const u64 own = list.keys[r];
         int place = 0;
 #pragma unroll 4
         for (int o = 0; o < count; ++o) place += list.keys[o] > own ? 1 : 0;
-        if (place < k) list.sorted[place] = own;
+        if (place < k) emit(place, own);
+    }
+}
+
+// Cuts the list back: what does not reach the prefix of its k-th key goes; where ties leave too much, all but the k
+// first.  Returns the new count; `low` is a value that a class behind all of these has to exceed.
+__device__ __forceinline__ int trim_list(TopList& list, int count, int k, float& low) {
+    const unsigned bound = count <= 4 * 64 ? prefix_of<4>(list.keys, count, k)
+                                           : (count <= 8 * 64 ? prefix_of<8>(list.keys, count, k)
+                                                              : prefix_of<kListMax / 64>(list.keys, count, k));
+    if (threadIdx.x == 0) list.count = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < count; r += kThreads) {
+        const u64 own = list.keys[r];
+        if ((unsigned)(own >> 48) >= bound) {
+            const int at = atomicAdd(&list.count, 1);
+            if (at < kListKeep) list.kept[at] = own;
+        }
     }
     __syncthreads();
-    const int n = count < k ? count : k;
-    for (int r = threadIdx.x; r < n; r += kThreads) list.keys[r] = list.sorted[r];
+    int n = list.count;
+    if (n > kListKeep) {
+        rank_list(list, count, k, [&](int place, u64 key) { list.kept[place] = key; });
+        __syncthreads();
+        n = count < k ? count : k;
+    }
+    for (int r = threadIdx.x; r < n; r += kThreads) list.keys[r] = list.kept[r];
     __syncthreads();
+    low = order_value(bound << 16);
     return n;
 }
 
 // A part of a longer row: a workgroup walks over it, kThreads * NE classes at a time, the next ones being loaded
-// meanwhile.  Every wave keeps its own maximum and its lanes their own sums until the end.  Of the best classes the
-// first step finds its k by select_top; what a later step has above the k-th of the list joins the list, which is cut
-// back to k when it has grown to kListTrim.  Steps that would overrun it (rising rows) go through select_top as well.
+// meanwhile.  Every wave keeps its own maximum and its lanes their own sums until the end.  The best classes gather in
+// a list: of the first step all that reach the bound select_top would take (see there), of the later steps what exceeds
+// the list's own bound, which rises whenever the list has grown to kListTrim and is cut back.  Steps that would overrun
+// the list (rising rows, ties) or have no finite bound hand it their k first by select_top instead.
 template <typename T, int NE, bool TOP>
-__global__ __launch_bounds__(kThreads, 8) void logprobs_stream_kernel(const T* __restrict__ logits, LogprobsArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 6) void logprobs_stream_kernel(const T* __restrict__ logits, LogprobsArgs a) {
     __shared__ float red[4][4];
     __shared__ typename std::conditional<TOP, TopShared<4>, char>::type shared;
     __shared__ typename std::conditional<TOP, TopList, char>::type list;
@@ -531,17 +575,19 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_stream_kernel(const T* _
     const T* z = logits + row * a.row_stride;
     using S = Span<T, 4, NE>;
     const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
+    S ahead(z, lo, hi, tid);
     unsigned raw[S::kWords];
-    S(lo, hi, tid).fetch(z, raw);
+    ahead.fetch(z, raw);
     Sums t{-INFINITY, 0.0f, 0.0f};  // (m of the wave; s, u of the lane)
     int count = 0;
-    float low = -INFINITY;   // what a further class has to exceed
-    bool trusted = false;    // ... where the list holds k real classes
-    for (int base = lo; base < hi; base += S::kCols) {
-        const S span(base, hi, tid);
+    float low = -INFINITY;  // what a further class has to exceed ...
+    bool bounded = false;   // ... once the list holds k classes above some finite value
+    while (ahead.more()) {
+        const S span = ahead;
         float v[NE];
         span.unpack(raw, v);
-        if (base + S::kCols < hi) S(base + S::kCols, hi, tid).fetch(z, raw);
+        ahead.next();
+        if (ahead.more()) ahead.fetch(z, raw);
         float m = v[0];
 #pragma unroll
         for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
@@ -563,17 +609,24 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_stream_kernel(const T* _
                 const int i = span.cls(e);
                 return i < 0 ? 0ull : order_key(ld(z, i), i);
             };
-            bool select = !trusted;
-            if (trusted) {
+            float reach = above(low);
+            bool fits = true;
+            if (!bounded) {
+                const unsigned bound = group_bound(lane_max, a.top, shared);
+                fits = bound > 0x7fu;
+                low = order_value(bound << 16);
+                reach = low;  // (classes of one step are not in order: those at the bound count as well)
+            }
+            if (tid == 0) list.count = count;
+            __syncthreads();
+            if (fits) {
                 unsigned hit = 0;
-                if (__ballot(lane_max > low)) {
+                if (__ballot(lane_max >= reach)) {
 #pragma unroll
-                    for (int e = 0; e < NE; ++e) hit |= (v[e] > low ? 1u : 0u) << e;
+                    for (int e = NE - 1; e >= 0; --e) hit = hit + hit + (v[e] >= reach ? 1u : 0u);
                 }
-                if (tid == 0) list.count = count;
-                __syncthreads();
-                int at = 0;
                 const int mine = __builtin_popcount(hit);
+                int at = 0;
                 if (mine) at = atomicAdd(&list.count, mine);
                 if (at + mine <= kListMax)
                     while (hit) {
@@ -583,22 +636,21 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_stream_kernel(const T* _
                     }
                 __syncthreads();
                 const int total = list.count;
-                select = total > kListMax;
-                if (!select) count = total;
+                fits = total <= kListMax;
+                if (fits) count = total, bounded = true;
             }
-            if (select) {
-                if (count > a.top) count = prune(list, count, a.top);
-                select_top<4, NE>(
-                    v, a.top, shared, reload,
-                    [&](int place, u64 k) { list.keys[count + place] = k; });
+            if (!fits) {
+                if (count > kListMax - kMaxTop) {
+                    float unused;
+                    count = trim_list(list, count, a.top, unused);
+                }
+                select_top<4, NE>(v, a.top, shared, reload, [&](int place, u64 k) { list.keys[count + place] = k; });
                 __syncthreads();
                 count += a.top;
             }
-            if (select || count > kListTrim) {
-                count = prune(list, count, a.top);
-                const unsigned kth = (unsigned)(list.keys[a.top - 1] >> 32);
-                trusted = count == a.top && kth > 1u;  // (0: fewer classes than that so far; 1: NaN)
-                low = order_value(kth);
+            if (count > kListTrim || !fits) {
+                count = trim_list(list, count, a.top, low);
+                bounded = low > -INFINITY;  // (no bound from classes at -inf or NaN)
             }
         }
     }
@@ -617,12 +669,11 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_stream_kernel(const T* _
         a.part[unit] = t;
     }
     if constexpr (TOP) {
-        if (count > a.top) count = prune(list, count, a.top);
-        for (int j = tid; j < a.top; j += kThreads) {
-            const u64 k = j < count ? list.keys[j] : 0ull;
-            if (a.splits == 1) row_alternative(a, row, r, j, k);
-            else a.part_keys[unit * a.top + j] = k;
-        }
+        if (count > 2 * a.top) count = trim_list(list, count, a.top, low);
+        rank_list(list, count, a.top, [&](int place, u64 key) {
+            if (a.splits == 1) row_alternative(a, row, r, place, key);
+            else a.part_keys[unit * a.top + place] = key;
+        });
     }
 }
 
@@ -689,8 +740,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restr
     const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
     using S = Span<T, W, NE>;
     const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
-    const S span(lo, hi, tid);
     T* d = dlogits + row * a.cols;
+    const S span(d, lo, hi, tid);  // (aligned as the gradient; dense logits lie the same way)
     const float m = a.stats[4 * row], l2s = a.stats[4 * row + 1], H = a.stats[4 * row + 2];
     const bool zero = l2s == INFINITY;  // a dead row, or no class has probability: nothing to move
     const T* z = logits + row * a.row_stride;
@@ -901,7 +952,7 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
     }
     const T* z = logits + row * a.row_stride;
     using S = Span<T, 1, NE>;
-    const S span(0, a.cols, lane);
+    const S span(z, 0, a.cols, lane);
     float v[NE];
     span.template load<true>(z, v);
     DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
@@ -934,7 +985,7 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
 template <typename T, int NE, bool TAIL>
 __global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __restrict__ logits, DistillArgs a) {
     __shared__ DistillPart red[4];
-    __shared__ unsigned char marks[TAIL ? kMarkCols / 8 : 1] __attribute__((aligned(16)));
+    __shared__ unsigned char marks[TAIL ? kMarkCols / 8 + 4 : 4] __attribute__((aligned(16)));
     __shared__ unsigned repeated;
     const int tid = threadIdx.x, lane = tid & 63;
     const long long unit = block_index();
@@ -949,33 +1000,36 @@ __global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __res
     using S = Span<T, 4, NE>;
     const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
     unsigned raw[S::kWords];
-    S(lo, hi, tid).fetch(z, raw);
+    S ahead(z, lo, hi, tid);
+    const int zero = ahead.first;  // the class of the first mark
+    ahead.fetch(z, raw);
     DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
     if constexpr (TAIL) {
         unsigned* words = reinterpret_cast<unsigned*>(marks);
-        for (int i = tid; i < (hi - lo + 31) / 32; i += kThreads) words[i] = 0u;
+        for (int i = tid; i < (hi - zero + 31) / 32; i += kThreads) words[i] = 0u;
         if (tid == 0) repeated = 0u;
         __syncthreads();
         mark_entries<4>(a, z, row, lo, hi, &repeated, t, [&](int i) {
-            const int b = i - lo;
+            const int b = i - zero;
             return (atomicOr(&words[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) != 0;
         });
     }
     float s = 0.0f;
-    for (int base = lo; base < hi; base += S::kCols) {
-        const S span(base, hi, tid);
+    while (ahead.more()) {
+        const S span = ahead;
         float v[NE];
         span.unpack(raw, v);
-        if (base + S::kCols < hi) S(base + S::kCols, hi, tid).fetch(z, raw);
+        ahead.next();
+        if (ahead.more()) ahead.fetch(z, raw);
         if constexpr (TAIL) {
 #pragma unroll
             for (int q = 0; q < S::NV; ++q) {
-                const int first = span.start(q);
+                const int first = span.start(q), b = first - zero;
                 unsigned bits = 0;
-                if (first < hi) bits = (unsigned)marks[(first - lo) >> 3] >> ((first - lo) & 7);
-                if (__ballot(bits != 0)) {  // (the row's last vector lies `over` classes further down)
-                    const int over = first - span.offset(q);
-                    bits <<= over > 0 && over < S::VE ? over : 0;
+                if (first < hi) bits = (unsigned)marks[b >> 3] >> (b & 7) & ((1u << S::VE) - 1u);
+                if (__ballot(bits != 0)) {
+                    const int from = first - span.inside(first);  // (an outer vector is read from further in)
+                    bits = from >= 0 ? bits << from : bits >> -from;
 #pragma unroll
                     for (int j = 0; j < S::VE; ++j) v[q * S::VE + j] = bits >> j & 1u ? -INFINITY : v[q * S::VE + j];
                 }
@@ -1054,8 +1108,8 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
     using S = Span<T, W, NE>;
     const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
-    const S span(lo, hi, tid);
     T* d = dlogits + row * a.cols;
+    const S span(d, lo, hi, tid);  // (aligned as the gradient; dense logits lie the same way)
     const DistillStats st = a.stats[row];
     const bool zero = st.l2s == INFINITY;  // a dead row, or no class has probability
     const T* z = logits + row * a.row_stride;
@@ -1112,23 +1166,25 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
-// How a row is cut: one wave for up to kWaveCols classes.  Beyond, the forward passes walk over parts of a row, as many
+// How a row is cut: one wave for what its registers hold.  Beyond, the forward passes walk over parts of a row, as many
 // as give kUnits workgroups but of at least kWaveCols classes; the backward passes have nothing to join and take
-// workgroups of at most 32 classes a thread.  Parts are equal, of whole vectors.
+// workgroups of at most 32 classes a thread.  Parts are equal but for the rounding to 8 classes.  (`ve - 1` classes of
+// room for a part that starts between two 16-byte boundaries.)
 constexpr long long kUnits = 4096;
 constexpr int kMaxSplits = 128;
 struct Cut {
     int waves, ne, splits, per;
 };
 int equal_part(int cols, int splits) { return ((cols + splits - 1) / splits + 7) / 8 * 8; }
-Cut cut_wave(int cols) {
-    int ne = 1;
-    while (64 * ne < cols) ne *= 2;
-    if (ne == 32 && cols <= 64 * 24) ne = 24;
-    return Cut{1, ne, 1, cols};
+// 0: too long for a wave
+int wave_elements(int cols, int dtype) {
+    const int sizes[] = {1, 2, 4, 8, 16, 24, 32}, most = dtype == ISG_F32 ? 4 : 8;
+    for (int ne : sizes)
+        if (cols + (ne < most ? ne : most) - 1 <= 64 * ne) return ne;
+    return 0;
 }
-Cut cut_forward(long long rows, int cols) {
-    if (cols <= kWaveCols) return cut_wave(cols);
+Cut cut_forward(long long rows, int cols, int dtype) {
+    if (const int ne = wave_elements(cols, dtype)) return Cut{1, ne, 1, cols};
     long long splits = (kUnits + rows - 1) / (rows > 0 ? rows : 1);
     const int most = cols / kWaveCols < kMaxSplits ? cols / kWaveCols : kMaxSplits, least = (cols + kMarkCols - 1) / kMarkCols;
     splits = splits > most ? most : splits;
@@ -1136,13 +1192,12 @@ Cut cut_forward(long long rows, int cols) {
     const int per = equal_part(cols, (int)splits);
     return Cut{4, 16, (cols + per - 1) / per, per};
 }
-Cut cut_backward(long long rows, int cols) {
-    if (cols <= kWaveCols) return cut_wave(cols);
+Cut cut_backward(long long rows, int cols, int dtype) {
+    if (const int ne = wave_elements(cols, dtype)) return Cut{1, ne, 1, cols};
+    const auto parts = [&](int ne) { return (cols + kThreads * ne - 9) / (kThreads * ne - 8); };
     for (int ne = 8;; ne *= 2) {
-        const int splits = (cols + kThreads * ne - 1) / (kThreads * ne);
-        const int half = (cols + kThreads * 2 * ne - 1) / (kThreads * 2 * ne);
-        if (ne < 32 && rows * half >= 1024) continue;  // (still four workgroups for each of the 256 CUs)
-        const int per = equal_part(cols, splits);
+        if (ne < 32 && rows * parts(2 * ne) >= 1024) continue;  // (still four workgroups for each of the 256 CUs)
+        const int per = equal_part(cols, parts(ne));
         return Cut{4, ne, (cols + per - 1) / per, per};
     }
 }
@@ -1276,7 +1331,7 @@ void scale_of(float temperature, float& c, float& c_lo, float& inv_t) {
 
 extern "C" long long isg_token_logprobs_workspace_bytes(int rows, int cols, int top) {
     if (rows < 0 || cols < 1 || cols > kMaxCols || top < 0 || top > kMaxTop) return -1;
-    const Cut cut = cut_forward(rows, cols);
+    const Cut cut = cut_forward(rows, cols, ISG_BF16);  // (the same for float: types differ in rows of one part)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * ((long long)sizeof(Sums) + 8 * top) + 8;
 }
 
@@ -1294,7 +1349,7 @@ extern "C" int isg_token_logprobs_fwd(const void* logits, long long row_stride, 
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && entropy && (!tokens || logprobs) && (top == 0 || (top_logprobs && top_classes)), ISG_EINVAL,
                 "%s: null pointer", who);
-    const Cut cut = cut_forward(rows, cols);
+    const Cut cut = cut_forward(rows, cols, dtype);
     ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     ISG_REQUIRE(((uintptr_t)workspace | (uintptr_t)stats) % 8 == 0 && (uintptr_t)stats % 16 == 0, ISG_EINVAL,
                 "%s: workspace and stats must be aligned to 8 and 16 bytes", who);
@@ -1339,7 +1394,7 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
     ISG_REQUIRE(logits && stats && dlogits && (!dlogprobs || tokens) && (!dtop_logprobs || (top > 0 && top_classes)),
                 ISG_EINVAL, "%s: null pointer", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
-    const Cut cut = cut_backward(rows, cols);
+    const Cut cut = cut_backward(rows, cols, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     LogprobsBwdArgs a{};
     a.tokens = tokens, a.top_classes = top_classes, a.stats = stats;
@@ -1355,7 +1410,7 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
 
 extern "C" long long isg_distill_workspace_bytes(int rows, int cols) {
     if (rows < 0 || cols < 1 || cols > kMaxCols) return -1;
-    const Cut cut = cut_forward(rows, cols);
+    const Cut cut = cut_forward(rows, cols, ISG_BF16);  // (the same for float: types differ in rows of one part)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * (long long)sizeof(DistillPart);
 }
 
@@ -1371,7 +1426,7 @@ extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const f
     if (rc != ISG_OK) return rc;
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && loss, ISG_EINVAL, "%s: null pointer", who);
-    const Cut cut = cut_forward(rows, cols);
+    const Cut cut = cut_forward(rows, cols, dtype);
     ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
     DistillArgs a{};
@@ -1411,7 +1466,7 @@ extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const f
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && stats && dloss && dlogits, ISG_EINVAL, "%s: null pointer", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
-    const Cut cut = cut_backward(rows, cols);
+    const Cut cut = cut_backward(rows, cols, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     DistillBwdArgs a{};
     a.values = values, a.classes = classes, a.stats = reinterpret_cast<const DistillStats*>(stats), a.dloss = dloss;

@@ -271,28 +271,63 @@ def test_a_student_mass_below_the_floats_keeps_its_logarithm():
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("cols,width", [(785, 792), (785, 786), (9000, 9001), (50, 64)])
+@pytest.mark.parametrize("cols,width", [(785, 792), (785, 786), (9000, 9001), (50, 64), (2047, 2050), (6, 8)])
 def test_rows_apart_are_read_in_place(cols, width, dtype):
-    decode = _decode()
-    wide = torch.full([40, width], float("nan"), dtype=DT[dtype], device=DEV)
-    dense = torch.randn([40, cols], device=DEV).to(DT[dtype])
-    wide[:, :cols] = dense
-    tok = torch.randint(0, cols, [40], device=DEV)
-    a = dense.clone().requires_grad_(True)
-    values, classes = torch.topk(dense.float(), 6, dim=1)
-    for view in (wide[:, :cols], wide[::2, :cols], wide[3:, :cols]):
-        sel = slice(0, None, 2) if view.shape[0] == 20 else slice(40 - view.shape[0], None)
-        v = view.detach().requires_grad_(True)
-        x, y = decode.token_logprobs(v, tok[sel], top=6), decode.token_logprobs(a[sel], tok[sel], top=6)
-        assert all(torch.equal(p, q) for p, q in zip(x, y))
-        gx, = torch.autograd.grad(x.logprobs.sum() + x.entropy.sum() + x.top_logprobs.sum(), v)
-        gy, = torch.autograd.grad(y.logprobs.sum() + y.entropy.sum() + y.top_logprobs.sum(), a)
-        assert gx.shape == v.shape and torch.equal(gx, gy[sel])
+    """Column slices, every other row and rows from any address on: the classes outside the slice are NaN and reach no
+    output, and no copy is made (a row's first address decides which classes a thread holds, so the order of a sum's
+    additions and its last bits may differ from a dense copy's; both are within the bounds)."""
+    wide, _ = _logits(40, width, dtype, "peaked", cols)
+    z = _f64(wide[:, 1:1 + cols])
+    tokens = np.random.RandomState(cols).randint(0, cols, [40])
+    wide[:, 0] = float("nan")
+    wide[:, 1 + cols:] = float("nan")
+    values, classes = _teacher(z, min(cols, 6), 1.0, True, 5)
+    for rows in (slice(0, None), slice(0, None, 2), slice(3, None), slice(1, None, 3)):
+        view = wide[rows, 1:1 + cols]
+        assert view.data_ptr() != view.contiguous().data_ptr()
+        _check_logprobs(view, z[rows], 1.0, tokens[rows], min(cols, 6), dtype)
         for tail in (False, True):
-            x = decode.distill_rows(v, values[sel], classes[sel], tail=tail)
-            y = decode.distill_rows(a[sel], values[sel], classes[sel], tail=tail)
-            assert torch.equal(x, y)
-            assert torch.equal(torch.autograd.grad(x.sum(), v)[0], torch.autograd.grad(y.sum(), a)[0][sel])
+            _check_distill(view, z[rows], values[rows], classes[rows], 1.0, tail, dtype)
+
+
+def test_rows_from_every_address():
+    """A dense row that starts any number of classes behind a 16-byte boundary."""
+    for dtype in ("f32", "bf16"):
+        for cols in (9, 70, 130, 510, 785, 2041, 2048, 4100, 8190):
+            flat, _ = _logits(1, cols + 8, dtype, "peaked", cols)
+            flat = flat[0]
+            for shift in range(8):
+                row = flat[shift:shift + cols][None]
+                z = _f64(row)
+                tokens = np.array([(shift * 97) % cols])
+                _check_logprobs(row, z, 1.0, tokens, min(cols, 9), dtype)
+                values, classes = _teacher(z, min(cols, 9), 1.0, True, shift)
+                classes[0, -1], classes[0, 0] = cols - 1, 0  # the row's two ends, wherever they lie
+                _check_distill(row, z, values, classes, 1.0, True, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1, 300000), (5000, 9000)])
+def test_the_best_classes_along_a_walk(rows, cols, dtype):
+    """Rows on which a workgroup's list of best classes overruns, is cut back or never finds a bound: rising, falling,
+    rising in steps, constant, two values, all but a few classes masked, zeros of both signs."""
+    rs = np.random.RandomState(cols)
+    ramp = np.linspace(-8, 8, cols)
+    kinds = [ramp, ramp[::-1], np.floor(ramp * 4) / 4, np.zeros(cols), (np.arange(cols) % 1000 == 0) * 1.0,
+             np.where(np.arange(cols) % (cols // 7) == 3, ramp, -np.inf), np.where(np.arange(cols) % 2, 0.0, -0.0),
+             np.abs(rs.randn(cols)) * -1e-40, np.full(cols, -np.inf)]
+    t = torch.tensor(np.stack(kinds), device=DEV).to(DT[dtype])
+    z = _f64(t)
+    if rows == 1:
+        for n in range(len(kinds)):
+            for top in (1, 20, 64):
+                _check_logprobs(t[n:n + 1], z[n:n + 1], 1.0, None, top, dtype, graded=False)
+    else:  # (rows in one part each)
+        decode = _decode()
+        out = decode.token_logprobs(t.repeat(rows // len(kinds) + 1, 1)[:rows], top=64)
+        want = ref.token_logprobs(z, 1.0, None, 64)
+        got = out.top_classes.cpu().numpy()
+        assert all(np.array_equal(got[r], want["top_classes"][r % len(kinds)]) for r in range(rows))
 
 
 def test_shapes_types_and_orders_of_the_arguments():
@@ -469,29 +504,35 @@ def test_captured_and_replayed(rows, cols):
 
 
 def test_rows_past_two_to_the_thirty_one_elements():
-    """Offsets that do not fit 32 bits: the last rows of 2.2e9 bf16 elements."""
+    """Offsets that do not fit 32 bits: the last rows of 2.2e9 bf16 elements, against the reference as any others (how a
+    row is cut depends on the number of rows, so its last bits may differ from the same rows' alone)."""
     decode = _decode()
     rows, cols = 2200, 1000003
     z = torch.zeros([rows, cols], dtype=torch.bfloat16, device=DEV)
     z[-2:] = torch.randn([2, cols], device=DEV).to(torch.bfloat16) * 3
-    tail = z[-2:].clone()
+    last = _f64(z[-2:])
+    tokens = np.array([cols - 1, 12345])
     tok = torch.full([rows], cols - 1, device=DEV)
+    tok[-1] = 12345
     z.requires_grad_(True)
     out = decode.token_logprobs(z, tok, top=3)
-    small = decode.token_logprobs(tail, tok[-2:], top=3)
-    for a, b in zip(out, small):
-        assert torch.equal(a[-2:], b)
-    assert (out.top_classes[0] == torch.arange(3, device=DEV)).all()
-    g, = torch.autograd.grad(out.logprobs.sum(), z)
-    tail.requires_grad_(True)
-    gs, = torch.autograd.grad(decode.token_logprobs(tail, tok[-2:]).logprobs.sum(), tail)
-    assert torch.equal(g[-2:], gs)
-    del g, gs, out
-    v, c = small.top_logprobs, small.top_classes
+    want = ref.token_logprobs(last, 1.0, tokens, 3)
+    for name in ("logprobs", "entropy", "top_logprobs"):
+        ref.close(_f64(getattr(out, name)[-2:]), want[name], want[name + "_tol"])
+    assert np.array_equal(out.top_classes[-2:].cpu().numpy(), want["top_classes"])
+    assert (out.top_classes[:-2] == torch.arange(3, device=DEV)).all()
+    g, = torch.autograd.grad(out.logprobs.sum() + out.entropy.sum(), z)
+    wd, wtol = ref.token_logprobs_grad(last, 1.0, tokens, None, np.ones(2), np.ones(2), None, "bf16")
+    ref.close(_f64(g[-2:]), wd, wtol)
+    values, classes = _f64(out.top_logprobs[-2:]), want["top_classes"]
+    del g, out
     live = torch.zeros([rows], dtype=torch.bool, device=DEV)
     live[-2:] = True
-    loss = decode.distill_rows(z, v[:1].expand(rows, 3), c[:1].expand(rows, 3), tail=True, live=live)
+    v, c = torch.zeros([rows, 3], device=DEV), torch.zeros([rows, 3], dtype=torch.int32, device=DEV)
+    v[-2:], c[-2:] = torch.tensor(values, device=DEV), torch.tensor(classes, device=DEV)
+    loss = decode.distill_rows(z, v, c, tail=True, live=live)
     g, = torch.autograd.grad(loss.sum(), z)
-    ls = decode.distill_rows(tail, v[:1].expand(2, 3), c[:1].expand(2, 3), tail=True)
-    gs, = torch.autograd.grad(ls.sum(), tail)
-    assert torch.equal(loss[-2:].detach(), ls.detach()) and torch.equal(g[-2:], gs) and not g[:-2].any()
+    want = ref.distill(last, _f64(v[-2:]), classes, 1.0, True, np.ones(2), "bf16")
+    ref.close(_f64(loss[-2:]), want["loss"], want["loss_tol"])
+    ref.close(_f64(g[-2:]), want["dlogits"], want["dlogits_tol"])
+    assert not loss[:-2].any() and not g[:-2].any()
