@@ -34,40 +34,32 @@ constexpr int kListKeep = 128;                // this many
 
 typedef unsigned long long u64;
 
-// ---- across the lanes of a wave: data-parallel moves inside the vector unit (six instructions, no LDS) -------------
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp(float old, float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
-}
+// ---- across the lanes of a wave --------------------------------------------------------------------------------------
+// Data-parallel moves as part of the operation itself: six instructions and no LDS.  A lane without a source keeps its
+// value, lane 63 ends up with the whole wave's.  (Written out: as compiler builtins every step becomes a move, a
+// quieting maximum and the operation.)  The s_nop are the two states such a read has to stay behind the write.
+#define ISG_WAVE_STEPS(op)                                                 \
+    "s_nop 1\n\t" op " %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\t"  \
+    "s_nop 1\n\t" op " %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\t"  \
+    "s_nop 1\n\t" op " %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\t"  \
+    "s_nop 1\n\t" op " %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n\t"  \
+    "s_nop 1\n\t" op " %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n\t" \
+    "s_nop 1\n\t" op " %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf\n\t" \
+    "s_nop 1"
 __device__ __forceinline__ float last_lane(float v) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, dpp<0x111, 0xf>(v, v));  // row_shr:1, 2, 4, 8
-    v = fmaxf(v, dpp<0x112, 0xf>(v, v));
-    v = fmaxf(v, dpp<0x114, 0xf>(v, v));
-    v = fmaxf(v, dpp<0x118, 0xf>(v, v));
-    v = fmaxf(v, dpp<0x142, 0xa>(v, v));  // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
-    v = fmaxf(v, dpp<0x143, 0xc>(v, v));
+    asm volatile(ISG_WAVE_STEPS("v_max_f32_dpp") : "+v"(v));
     return last_lane(v);
 }
 __device__ __forceinline__ float wave_sum(float v) {
-    v += dpp<0x111, 0xf>(0.0f, v);
-    v += dpp<0x112, 0xf>(0.0f, v);
-    v += dpp<0x114, 0xf>(0.0f, v);
-    v += dpp<0x118, 0xf>(0.0f, v);
-    v += dpp<0x142, 0xa>(0.0f, v);
-    v += dpp<0x143, 0xc>(0.0f, v);
+    asm volatile(ISG_WAVE_STEPS("v_add_f32_dpp") : "+v"(v));
     return last_lane(v);
 }
 // sum of the lanes up to and including this one
 __device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    asm volatile(ISG_WAVE_STEPS("v_add_u32_dpp") : "+v"(v));
     return v;
 }
 __device__ __forceinline__ u64 wave_max_key(u64 k) {
@@ -131,9 +123,10 @@ __device__ __forceinline__ void store_vector(__hip_bfloat16* p, const float* v) 
 
 // Where the elements of a thread lie in its unit's part [lo, hi) of a row: NE of them in vectors of VE (16 bytes), the
 // vectors of a slot side by side over the unit's W * 64 threads, on 16-byte boundaries of memory from `first` <= lo on.
-// (Two-byte boundaries cost a 16-byte load three to four cache accesses instead of one.)  The part's first and last
-// vector may reach outside; they are read from lo and up to hi instead, and `start` tells which of their elements are
-// this thread's own.
+// (Rows of 131,071 bf16 logits start on any even address, where a 16-byte load takes three cache accesses instead of one:
+// the walk over 2,048 of them took 156 us instead of 141.  Boundaries of 128 bytes gained nothing more.)  The part's
+// outer vectors may reach outside; they are read from lo and up to hi instead, and `start` tells which of their elements
+// are this thread's own.
 template <typename T, int W, int NE>
 struct Span {
     static constexpr int VE = NE < 16 / (int)sizeof(T) ? NE : 16 / (int)sizeof(T);
@@ -206,7 +199,7 @@ struct Span {
     // a slot's gradients (what the outer vectors repeat of their neighbours they repeat with the same values)
     __device__ __forceinline__ void store(T* d, int t, const float* o) const {
         const int s = start(t);
-        if (s < hi) store_vector<VE>(d + inside(s), o);
+        if (s < hi && s + VE > lo) store_vector<VE>(d + inside(s), o);
     }
 };
 
@@ -229,6 +222,33 @@ __device__ __forceinline__ float order_value(unsigned k) {
 __device__ __forceinline__ float above(float x) { return order_value(order_bits(x) + 1u); }
 __device__ __forceinline__ u64 order_key(float v, int c) { return ((u64)order_bits(v) << 32) | (unsigned)~c; }
 
+// one bit an element (bit e: element e) where v[e] >= low: a comparison and an addition with carry each
+template <int NE>
+__device__ __forceinline__ unsigned reach_mask(const float (&v)[NE], float low) {
+    unsigned hit = 0;
+    if constexpr (NE % 8 == 0) {
+#pragma unroll
+        for (int e = NE - 4; e >= 0; e -= 4) {
+            u64 a, b, c, d;  // (four comparisons ahead: a mask is read two states behind its write at the earliest)
+            asm("v_cmp_ge_f32_e64 %1, %5, %9\n\t"
+                "v_cmp_ge_f32_e64 %2, %6, %9\n\t"
+                "v_cmp_ge_f32_e64 %3, %7, %9\n\t"
+                "v_cmp_ge_f32_e64 %4, %8, %9\n\t"
+                "s_nop 0\n\t"
+                "v_addc_co_u32_e64 %0, %1, %0, %0, %1\n\t"
+                "v_addc_co_u32_e64 %0, %2, %0, %0, %2\n\t"
+                "v_addc_co_u32_e64 %0, %3, %0, %0, %3\n\t"
+                "v_addc_co_u32_e64 %0, %4, %0, %0, %4"
+                : "+v"(hit), "=&s"(a), "=&s"(b), "=&s"(c), "=&s"(d)
+                : "v"(v[e + 3]), "v"(v[e + 2]), "v"(v[e + 1]), "v"(v[e]), "v"(low));
+        }
+    } else {
+#pragma unroll
+        for (int e = NE - 1; e >= 0; --e) hit = hit + hit + (v[e] >= low ? 1u : 0u);
+    }
+    return hit;
+}
+
 // log p of a logit; a row without any probability (log2 s = +inf) gives -inf.  In nats throughout: at T = 1 the
 // type's lowest value has a finite logarithm, its binary one would overflow.
 __device__ __forceinline__ float log_prob(float z, float m, float inv_t, float l2s) {
@@ -245,9 +265,17 @@ template <int W>
 struct TopShared {
     u64 cand[4 * kCandidates];   // W = 1: a quarter for each wave
     unsigned group[W == 1 ? 1 : kThreads];
-    unsigned count;
+    int count;
     u64 best[4];
 };
+
+// where a wave's elements go in a list the workgroup shares: its first place, for the lanes' running total `upto`
+__device__ __forceinline__ int wave_places(int* count, int upto) {
+    const int all = __builtin_amdgcn_readlane(upto, 63);
+    int first = 0;
+    if (all && (threadIdx.x & 63) == 0) first = atomicAdd(count, all);
+    return __builtin_amdgcn_readfirstlane(first);
+}
 
 __device__ __forceinline__ unsigned group_bound(float lane_max, int k, TopShared<4>& sh) {
     const int lane = threadIdx.x & 63;
@@ -309,19 +337,15 @@ __device__ __forceinline__ void select_top(const float (&v)[NE], int k, TopShare
     int total = kCap + 1;
     if (bound > 0x7fu) {  // (0x7f begins the key of -inf)
         const float low = order_value(bound << 16);
-        unsigned hit = 0;
-#pragma unroll
-        for (int e = NE - 1; e >= 0; --e) hit = hit + hit + (v[e] >= low ? 1u : 0u);
-        const int mine = __builtin_popcount(hit);
-        int at;
+        unsigned hit = reach_mask(v, low);
+        const int mine = __builtin_popcount(hit), upto = wave_scan(mine);
+        int at = upto - mine;
         if constexpr (W == 1) {
-            const int upto = wave_scan(mine);
             total = __builtin_amdgcn_readlane(upto, 63);
-            at = upto - mine;
         } else {
-            at = mine ? (int)atomicAdd(&sh.count, (unsigned)mine) : 0;
+            at += wave_places(&sh.count, upto);
             together<W>();
-            total = (int)sh.count;
+            total = sh.count;
         }
         if (total <= kCap) {
             while (hit) {
@@ -588,12 +612,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 6) void logprobs_str
         span.unpack(raw, v);
         ahead.next();
         if (ahead.more()) ahead.fetch(z, raw);
-        float m = v[0];
+        float lane_max = v[0];
 #pragma unroll
-        for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
-        const float lane_max = m;
-        m = wave_max(m);
-        if (m > t.m) {  // (uniform in the wave)
+        for (int e = 1; e < NE; ++e) lane_max = fmaxf(lane_max, v[e]);
+        if (__ballot(lane_max > t.m)) {
+            const float m = wave_max(lane_max);
             if (t.m != -INFINITY) {
                 const float d = (t.m - m) * a.c, f = __builtin_amdgcn_exp2f(d);
                 t.u = f * (t.u + fmaxf(d, -1000.0f) * t.s);
@@ -620,20 +643,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 6) void logprobs_str
             if (tid == 0) list.count = count;
             __syncthreads();
             if (fits) {
-                unsigned hit = 0;
                 if (__ballot(lane_max >= reach)) {
-#pragma unroll
-                    for (int e = NE - 1; e >= 0; --e) hit = hit + hit + (v[e] >= reach ? 1u : 0u);
+                    unsigned hit = reach_mask(v, reach);
+                    const int mine = __builtin_popcount(hit), upto = wave_scan(mine);
+                    int at = wave_places(&list.count, upto) + upto - mine;
+                    if (at + mine <= kListMax)
+                        while (hit) {  // (a lane's only one is its largest)
+                            const int e = __builtin_ctz(hit);
+                            hit &= hit - 1;
+                            const int i = span.inside(span.start(e / S::VE)) + e % S::VE;
+                            list.keys[at++] = order_key(mine == 1 ? lane_max : ld(z, i), i);
+                        }
                 }
-                const int mine = __builtin_popcount(hit);
-                int at = 0;
-                if (mine) at = atomicAdd(&list.count, mine);
-                if (at + mine <= kListMax)
-                    while (hit) {
-                        const int e = __builtin_ctz(hit);
-                        hit &= hit - 1;
-                        list.keys[at++] = reload(e);
-                    }
                 __syncthreads();
                 const int total = list.count;
                 fits = total <= kListMax;
@@ -856,7 +877,8 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
     const float s_exp = (float)__builtin_amdgcn_frexp_expf(s), s_log = kLn2 * __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s));
     // the teacher's distribution over its entries
     const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? (float)(1.4426950408889634074 - (double)kLog2e) : a.c_lo;
-    float mv = 0.0f, lv = 0.0f, bad = 0.0f, sv = 0.0f;
+    float mv = 0.0f, lv = 0.0f, sv = 0.0f;
+    bool bad = false;
     if (!a.tail) {
         mv = -INFINITY;
         for (int j = lane; j < a.k; j += 64)
@@ -867,7 +889,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
     for (int j = lane; j < a.k; j += 64) {
         const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
         if (i >= 0) sv += power(v[j], mv, cv, cv_lo);
-        if (i >= a.cols) bad = 1.0f;
+        bad |= i >= a.cols;
     }
     sv = wave_sum(sv);
     if (!a.tail) lv = sv == 0.0f ? INFINITY : __builtin_amdgcn_logf(sv);
@@ -883,7 +905,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
         if (q != 0.0f) l += s == 0.0f ? INFINITY : q * (__builtin_fmaf(s_exp, kLn2, d) + s_log);
     }
     l = wave_sum(l);
-    bad = wave_max(bad);
+    bad = __ballot(bad) != 0;
     if (lane == 0) {
         float coef = qsum, mb = m, lb = l2s;
         if (a.tail) {
@@ -897,7 +919,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
             coef = none ? 0.0f : (qsum + qr) * pr - qr;
             mb = mr, lb = lr;
         }
-        if (bad != 0.0f) l = NAN, coef = NAN;
+        if (bad) l = NAN, coef = NAN;
         a.loss[row] = l;
         if (a.stats) a.stats[row] = DistillStats{mb, lb, coef, qsum + qr, m, l2s, mv, lv};
     }
@@ -985,7 +1007,7 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
 template <typename T, int NE, bool TAIL>
 __global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __restrict__ logits, DistillArgs a) {
     __shared__ DistillPart red[4];
-    __shared__ unsigned char marks[TAIL ? kMarkCols / 8 + 4 : 4] __attribute__((aligned(16)));
+    __shared__ unsigned char marks[TAIL ? kMarkCols / 8 + 16 : 16] __attribute__((aligned(16)));
     __shared__ unsigned repeated;
     const int tid = threadIdx.x, lane = tid & 63;
     const long long unit = block_index();
@@ -1035,11 +1057,11 @@ __global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __res
                 }
             }
         }
-        float m = v[0];
+        float lane_max = v[0];
 #pragma unroll
-        for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
-        m = wave_max(m);
-        if (m > t.m) {
+        for (int e = 1; e < NE; ++e) lane_max = fmaxf(lane_max, v[e]);
+        if (__ballot(lane_max > t.m)) {
+            const float m = wave_max(lane_max);
             if (t.m != -INFINITY) s *= power(t.m, m, a.c, a.c_lo);
             t.m = m;
         }
@@ -1168,8 +1190,8 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
 // ---- launches ------------------------------------------------------------------------------------------------------
 // How a row is cut: one wave for what its registers hold.  Beyond, the forward passes walk over parts of a row, as many
 // as give kUnits workgroups but of at least kWaveCols classes; the backward passes have nothing to join and take
-// workgroups of at most 32 classes a thread.  Parts are equal but for the rounding to 8 classes.  (`ve - 1` classes of
-// room for a part that starts between two 16-byte boundaries.)
+// workgroups of at most 32 classes a thread.  Parts are equal but for the rounding to 8 classes; there is room for those
+// that start between two boundaries (Span).
 constexpr long long kUnits = 4096;
 constexpr int kMaxSplits = 128;
 struct Cut {
@@ -1194,7 +1216,7 @@ Cut cut_forward(long long rows, int cols, int dtype) {
 }
 Cut cut_backward(long long rows, int cols, int dtype) {
     if (const int ne = wave_elements(cols, dtype)) return Cut{1, ne, 1, cols};
-    const auto parts = [&](int ne) { return (cols + kThreads * ne - 9) / (kThreads * ne - 8); };
+    const auto parts = [&](int ne) { return (cols + kThreads * ne - 8 - 1) / (kThreads * ne - 8); };
     for (int ne = 8;; ne *= 2) {
         if (ne < 32 && rows * parts(2 * ne) >= 1024) continue;  // (still four workgroups for each of the 256 CUs)
         const int per = equal_part(cols, parts(ne));
