@@ -21,6 +21,7 @@
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eLo = (float)(1.44269504088896340736 - (double)kLog2e);  // (positive)
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kThreads = 256;
 constexpr int kMaxTop = ISG_TOP_MAX;          // classes kept per row
@@ -255,6 +256,13 @@ __device__ __forceinline__ float log_prob(float z, float m, float inv_t, float l
     return (z - m) * inv_t - kLn2 * l2s;
 }
 
+// 2^((z - m) (c + c_lo)) with the exponent's whole part taken off before anything is rounded: an exponent of -8 as one
+// float is off by 5e-7 of the power already.  For float gradients and for differences of probabilities.
+__device__ __forceinline__ float power_exact(float z, float m, float c, float c_lo) {
+    const float d = z - m, n = rintf(fmaxf(d * c, -300.0f));
+    return ldexpf(__builtin_amdgcn_exp2f(__builtin_fmaf(d, c_lo, __builtin_fmaf(d, c, -n))), (int)n);
+}
+
 // ---- the `top` first keys of a unit ----------------------------------------------------------------------------------
 // The k-th largest of the threads' group maxima is a lower bound of the k-th largest element (k groups hold one at
 // least as large), so the elements not below it are few more than k: k + k^2 / (2 groups) for values in any order.
@@ -431,7 +439,7 @@ __device__ __forceinline__ void merge_sums(Sums& t, const Sums& p, float c) {
 // What a row's results follow from.  `c_rel`: by how much log2(e) / T exceeds the float c, relative; the logarithm of
 // the sum moves with the exponents' scale as their mean does, u / s.
 struct RowStats {
-    float m, l2s, H;
+    float m, l2s, H, inv_s;
 };
 __device__ __forceinline__ RowStats row_stats(const Sums& t, float c_rel) {
     RowStats r;
@@ -439,6 +447,7 @@ __device__ __forceinline__ RowStats row_stats(const Sums& t, float c_rel) {
     const float mean = t.u / t.s;
     r.l2s = t.s == 0.0f ? INFINITY : __builtin_amdgcn_logf(t.s) + c_rel * mean;
     r.H = t.s == 0.0f ? 0.0f : kLn2 * (r.l2s - mean);
+    r.inv_s = 1.0f / t.s;
     return r;
 }
 
@@ -475,7 +484,7 @@ __device__ __forceinline__ void row_outputs(const LogprobsArgs& a, const T* z, l
         a.logprobs[row] = t >= 0 && t < a.cols ? log_prob(ld(z, t), r.m, a.inv_t, r.l2s) : NAN;
     }
     a.entropy[row] = r.H;
-    if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(r.m, r.l2s, r.H, 0.0f);
+    if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(r.m, r.l2s, r.H, r.inv_s);
 }
 
 __device__ __forceinline__ void row_alternative(const LogprobsArgs& a, long long row, const RowStats& r, int place, u64 key) {
@@ -748,22 +757,24 @@ struct LogprobsBwdArgs {
     const float* dtop;
     long long row_stride, units;
     int token_bytes, cols, splits, per, top;
-    float c, inv_t;
+    float c, c_lo, inv_t;
 };
 
 template <typename T, int W, int NE>
 __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restrict__ logits, LogprobsBwdArgs a,
                                                                T* __restrict__ dlogits) {
     const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
-    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
-    if (unit >= a.units) return;
+    // (from the last unit back: what the forward pass read last is still in the last-level cache)
+    const long long unit = a.units - 1 - (W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index());
+    if (unit < 0) return;
     const long long row = a.splits == 1 ? unit : unit / a.splits;
     const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
     using S = Span<T, W, NE>;
     const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
     T* d = dlogits + row * a.cols;
     const S span(d, lo, hi, tid);  // (aligned as the gradient; dense logits lie the same way)
-    const float m = a.stats[4 * row], l2s = a.stats[4 * row + 1], H = a.stats[4 * row + 2];
+    const float4 stats = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+    const float m = stats.x, l2s = stats.y;
     const bool zero = l2s == INFINITY;  // a dead row, or no class has probability: nothing to move
     const T* z = logits + row * a.row_stride;
     float v[NE];
@@ -776,16 +787,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restr
     if (a.dtop && lane < a.top) gt = a.dtop[row * a.top + lane], ti = a.top_classes[row * a.top + lane];
     float g = a.dtop ? wave_sum(gt) + ga : ga;
     if (a.dlogprobs && ga != 0.0f && (tok < 0 || tok >= a.cols)) g = NAN;  // a class the row does not have
+    // p (g + g_H (log p + H)) / T with p = 2^x / s and log p = ln 2 (x - log2 s): the row's constants put together
+    const float k0 = -a.inv_t * stats.w * (g + gh * (stats.z - kLn2 * l2s)), k1 = -a.inv_t * stats.w * (gh * kLn2);
     const auto dense = [&](float zi) {
-        const float x = (zi - m) * a.c - l2s;
-        return -__builtin_amdgcn_exp2f(x) * (g + gh * (kLn2 * fmaxf(x, -1000.0f) + H));
+        const float x = (zi - m) * a.c;
+        const float e = sizeof(T) == 4 ? power_exact(zi, m, a.c, a.c_lo) : __builtin_amdgcn_exp2f(x);
+        return e * __builtin_fmaf(k1, fmaxf(x, -1000.0f), k0);
     };
 #pragma unroll
     for (int t = 0; t < S::NV; ++t) {
         if (span.empty(t)) break;
         float o[S::VE];
 #pragma unroll
-        for (int j = 0; j < S::VE; ++j) o[j] = zero ? 0.0f : a.inv_t * dense(v[t * S::VE + j]);
+        for (int j = 0; j < S::VE; ++j) o[j] = zero ? 0.0f : dense(v[t * S::VE + j]);
         span.store(d, t, o);
     }
     if (zero) return;
@@ -793,20 +807,21 @@ __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restr
     if (tid >= 64) return;
     const bool both = __ballot(ti >= 0 && ti == tok) != 0;
     if (ti >= lo && ti < hi) {
-        const float o = a.inv_t * (dense(ld(z, ti)) + gt + (ti == tok ? ga : 0.0f));
+        const float o = __builtin_fmaf(a.inv_t, gt + (ti == tok ? ga : 0.0f), dense(ld(z, ti)));
         store_vector<1>(d + ti, &o);
     }
     if (lane == 0 && !both && tok >= lo && tok < hi) {
-        const float o = a.inv_t * (dense(ld(z, tok)) + ga);
+        const float o = __builtin_fmaf(a.inv_t, ga, dense(ld(z, tok)));
         store_vector<1>(d + tok, &o);
     }
 }
 
 // ---- distill_rows --------------------------------------------------------------------------------------------------
-// What the backward pass keeps of a row: the dense part of its gradient is coef * 2^((z - mb) c - lb); at the
-// teacher's classes it is total * 2^((z - m) c - l2s) - q.  q of entry j is 2^((v_j - mv) cv - lv).
+// What the backward pass keeps of a row: the dense part of its gradient is coef * ib * 2^((z - mb) c); at the teacher's
+// classes it is total * is * 2^((z - m) c) - q, and q of entry j is iv * 2^((v_j - mv) cv).  is = 0: a row without
+// gradient.
 struct DistillStats {
-    float mb, lb, coef, total, m, l2s, mv, lv;
+    float mb, ib, coef, total, m, is, mv, iv;
 };
 
 // maximum and sum of powers of a row's classes outside the teacher's entries, and of the entries' own classes
@@ -853,7 +868,7 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, fl
 
 __device__ __forceinline__ void distill_dead(const DistillArgs& a, long long row) {
     a.loss[row] = 0.0f;
-    if (a.stats) a.stats[row] = DistillStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, INFINITY, 0.0f, 0.0f};
+    if (a.stats) a.stats[row] = DistillStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 }
 
 // whether an earlier entry names the class as well
@@ -861,6 +876,12 @@ __device__ bool named_before(const DistillArgs& a, long long row, int j, long lo
     for (int o = 0; o < j; ++o)
         if (class_at(a.classes, a.class_bytes, row * a.k + o) == cls) return true;
     return false;
+}
+
+// log(1 + x): the logarithm of the rounded sum, corrected for what the rounding took
+__device__ __forceinline__ float log1p_of(float x) {
+    const float u = 1.0f + x;
+    return u == 1.0f ? x : kLn2 * __builtin_amdgcn_logf(u) * (x / (u - 1.0f));
 }
 
 // The loss of a row from its sums, by one wave.
@@ -876,7 +897,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
     // same size it loses a rounding of that difference, not one of its own that every entry of the row would share)
     const float s_exp = (float)__builtin_amdgcn_frexp_expf(s), s_log = kLn2 * __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s));
     // the teacher's distribution over its entries
-    const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? (float)(1.4426950408889634074 - (double)kLog2e) : a.c_lo;
+    const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
     float mv = 0.0f, lv = 0.0f, sv = 0.0f;
     bool bad = false;
     if (!a.tail) {
@@ -907,21 +928,32 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
     l = wave_sum(l);
     bad = __ballot(bad) != 0;
     if (lane == 0) {
-        float coef = qsum, mb = m, lb = l2s;
+        float coef = qsum, mb = m, ib = 1.0f / s;
         if (a.tail) {
             const bool none = t.s == 0.0f;
             const float mr = t.m == -INFINITY ? 0.0f : t.m, lr = none ? INFINITY : __builtin_amdgcn_logf(t.s);
             if (none && qr <= kNoMass) qr = 0.0f;
-            // the student's mass outside; its logarithm from the logarithms where it is no normal float
-            const float pr = t.s * power(mr, m, a.c, a.c_lo) / s;
-            const float lpr = pr > 1e-30f ? __builtin_amdgcn_logf(pr) : (mr - m) * a.c + (lr - l2s);
-            if (qr > 0.0f) l += none ? INFINITY : qr * kLn2 * (__builtin_amdgcn_logf(qr) - lpr);
+            // The student's mass outside, and the logarithm of the masses' ratio: from the logarithms where it is no
+            // normal float; where the entries have less than half of it from their masses, as 1 - (a few) per cent on
+            // both sides would cancel.
+            const float pr = t.s * power(mr, m, a.c, a.c_lo) / s, pe = t.se * power(t.me, m, a.c, a.c_lo) / s;
+            float ratio;
             coef = none ? 0.0f : (qsum + qr) * pr - qr;
-            mb = mr, lb = lr;
+            if (pe < 0.5f && sv < 1.0f) {
+                coef = sv - pe;
+                ratio = log1p_of((pe - sv) / pr);
+            } else {
+                const float lpr = pr > 1e-30f ? __builtin_amdgcn_logf(pr) : (mr - m) * a.c + (lr - l2s);
+                ratio = kLn2 * (__builtin_amdgcn_logf(qr) - lpr);
+            }
+            if (qr > 0.0f) l += none ? INFINITY : qr * ratio;
+            mb = mr, ib = none ? 0.0f : 1.0f / t.s;
         }
         if (bad) l = NAN, coef = NAN;
         a.loss[row] = l;
-        if (a.stats) a.stats[row] = DistillStats{mb, lb, coef, qsum + qr, m, l2s, mv, lv};
+        if (a.stats)
+            a.stats[row] = DistillStats{mb, ib, coef, qsum + qr, m, s == 0.0f ? 0.0f : 1.0f / s, mv,
+                                        a.tail ? 1.0f : (sv == 0.0f ? 0.0f : 1.0f / sv)};
     }
 }
 
@@ -1115,7 +1147,7 @@ struct DistillBwdArgs {
     const float* dloss;
     long long row_stride, units;
     int class_bytes, cols, splits, per, k, tail;
-    float c, inv_t;
+    float c, c_lo, inv_t;
 };
 
 template <typename T, int W, int NE>
@@ -1124,8 +1156,8 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     __shared__ unsigned marks[kThreads];
     __shared__ unsigned repeated;
     const int lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
-    const long long unit = W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index();
-    if (unit >= a.units) return;
+    const long long unit = a.units - 1 - (W == 1 ? block_index() * 4 + (threadIdx.x >> 6) : block_index());
+    if (unit < 0) return;
     const long long row = a.splits == 1 ? unit : unit / a.splits;
     const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
     using S = Span<T, W, NE>;
@@ -1133,20 +1165,22 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     T* d = dlogits + row * a.cols;
     const S span(d, lo, hi, tid);  // (aligned as the gradient; dense logits lie the same way)
     const DistillStats st = a.stats[row];
-    const bool zero = st.l2s == INFINITY;  // a dead row, or no class has probability
+    const bool zero = st.is == 0.0f;  // a dead row, or no class has probability
     const T* z = logits + row * a.row_stride;
     float v[NE];
     if (!zero) span.template load<false>(z, v);
     const float g = a.dloss[row] * a.inv_t;
-    // (no class outside the entries has probability: lb = +inf, and the powers come out as 0 from a finite mb)
-    const float gc = g * st.coef;
+    const float gc = g * st.coef * st.ib;
 #pragma unroll
     for (int t = 0; t < S::NV; ++t) {
         if (span.empty(t)) break;
         float o[S::VE];
 #pragma unroll
-        for (int j = 0; j < S::VE; ++j)
-            o[j] = zero ? 0.0f : gc * __builtin_amdgcn_exp2f((v[t * S::VE + j] - st.mb) * a.c - st.lb);
+        for (int j = 0; j < S::VE; ++j) {
+            const float zi = v[t * S::VE + j];
+            const float e = sizeof(T) == 4 ? power_exact(zi, st.mb, a.c, a.c_lo) : __builtin_amdgcn_exp2f((zi - st.mb) * a.c);
+            o[j] = zero ? 0.0f : gc * e;
+        }
         span.store(d, t, o);
     }
     if (zero || st.coef != st.coef) return;  // (NaN: an entry the row does not have; the whole row is)
@@ -1170,18 +1204,18 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
         together<W>();
         twice = repeated != 0;
     }
-    const float cv = a.tail ? kLog2e : a.c;
+    const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
     for (int j = tid; j < a.k; j += W * 64) {
         const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
         if (i < lo || i >= hi) continue;
-        float q = __builtin_amdgcn_exp2f((a.values[row * a.k + j] - st.mv) * cv - st.lv);
+        float q = st.iv * power_exact(a.values[row * a.k + j], st.mv, cv, cv_lo);
         if (twice) {  // (every place of the class writes the same sum)
             q = 0.0f;
             for (int o = 0; o < a.k; ++o)
                 if (class_at(a.classes, a.class_bytes, row * a.k + o) == i)
-                    q += __builtin_amdgcn_exp2f((a.values[row * a.k + o] - st.mv) * cv - st.lv);
+                    q += st.iv * power_exact(a.values[row * a.k + o], st.mv, cv, cv_lo);
         }
-        const float p = __builtin_amdgcn_exp2f((ld(z, i) - st.m) * a.c - st.l2s);
+        const float p = st.is * power_exact(ld(z, i), st.m, a.c, a.c_lo);
         const float o = g * (st.total * p - q);
         store_vector<1>(d + i, &o);
     }
@@ -1423,8 +1457,7 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
     a.dlogprobs = dlogprobs, a.dentropy = dentropy, a.dtop = dtop_logprobs;
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
     a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.top = top;
-    float c_lo;
-    scale_of(temperature, a.c, c_lo, a.inv_t);
+    scale_of(temperature, a.c, a.c_lo, a.inv_t);
     if (dtype == ISG_F32) launch_backward<LogprobsBwd<float>>(cut, logits, a, dlogits, s);
     else launch_backward<LogprobsBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
     return isg::check_launch("logprobs_bwd_kernel");
@@ -1494,8 +1527,7 @@ extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const f
     a.values = values, a.classes = classes, a.stats = reinterpret_cast<const DistillStats*>(stats), a.dloss = dloss;
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
     a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.k = k, a.tail = tail;
-    float c_lo;
-    scale_of(temperature, a.c, c_lo, a.inv_t);
+    scale_of(temperature, a.c, a.c_lo, a.inv_t);
     if (dtype == ISG_F32) launch_backward<DistillBwd<float>>(cut, logits, a, dlogits, s);
     else launch_backward<DistillBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
     return isg::check_launch("distill_bwd_kernel");
