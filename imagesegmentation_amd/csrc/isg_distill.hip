@@ -1,0 +1,514 @@
+// The divergence of a row from a teacher's most probable classes, forward and backward (layout: isg_classes.h).
+#include "isg_classes.h"
+
+namespace {
+
+constexpr int kMaxEntries = ISG_DISTILL_MAX;  // a teacher's classes per row
+
+// What the backward pass keeps of a row: the dense part of its gradient is coef * ib * 2^((z - mb) c); at the teacher's
+// classes it is total * is * 2^((z - m) c) - q, and q of entry j is iv * 2^((v_j - mv) cv).  is = 0: a row without
+// gradient.
+struct DistillStats {
+    float mb, ib, coef, total, m, is, mv, iv;
+};
+
+// maximum and sum of powers of a row's classes outside the teacher's entries, and of the entries' own classes
+struct DistillPart {
+    float m, s, me, se;
+};
+
+struct DistillArgs {
+    const float* values;
+    const void* classes;
+    const unsigned char* live;
+    float* loss;
+    DistillStats* stats;
+    DistillPart* part;  // [rows][splits]
+    long long row_stride, units;
+    int class_bytes, cols, splits, per, k, tail;
+    float c, c_lo, c_near, inv_t;
+};
+
+// 2^((z - m) (c + c_lo)): log2(e) / T to twice a float's digits, as a rounded c shifts every exponent the same way
+__device__ __forceinline__ float power(float z, float m, float c, float c_lo) {
+    const float d = z - m;
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c_lo, d * c));
+}
+
+// ... of the many classes of a row: of bf16 logits by the nearest float alone (x is off by 2^-25 of itself at most)
+template <typename T>
+__device__ __forceinline__ float power_of(const DistillArgs& a, float z, float m) {
+    return sizeof(T) == 4 ? power(z, m, a.c, a.c_lo) : __builtin_amdgcn_exp2f((z - m) * a.c_near);
+}
+
+// A remaining mass that rounding alone can leave of the entries' log-probabilities (k of them, each good to 2^-24 of
+// its size): where the student has no class outside the entries it is no mass, anything above it has nowhere to go.
+constexpr float kNoMass = 1e-5f;
+
+// (m, s) of two disjoint parts
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float c, float c_lo) {
+    const float n = fmaxf(m, m2);
+    const float a = s == 0.0f ? 0.0f : s * power(m, n, c, c_lo), b = s2 == 0.0f ? 0.0f : s2 * power(m2, n, c, c_lo);
+    m = n, s = a + b;
+}
+
+__device__ __forceinline__ void distill_dead(const DistillArgs& a, long long row) {
+    a.loss[row] = 0.0f;
+    if (a.stats) a.stats[row] = DistillStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// whether an earlier entry names the class as well
+__device__ bool named_before(const DistillArgs& a, long long row, int j, long long cls) {
+    for (int o = 0; o < j; ++o)
+        if (class_at(a.classes, a.class_bytes, row * a.k + o) == cls) return true;
+    return false;
+}
+
+// log(1 + x): the logarithm of the rounded sum, corrected for what the rounding took
+__device__ __forceinline__ float log1p_of(float x) {
+    const float u = 1.0f + x;
+    return u == 1.0f ? x : kLn2 * __builtin_amdgcn_logf(u) * (x / (u - 1.0f));
+}
+
+// The loss of a row from its sums, by G lanes of a wave.
+template <int G, typename T>
+__device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z, long long row, const DistillPart& t) {
+    const int lane = threadIdx.x & (G - 1);
+    const float* v = a.values + row * a.k;
+    float m = t.m, s = t.s;
+    if (a.tail) merge(m, s, t.me, t.se, a.c, a.c_lo);
+    m = m == -INFINITY ? 0.0f : m;
+    const float l2s = s == 0.0f ? INFINITY : __builtin_amdgcn_logf(s);
+    // (log s as a whole number of ln 2 and the logarithm of a fraction: added one after the other to a difference of the
+    // same size it loses a rounding of that difference, not one of its own that every entry of the row would share)
+    const float s_exp = (float)__builtin_amdgcn_frexp_expf(s), s_log = kLn2 * __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s));
+    // the teacher's distribution over its entries
+    const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
+    float mv = 0.0f, lv = 0.0f, sv = 0.0f;
+    bool bad = false;
+    if (!a.tail) {
+        mv = -INFINITY;
+        for (int j = lane; j < a.k; j += G)
+            if (class_at(a.classes, a.class_bytes, row * a.k + j) >= 0) mv = fmaxf(mv, v[j]);
+        mv = group_max<G>(mv);
+        if (mv == -INFINITY) mv = 0.0f;
+    }
+    for (int j = lane; j < a.k; j += G) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i >= 0) sv += power(v[j], mv, cv, cv_lo);
+        bad |= i >= a.cols;
+    }
+    sv = group_sum<G>(sv);
+    if (!a.tail) lv = sv == 0.0f ? INFINITY : __builtin_amdgcn_logf(sv);
+    const float qsum = a.tail ? sv : (sv == 0.0f ? 0.0f : 1.0f);
+    float qr = a.tail ? fmaxf(1.0f - sv, 0.0f) : 0.0f;
+    float l = 0.0f;
+    for (int j = lane; j < a.k; j += G) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < 0 || i >= a.cols) continue;
+        const float q = power(v[j], mv, cv, cv_lo) * __builtin_amdgcn_exp2f(-lv);
+        const float lq = (v[j] - mv) * (a.tail ? 1.0f : a.inv_t) - kLn2 * lv;
+        const float d = lq - (ld(z, i) - m) * a.inv_t;  // log q - log p - log s
+        if (q != 0.0f) l += s == 0.0f ? INFINITY : q * (__builtin_fmaf(s_exp, kLn2, d) + s_log);
+    }
+    l = group_sum<G>(l);
+    bad = group_any<G>(bad);
+    if (lane == 0) {
+        float coef = qsum, mb = m, ib = 1.0f / s;
+        if (a.tail) {
+            const bool none = t.s == 0.0f;
+            const float mr = t.m == -INFINITY ? 0.0f : t.m, lr = none ? INFINITY : __builtin_amdgcn_logf(t.s);
+            if (none && qr <= kNoMass) qr = 0.0f;
+            // The student's mass outside, and the logarithm of the masses' ratio: from the logarithms where it is no
+            // normal float; where the entries have less than half of it on both sides from their masses, as 1 - (a
+            // few per cent) over the same would lose them.
+            const float pr = t.s * power(mr, m, a.c, a.c_lo) / s, pe = t.se * power(t.me, m, a.c, a.c_lo) / s;
+            float ratio;
+            coef = none ? 0.0f : (qsum + qr) * pr - qr;
+            if (pe < 0.5f && sv < 1.0f) coef = sv - pe;
+            if (pe < 0.5f && sv < 0.5f) {
+                ratio = log1p_of((pe - sv) / pr);
+            } else {
+                const float lpr = pr > 1e-30f ? __builtin_amdgcn_logf(pr) : (mr - m) * a.c + (lr - l2s);
+                ratio = kLn2 * (__builtin_amdgcn_logf(qr) - lpr);
+            }
+            if (qr > 0.0f) l += none ? INFINITY : qr * ratio;
+            mb = mr, ib = none ? 0.0f : 1.0f / t.s;
+        }
+        if (bad) l = NAN, coef = NAN;
+        a.loss[row] = l;
+        if (a.stats)
+            a.stats[row] = DistillStats{mb, ib, coef, qsum + qr, m, s == 0.0f ? 0.0f : 1.0f / s, mv,
+                                        a.tail ? 1.0f : (sv == 0.0f ? 0.0f : 1.0f / sv)};
+    }
+}
+
+// loss = sum_j q_j (log q_j - log p_(i_j)), and with TAIL the mass outside the entries as one more class:
+// + q_r (log q_r - log p_r), where p_r is summed over those classes themselves (1 - sum would cancel).  For that every
+// class an entry names is marked in LDS and blanked when its thread comes to it; the entries' own classes are summed
+// from a second look at them.
+
+// The sums (me, se) over the classes the entries name in [lo, hi), each once; mark(class) says whether it was marked
+// before.  The G threads of the unit share the entries; the result is the wave's (or its group's).
+template <int G, typename T, typename Mark>
+__device__ __forceinline__ void mark_entries(const DistillArgs& a, const T* z, long long row, int lo, int hi, unsigned* repeated,
+                                             DistillPart& t, Mark mark) {
+    constexpr int L = G < 64 ? G : 64;
+    const int tid = threadIdx.x & (G - 1);
+    bool twice = false;
+    for (int j = tid; j < a.k; j += G) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i >= lo && i < hi) twice |= mark((int)i);
+    }
+    if constexpr (G <= 64) {
+        twice = group_any<G>(twice);
+        together<G>();
+    } else {
+        if (twice) *repeated = 1u;
+        together<G>();
+        twice = *repeated != 0;
+    }
+    for (int j = tid; j < a.k; j += G) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < lo || i >= hi) continue;
+        if (twice && named_before(a, row, j, i)) continue;
+        const float zi = ld(z, i);
+        merge(t.me, t.se, zi, zi == -INFINITY ? 0.0f : 1.0f, a.c, a.c_lo);
+    }
+    const float m = group_max<L>(t.me);
+    t.se = group_sum<L>(t.se == 0.0f ? 0.0f : t.se * power(t.me, m, a.c, a.c_lo));
+    t.me = m;
+}
+
+// A row in the registers of G lanes.
+template <typename T, int G, int NE, bool TAIL>
+__global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restrict__ logits, DistillArgs a) {
+    __shared__ u64 marks[TAIL ? kThreads : 1];  // a thread's elements that an entry names, one bit each
+    const int lane = threadIdx.x & (G - 1);
+    const long long row = block_index() * (kThreads / G) + threadIdx.x / G;
+    if (row >= a.units) return;
+    if (a.live && !a.live[row]) {
+        if (lane == 0) distill_dead(a, row);
+        return;
+    }
+    const T* z = logits + row * a.row_stride;
+    using S = Span<T, G, NE>;
+    const S span(z, 0, a.cols, lane);
+    float v[NE];
+    span.template load<true>(z, v);
+    DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    if constexpr (TAIL) {
+        u64* mine = marks + (threadIdx.x - lane);
+        mine[lane] = 0ull;
+        together<G>();
+        mark_entries<G>(a, z, row, 0, a.cols, nullptr, t, [&](int i) {
+            int thread, e;
+            span.locate(i, thread, e);
+            return (atomicOr(&mine[thread], 1ull << e) >> e & 1ull) != 0;
+        });
+        const unsigned hit[2] = {(unsigned)mine[lane], (unsigned)(mine[lane] >> 32)};
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] = hit[e / 32] >> (e % 32) & 1u ? -INFINITY : v[e];
+    }
+    float m = v[0];
+#pragma unroll
+    for (int e = 1; e < NE; ++e) m = fmaxf(m, v[e]);
+    t.m = group_max<G>(m);
+    const float mz = t.m == -INFINITY ? 0.0f : t.m;
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s += power_of<T>(a, v[e], mz);
+    t.s = group_sum<G>(s);
+    distill_finish<G>(a, z, row, t);
+}
+
+// A part of a longer row: a workgroup walks over it, kThreads * NE classes at a time, the next ones being loaded
+// meanwhile.  Every wave keeps its own maximum and its lanes their own sums until the end.  The marks are one bit a class
+// of the part.
+template <typename T, int NE, bool TAIL>
+__global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __restrict__ logits, DistillArgs a) {
+    __shared__ DistillPart red[4];
+    __shared__ unsigned char marks[TAIL ? kMarkCols / 8 + 16 : 16] __attribute__((aligned(16)));
+    __shared__ unsigned repeated;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const long long unit = block_index();
+    if (unit >= a.units) return;
+    const long long row = a.splits == 1 ? unit : unit / a.splits;
+    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    if (a.live && !a.live[row]) {
+        if (tid == 0 && a.splits == 1) distill_dead(a, row);
+        return;
+    }
+    const T* z = logits + row * a.row_stride;
+    using S = Span<T, kThreads, NE>;
+    const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
+    unsigned raw[S::kWords];
+    S ahead(z, lo, hi, tid);
+    const int zero = ahead.first;  // the class of the first mark
+    ahead.fetch(z, raw);
+    DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    if constexpr (TAIL) {
+        unsigned* words = reinterpret_cast<unsigned*>(marks);
+        for (int i = tid; i < (hi - zero + 31) / 32; i += kThreads) words[i] = 0u;
+        if (tid == 0) repeated = 0u;
+        __syncthreads();
+        mark_entries<kThreads>(a, z, row, lo, hi, &repeated, t, [&](int i) {
+            const int b = i - zero;
+            return (atomicOr(&words[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) != 0;
+        });
+    }
+    float s = 0.0f;
+    while (ahead.more()) {
+        const S span = ahead;
+        float v[NE];
+        span.unpack(raw, v);
+        ahead.next();
+        if (ahead.more()) ahead.fetch(z, raw);
+        if constexpr (TAIL) {
+#pragma unroll
+            for (int q = 0; q < S::NV; ++q) {
+                const int first = span.start(q), b = first - zero;
+                unsigned bits = 0;
+                if (first < hi) bits = (unsigned)marks[b >> 3] >> (b & 7) & ((1u << S::VE) - 1u);
+                if (__ballot(bits != 0)) {
+                    const int from = first - span.inside(first);  // (an outer vector is read from further in)
+                    bits = from >= 0 ? bits << from : bits >> -from;
+#pragma unroll
+                    for (int j = 0; j < S::VE; ++j) v[q * S::VE + j] = bits >> j & 1u ? -INFINITY : v[q * S::VE + j];
+                }
+            }
+        }
+        float lane_max = v[0];
+#pragma unroll
+        for (int e = 1; e < NE; ++e) lane_max = fmaxf(lane_max, v[e]);
+        if (__ballot(lane_max > t.m)) {
+            const float m = group_max<64>(lane_max);
+            if (t.m != -INFINITY) s *= power(t.m, m, a.c, a.c_lo);
+            t.m = m;
+        }
+        const float mz = t.m == -INFINITY ? 0.0f : t.m;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) s += power_of<T>(a, v[e], mz);
+    }
+    t.s = group_sum<64>(s);
+    if (lane == 0) red[tid >> 6] = t;
+    __syncthreads();
+    if (tid >= 64) return;
+    t = red[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        merge(t.m, t.s, red[w].m, red[w].s, a.c, a.c_lo);
+        if constexpr (TAIL) merge(t.me, t.se, red[w].me, red[w].se, a.c, a.c_lo);
+    }
+    if (a.splits == 1)
+        distill_finish<64>(a, z, row, t);
+    else if (lane == 0)
+        a.part[unit] = t;
+}
+
+// Joins the parts of a row: one wave.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void distill_join_kernel(const T* __restrict__ logits, DistillArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long row = block_index() * 4 + (threadIdx.x >> 6);
+    if (row >= a.units) return;
+    if (a.live && !a.live[row]) {
+        if (lane == 0) distill_dead(a, row);
+        return;
+    }
+    DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    for (int i = lane; i < a.splits; i += 64) {
+        const DistillPart p = a.part[row * a.splits + i];
+        merge(t.m, t.s, p.m, p.s, a.c, a.c_lo);
+        merge(t.me, t.se, p.me, p.se, a.c, a.c_lo);
+    }
+    const float m = group_max<64>(t.m), me = group_max<64>(t.me);
+    t.s = group_sum<64>(t.s == 0.0f ? 0.0f : t.s * power(t.m, m, a.c, a.c_lo));
+    t.se = group_sum<64>(t.se == 0.0f ? 0.0f : t.se * power(t.me, me, a.c, a.c_lo));
+    t.m = m, t.me = me;
+    distill_finish<64>(a, logits + row * a.row_stride, row, t);
+}
+
+struct DistillBwdArgs {
+    const float* values;
+    const void* classes;
+    const DistillStats* stats;
+    const float* dloss;
+    long long row_stride, units;
+    int class_bytes, cols, splits, per, k, tail;
+    float c, c_lo, inv_t;
+};
+
+template <typename T, int G, int NE>
+__global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restrict__ logits, DistillBwdArgs a,
+                                                              T* __restrict__ dlogits) {
+    __shared__ u64 marks[kThreads];
+    __shared__ unsigned repeated;
+    const int tid = threadIdx.x & (G - 1);
+    // (from the last unit back: what the forward pass read last is still in the last-level cache)
+    const long long unit = a.units - 1 - (block_index() * (kThreads / G) + threadIdx.x / G);
+    if (unit < 0) return;
+    const long long row = a.splits == 1 ? unit : unit / a.splits;
+    const int split = a.splits == 1 ? 0 : (int)(unit - row * a.splits);
+    using S = Span<T, G, NE>;
+    const int lo = split * a.per, hi = lo + a.per < a.cols ? lo + a.per : a.cols;
+    T* d = dlogits + row * a.cols;
+    const S span(d, lo, hi, tid);  // (aligned as the gradient; dense logits lie the same way)
+    const DistillStats st = a.stats[row];
+    const bool zero = st.is == 0.0f;  // a dead row, or no class has probability
+    const T* z = logits + row * a.row_stride;
+    float v[NE];
+    if (!zero) span.template load<false>(z, v);
+    const float g = a.dloss[row] * a.inv_t;
+    const float gc = g * st.coef * st.ib;
+#pragma unroll
+    for (int t = 0; t < S::NV; ++t) {
+        if (span.beyond(t)) break;
+        float o[S::VE];
+#pragma unroll
+        for (int j = 0; j < S::VE; ++j) {
+            const float zi = v[t * S::VE + j];
+            const float e = sizeof(T) == 4 ? power_exact(zi, st.mb, a.c, a.c_lo) : __builtin_amdgcn_exp2f((zi - st.mb) * a.c);
+            o[j] = zero ? 0.0f : gc * e;
+        }
+        span.store(d, t, o);
+    }
+    if (zero || st.coef != st.coef) return;  // (NaN: an entry the row does not have; the whole row is)
+    // the entries' classes once more, behind the dense part
+    u64* mine = marks + (threadIdx.x - tid);
+    mine[tid] = 0ull;
+    if (G > 64 && tid == 0) repeated = 0u;
+    together<G>();
+    bool twice = false;
+    for (int j = tid; j < a.k; j += G) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < lo || i >= hi) continue;
+        int thread, e;
+        span.locate((int)i, thread, e);
+        twice |= (atomicOr(&mine[thread], 1ull << e) >> e & 1ull) != 0;
+    }
+    if constexpr (G <= 64) {
+        twice = group_any<G>(twice);
+    } else {
+        if (twice) repeated = 1u;
+        together<G>();
+        twice = repeated != 0;
+    }
+    const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
+    for (int j = tid; j < a.k; j += G) {
+        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
+        if (i < lo || i >= hi) continue;
+        float q = st.iv * power_exact(a.values[row * a.k + j], st.mv, cv, cv_lo);
+        if (twice) {  // (every place of the class writes the same sum)
+            q = 0.0f;
+            for (int o = 0; o < a.k; ++o)
+                if (class_at(a.classes, a.class_bytes, row * a.k + o) == i)
+                    q += st.iv * power_exact(a.values[row * a.k + o], st.mv, cv, cv_lo);
+        }
+        const float p = st.is * power_exact(ld(z, i), st.m, a.c, a.c_lo);
+        const float o = g * (st.total * p - q);
+        store_vector<1>(d + i, &o);
+    }
+}
+
+template <typename T, bool TAIL>
+struct DistillFwd {
+    template <int G, int NE>
+    static void run(const void* logits, const DistillArgs& a, hipStream_t s) {
+        hipLaunchKernelGGL((distill_fwd_kernel<T, G, NE, TAIL>), grid_of(a.units, G), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits), a);
+    }
+    static void launch(const Cut& cut, const void* logits, const DistillArgs& a, hipStream_t s) {
+        if (cut.lanes != kThreads)
+            with_wave<DistillFwd>(cut, logits, a, s);
+        else
+            hipLaunchKernelGGL((distill_stream_kernel<T, 16, TAIL>), grid_of(a.units, kThreads), dim3(kThreads), 0, s,
+                               static_cast<const T*>(logits), a);
+    }
+};
+template <typename T>
+struct DistillBwd {
+    template <int G, int NE>
+    static void run(const void* logits, const DistillBwdArgs& a, void* dlogits, hipStream_t s) {
+        hipLaunchKernelGGL((distill_bwd_kernel<T, G, NE>), grid_of(a.units, G), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits), a, static_cast<T*>(dlogits));
+    }
+};
+
+int check_entries(const char* who, int k, int tail) {
+    ISG_REQUIRE(k >= 1 && k <= kMaxEntries, ISG_EINVAL, "%s: k=%d classes of the teacher (1 to %d)", who, k, kMaxEntries);
+    ISG_REQUIRE(tail == 0 || tail == 1, ISG_EINVAL, "%s: tail=%d", who, tail);
+    return ISG_OK;
+}
+
+}  // namespace
+
+extern "C" long long isg_distill_workspace_bytes(int rows, int cols) {
+    if (rows < 0 || cols < 1 || cols > kMaxCols) return -1;
+    const Cut cut = cut_forward(rows, cols, ISG_BF16);  // (the same for float: types differ in rows of one part)
+    return cut.splits == 1 ? 0 : (long long)rows * cut.splits * (long long)sizeof(DistillPart);
+}
+
+extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const float* values, const void* classes,
+                               int class_bytes, const unsigned char* live, int rows, int cols, int k, int dtype,
+                               float temperature, int tail, float* loss, float* stats, void* workspace, void* stream) {
+    const char* who = "isg_distill_fwd";
+    int rc = check_call(who, row_stride, rows, cols, dtype, temperature);
+    if (rc != ISG_OK) return rc;
+    rc = check_entries(who, k, tail);
+    if (rc != ISG_OK) return rc;
+    rc = check_bytes(who, classes, class_bytes);
+    if (rc != ISG_OK) return rc;
+    if (rows == 0) return ISG_OK;
+    ISG_REQUIRE(logits && values && classes && loss, ISG_EINVAL, "%s: null pointer", who);
+    const Cut cut = cut_forward(rows, cols, dtype);
+    ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DistillArgs a{};
+    a.values = values, a.classes = classes, a.live = live, a.loss = loss;
+    a.stats = reinterpret_cast<DistillStats*>(stats), a.part = static_cast<DistillPart*>(workspace);
+    a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
+    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.k = k, a.tail = tail;
+    scale_of(temperature, a.c, a.c_lo, a.inv_t);
+    a.c_near = (float)(1.4426950408889634074 / (double)temperature);
+    if (dtype == ISG_F32)
+        tail ? DistillFwd<float, true>::launch(cut, logits, a, s) : DistillFwd<float, false>::launch(cut, logits, a, s);
+    else
+        tail ? DistillFwd<__hip_bfloat16, true>::launch(cut, logits, a, s)
+             : DistillFwd<__hip_bfloat16, false>::launch(cut, logits, a, s);
+    rc = isg::check_launch("distill_fwd_kernel");
+    if (rc != ISG_OK || cut.splits == 1) return rc;
+    a.units = rows;
+    if (dtype == ISG_F32)
+        hipLaunchKernelGGL(distill_join_kernel<float>, grid_of(rows, 64), dim3(kThreads), 0, s,
+                           static_cast<const float*>(logits), a);
+    else
+        hipLaunchKernelGGL(distill_join_kernel<__hip_bfloat16>, grid_of(rows, 64), dim3(kThreads), 0, s,
+                           static_cast<const __hip_bfloat16*>(logits), a);
+    return isg::check_launch("distill_join_kernel");
+}
+
+extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const float* values, const void* classes,
+                               int class_bytes, const float* stats, const float* dloss, int rows, int cols, int k,
+                               int dtype, float temperature, int tail, void* dlogits, void* stream) {
+    const char* who = "isg_distill_bwd";
+    int rc = check_call(who, row_stride, rows, cols, dtype, temperature);
+    if (rc != ISG_OK) return rc;
+    rc = check_entries(who, k, tail);
+    if (rc != ISG_OK) return rc;
+    rc = check_bytes(who, classes, class_bytes);
+    if (rc != ISG_OK) return rc;
+    if (rows == 0) return ISG_OK;
+    ISG_REQUIRE(logits && values && classes && stats && dloss && dlogits, ISG_EINVAL, "%s: null pointer", who);
+    ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
+    const Cut cut = cut_backward(rows, cols, dtype);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DistillBwdArgs a{};
+    a.values = values, a.classes = classes, a.stats = reinterpret_cast<const DistillStats*>(stats), a.dloss = dloss;
+    a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
+    a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.k = k, a.tail = tail;
+    scale_of(temperature, a.c, a.c_lo, a.inv_t);
+    if (dtype == ISG_F32) launch_backward<DistillBwd<float>>(cut, logits, a, dlogits, s);
+    else launch_backward<DistillBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
+    return isg::check_launch("distill_bwd_kernel");
+}
