@@ -9,7 +9,8 @@
 //
 // Layout.  A row is read once, into registers: up to about 1,000 classes by 16 lanes (four rows a wave: what a row costs
 // once - reductions, logarithms, outputs - is paid for four rows in the same instructions), up to about 2,000 by 32
-// lanes.  Longer rows are walked over by workgroups, a part of the row each, whose results a second launch joins.
+// lanes, or by a whole wave where there are few rows.  Longer rows are walked over by workgroups, a part of the row each,
+// whose results a second launch joins.
 #pragma once
 #include <hip/hip_bf16.h>
 
@@ -305,17 +306,23 @@ struct Cut {
     int lanes, ne, splits, per;  // lanes = kThreads: workgroups
 };
 inline int equal_part(int cols, int splits) { return ((cols + splits - 1) / splits + 7) / 8 * 8; }
-// lanes = 0: too long for a wave's registers
-inline Cut cut_wave(int cols, int dtype) {
-    const int sizes[] = {1, 4, 8, 16, 24, 32, 40, 48, 56, 64}, most = dtype == ISG_F32 ? 4 : 8;
-    for (int ne : sizes)
-        if (cols + (ne < most ? ne : most) - 1 <= 16 * ne) return Cut{16, ne, 1, cols};
-    for (int ne : {48, 64})
-        if (cols + most - 1 <= 32 * ne) return Cut{32, ne, 1, cols};
+// lanes = 0: too long for a wave's registers.  16 lanes a row (32 for the longer) where there are rows enough for every
+// SIMD to have waves, else a whole wave: 16 rows of 785 classes take 4.6 us so and 6.8 us in 16 lanes each, 131,072 rows
+// 64 and 47 us.  `entries`: places a row needs in its threads' registers, four a thread (sixteen in rows of 64 classes).
+inline Cut cut_wave(long long rows, int cols, int dtype, int entries) {
+    const int most = dtype == ISG_F32 ? 4 : 8;
+    if (rows > 4096 && entries <= 64) {
+        for (int ne : {1, 4, 8, 16, 24, 32, 40, 48, 56, 64})
+            if (cols + (ne < most ? ne : most) - 1 <= 16 * ne) return Cut{16, ne, 1, cols};
+        for (int ne : {48, 64})
+            if (cols + most - 1 <= 32 * ne) return Cut{32, ne, 1, cols};
+    }
+    for (int ne : {1, 4, 8, 16, 24, 32})
+        if ((ne == 1 || entries <= 256) && cols + (ne < most ? ne : most) - 1 <= 64 * ne) return Cut{64, ne, 1, cols};
     return Cut{0, 0, 1, cols};
 }
-inline Cut cut_forward(long long rows, int cols, int dtype) {
-    const Cut wave = cut_wave(cols, dtype);
+inline Cut cut_forward(long long rows, int cols, int dtype, int entries = 0) {
+    const Cut wave = cut_wave(rows, cols, dtype, entries);
     if (wave.lanes) return wave;
     long long splits = (kUnits + rows - 1) / (rows > 0 ? rows : 1);
     const int most = cols / kPartCols < kMaxSplits ? cols / kPartCols : kMaxSplits, least = (cols + kMarkCols - 1) / kMarkCols;
@@ -324,8 +331,8 @@ inline Cut cut_forward(long long rows, int cols, int dtype) {
     const int per = equal_part(cols, (int)splits);
     return Cut{kThreads, 16, (cols + per - 1) / per, per};
 }
-inline Cut cut_backward(long long rows, int cols, int dtype) {
-    const Cut wave = cut_wave(cols, dtype);
+inline Cut cut_backward(long long rows, int cols, int dtype, int entries = 0) {
+    const Cut wave = cut_wave(rows, cols, dtype, entries);
     if (wave.lanes) return wave;
     const auto parts = [&](int ne) { return (cols + kThreads * ne - 8 - 1) / (kThreads * ne - 8); };
     for (int ne = 8;; ne *= 2) {
@@ -348,6 +355,17 @@ void with_wave(const Cut& cut, A&&... args) {
     if (cut.lanes == 32) {
         if (cut.ne == 48) F::template run<32, 48>(args...);
         else F::template run<32, 64>(args...);
+        return;
+    }
+    if (cut.lanes == 64) {
+        switch (cut.ne) {
+            case 1: F::template run<64, 1>(args...); break;
+            case 4: F::template run<64, 4>(args...); break;
+            case 8: F::template run<64, 8>(args...); break;
+            case 16: F::template run<64, 16>(args...); break;
+            case 24: F::template run<64, 24>(args...); break;
+            default: F::template run<64, 32>(args...);
+        }
         return;
     }
     switch (cut.ne) {

@@ -57,10 +57,38 @@ __device__ __forceinline__ void distill_dead(const DistillArgs& a, long long row
     if (a.stats) a.stats[row] = DistillStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 }
 
+// A row's entries in the registers of its G threads: entry i * G + thread in place i < N.  (Four places; sixteen, for
+// every k there can be, where a wave closes a row of any length and for rows too short for a workgroup.)
+template <int G, int N>
+struct Entries {
+    int cls[N];    // -1: none, cols: a class the row does not have
+    float val[N];
+
+    __device__ __forceinline__ void load(const float* values, const void* classes, int bytes, long long row, int k, int cols) {
+        const int thread = threadIdx.x & (G - 1);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            cls[i] = -1, val[i] = 0.0f;
+            const int j = i * G + thread;
+            if (i * G < k && j < k) {
+                const long long c = class_at(classes, bytes, row * k + j);
+                cls[i] = c < 0 ? -1 : (c < cols ? (int)c : cols);
+                val[i] = values[row * k + j];
+            }
+        }
+    }
+    // the logits of the classes in [lo, hi), -inf for the others
+    template <typename T>
+    __device__ __forceinline__ void gather(const T* z, int lo, int hi, float (&ze)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) ze[i] = cls[i] >= lo && cls[i] < hi ? ld(z, cls[i]) : -INFINITY;
+    }
+};
+
 // whether an earlier entry names the class as well
-__device__ bool named_before(const DistillArgs& a, long long row, int j, long long cls) {
+__device__ __noinline__ bool named_before(const void* classes, int bytes, long long row, int k, int j, int cls) {
     for (int o = 0; o < j; ++o)
-        if (class_at(a.classes, a.class_bytes, row * a.k + o) == cls) return true;
+        if (class_at(classes, bytes, row * k + o) == cls) return true;
     return false;
 }
 
@@ -71,10 +99,10 @@ __device__ __forceinline__ float log1p_of(float x) {
 }
 
 // The loss of a row from its sums, by G lanes of a wave.
-template <int G, typename T>
-__device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z, long long row, const DistillPart& t) {
+template <int G, int N>
+__device__ __forceinline__ void distill_finish(const DistillArgs& a, const Entries<G, N>& en, const float (&ze)[N],
+                                               long long row, const DistillPart& t) {
     const int lane = threadIdx.x & (G - 1);
-    const float* v = a.values + row * a.k;
     float m = t.m, s = t.s;
     if (a.tail) merge(m, s, t.me, t.se, a.c, a.c_lo);
     m = m == -INFINITY ? 0.0f : m;
@@ -84,32 +112,39 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
     const float s_exp = (float)__builtin_amdgcn_frexp_expf(s), s_log = kLn2 * __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s));
     // the teacher's distribution over its entries
     const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
-    float mv = 0.0f, lv = 0.0f, sv = 0.0f;
+    float mv = 0.0f, lv = 0.0f, sv = 0.0f, q[N];
     bool bad = false;
     if (!a.tail) {
         mv = -INFINITY;
-        for (int j = lane; j < a.k; j += G)
-            if (class_at(a.classes, a.class_bytes, row * a.k + j) >= 0) mv = fmaxf(mv, v[j]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) mv = en.cls[i] >= 0 ? fmaxf(mv, en.val[i]) : mv;
         mv = group_max<G>(mv);
         if (mv == -INFINITY) mv = 0.0f;
     }
-    for (int j = lane; j < a.k; j += G) {
-        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-        if (i >= 0) sv += power(v[j], mv, cv, cv_lo);
-        bad |= i >= a.cols;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        q[i] = 0.0f;
+        if (i * G < a.k) {
+            q[i] = en.cls[i] >= 0 ? power(en.val[i], mv, cv, cv_lo) : 0.0f;
+            sv += q[i];
+            bad |= en.cls[i] >= a.cols;
+        }
     }
     sv = group_sum<G>(sv);
     if (!a.tail) lv = sv == 0.0f ? INFINITY : __builtin_amdgcn_logf(sv);
     const float qsum = a.tail ? sv : (sv == 0.0f ? 0.0f : 1.0f);
     float qr = a.tail ? fmaxf(1.0f - sv, 0.0f) : 0.0f;
     float l = 0.0f;
-    for (int j = lane; j < a.k; j += G) {
-        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-        if (i < 0 || i >= a.cols) continue;
-        const float q = power(v[j], mv, cv, cv_lo) * __builtin_amdgcn_exp2f(-lv);
-        const float lq = (v[j] - mv) * (a.tail ? 1.0f : a.inv_t) - kLn2 * lv;
-        const float d = lq - (ld(z, i) - m) * a.inv_t;  // log q - log p - log s
-        if (q != 0.0f) l += s == 0.0f ? INFINITY : q * (__builtin_fmaf(s_exp, kLn2, d) + s_log);
+    const float iv = a.tail ? 1.0f : (sv == 0.0f ? 0.0f : 1.0f / sv);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i * G < a.k) {
+            const float qi = q[i] * iv;
+            const float lq = (en.val[i] - mv) * (a.tail ? 1.0f : a.inv_t) - kLn2 * lv;
+            const float d = lq - (ze[i] - m) * a.inv_t;  // log q - log p - log s
+            const float term = s == 0.0f ? INFINITY : qi * (__builtin_fmaf(s_exp, kLn2, d) + s_log);
+            if (qi != 0.0f && en.cls[i] < a.cols) l += term;
+        }
     }
     l = group_sum<G>(l);
     bad = group_any<G>(bad);
@@ -138,8 +173,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
         if (bad) l = NAN, coef = NAN;
         a.loss[row] = l;
         if (a.stats)
-            a.stats[row] = DistillStats{mb, ib, coef, qsum + qr, m, s == 0.0f ? 0.0f : 1.0f / s, mv,
-                                        a.tail ? 1.0f : (sv == 0.0f ? 0.0f : 1.0f / sv)};
+            a.stats[row] = DistillStats{mb, ib, coef, qsum + qr, m, s == 0.0f ? 0.0f : 1.0f / s, mv, iv};
     }
 }
 
@@ -150,16 +184,20 @@ __device__ __forceinline__ void distill_finish(const DistillArgs& a, const T* z,
 
 // The sums (me, se) over the classes the entries name in [lo, hi), each once; mark(class) says whether it was marked
 // before.  The G threads of the unit share the entries; the result is the wave's (or its group's).
-template <int G, typename T, typename Mark>
-__device__ __forceinline__ void mark_entries(const DistillArgs& a, const T* z, long long row, int lo, int hi, unsigned* repeated,
-                                             DistillPart& t, Mark mark) {
+template <int G, int N, typename Mark>
+__device__ __forceinline__ void mark_entries(const DistillArgs& a, const Entries<G, N>& en, const float (&ze)[N],
+                                             long long row, int lo, int hi, unsigned* repeated, DistillPart& t, Mark mark) {
     constexpr int L = G < 64 ? G : 64;
-    const int tid = threadIdx.x & (G - 1);
     bool twice = false;
-    for (int j = tid; j < a.k; j += G) {
-        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-        if (i >= lo && i < hi) twice |= mark((int)i);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i * G < a.k) {
+            if (en.cls[i] >= lo && en.cls[i] < hi) twice |= mark(en.cls[i]);
+            m = fmaxf(m, ze[i]);
+        }
     }
+    t.me = group_max<L>(m);
     if constexpr (G <= 64) {
         twice = group_any<G>(twice);
         together<G>();
@@ -168,16 +206,17 @@ __device__ __forceinline__ void mark_entries(const DistillArgs& a, const T* z, l
         together<G>();
         twice = *repeated != 0;
     }
-    for (int j = tid; j < a.k; j += G) {
-        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-        if (i < lo || i >= hi) continue;
-        if (twice && named_before(a, row, j, i)) continue;
-        const float zi = ld(z, i);
-        merge(t.me, t.se, zi, zi == -INFINITY ? 0.0f : 1.0f, a.c, a.c_lo);
+    const float mz = t.me == -INFINITY ? 0.0f : t.me;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i * G < a.k) {
+            bool first = en.cls[i] >= lo && en.cls[i] < hi;
+            if (twice && first)
+                first = !named_before(a.classes, a.class_bytes, row, a.k, i * G + (int)(threadIdx.x & (G - 1)), en.cls[i]);
+            if (first) t.se += power(ze[i], mz, a.c, a.c_lo);
+        }
     }
-    const float m = group_max<L>(t.me);
-    t.se = group_sum<L>(t.se == 0.0f ? 0.0f : t.se * power(t.me, m, a.c, a.c_lo));
-    t.me = m;
+    t.se = group_sum<L>(t.se);
 }
 
 // A row in the registers of G lanes.
@@ -194,14 +233,18 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
     const T* z = logits + row * a.row_stride;
     using S = Span<T, G, NE>;
     const S span(z, 0, a.cols, lane);
-    float v[NE];
+    constexpr int N = G == 64 && NE == 1 ? 16 : 4;
+    Entries<G, N> en;
+    en.load(a.values, a.classes, a.class_bytes, row, a.k, a.cols);
+    float v[NE], ze[N];
     span.template load<true>(z, v);
+    en.gather(z, 0, a.cols, ze);
     DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
     if constexpr (TAIL) {
         u64* mine = marks + (threadIdx.x - lane);
         mine[lane] = 0ull;
         together<G>();
-        mark_entries<G>(a, z, row, 0, a.cols, nullptr, t, [&](int i) {
+        mark_entries(a, en, ze, row, 0, a.cols, nullptr, t, [&](int i) {
             int thread, e;
             span.locate(i, thread, e);
             return (atomicOr(&mine[thread], 1ull << e) >> e & 1ull) != 0;
@@ -219,7 +262,17 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
 #pragma unroll
     for (int e = 0; e < NE; ++e) s += power_of<T>(a, v[e], mz);
     t.s = group_sum<G>(s);
-    distill_finish<G>(a, z, row, t);
+    distill_finish(a, en, ze, row, t);
+}
+
+// The loss of a longer row, by one wave.
+template <typename T>
+__device__ __forceinline__ void finish_row(const DistillArgs& a, const T* z, long long row, const DistillPart& t) {
+    Entries<64, 16> en;
+    en.load(a.values, a.classes, a.class_bytes, row, a.k, a.cols);
+    float ze[16];
+    en.gather(z, 0, a.cols, ze);
+    distill_finish(a, en, ze, row, t);
 }
 
 // A part of a longer row: a workgroup walks over it, kThreads * NE classes at a time, the next ones being loaded
@@ -248,11 +301,15 @@ __global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __res
     ahead.fetch(z, raw);
     DistillPart t{-INFINITY, 0.0f, -INFINITY, 0.0f};
     if constexpr (TAIL) {
+        Entries<kThreads, 4> en;
+        en.load(a.values, a.classes, a.class_bytes, row, a.k, a.cols);
+        float ze[4];
+        en.gather(z, lo, hi, ze);
         unsigned* words = reinterpret_cast<unsigned*>(marks);
         for (int i = tid; i < (hi - zero + 31) / 32; i += kThreads) words[i] = 0u;
         if (tid == 0) repeated = 0u;
         __syncthreads();
-        mark_entries<kThreads>(a, z, row, lo, hi, &repeated, t, [&](int i) {
+        mark_entries(a, en, ze, row, lo, hi, &repeated, t, [&](int i) {
             const int b = i - zero;
             return (atomicOr(&words[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) != 0;
         });
@@ -301,7 +358,7 @@ __global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __res
         if constexpr (TAIL) merge(t.me, t.se, red[w].me, red[w].se, a.c, a.c_lo);
     }
     if (a.splits == 1)
-        distill_finish<64>(a, z, row, t);
+        finish_row(a, z, row, t);
     else if (lane == 0)
         a.part[unit] = t;
 }
@@ -326,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void distill_join_kernel(const T* __restr
     t.s = group_sum<64>(t.s == 0.0f ? 0.0f : t.s * power(t.m, m, a.c, a.c_lo));
     t.se = group_sum<64>(t.se == 0.0f ? 0.0f : t.se * power(t.me, me, a.c, a.c_lo));
     t.m = m, t.me = me;
-    distill_finish<64>(a, logits + row * a.row_stride, row, t);
+    finish_row(a, logits + row * a.row_stride, row, t);
 }
 
 struct DistillBwdArgs {
@@ -357,8 +414,14 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     const DistillStats st = a.stats[row];
     const bool zero = st.is == 0.0f;  // a dead row, or no class has probability
     const T* z = logits + row * a.row_stride;
-    float v[NE];
-    if (!zero) span.template load<false>(z, v);
+    constexpr int N = G == 64 && NE == 1 ? 16 : 4;
+    Entries<G, N> en;
+    float v[NE], ze[N];
+    if (!zero) {
+        en.load(a.values, a.classes, a.class_bytes, row, a.k, a.cols);
+        span.template load<false>(z, v);
+        en.gather(z, lo, hi, ze);
+    }
     const float g = a.dloss[row] * a.inv_t;
     const float gc = g * st.coef * st.ib;
 #pragma unroll
@@ -380,13 +443,13 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     if (G > 64 && tid == 0) repeated = 0u;
     together<G>();
     bool twice = false;
-    for (int j = tid; j < a.k; j += G) {
-        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-        if (i < lo || i >= hi) continue;
-        int thread, e;
-        span.locate((int)i, thread, e);
-        twice |= (atomicOr(&mine[thread], 1ull << e) >> e & 1ull) != 0;
-    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i * G < a.k && en.cls[i] >= lo && en.cls[i] < hi) {
+            int thread, e;
+            span.locate(en.cls[i], thread, e);
+            twice |= (atomicOr(&mine[thread], 1ull << e) >> e & 1ull) != 0;
+        }
     if constexpr (G <= 64) {
         twice = group_any<G>(twice);
     } else {
@@ -395,19 +458,19 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
         twice = repeated != 0;
     }
     const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
-    for (int j = tid; j < a.k; j += G) {
-        const long long i = class_at(a.classes, a.class_bytes, row * a.k + j);
-        if (i < lo || i >= hi) continue;
-        float q = st.iv * power_exact(a.values[row * a.k + j], st.mv, cv, cv_lo);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = en.cls[i];
+        if (i * G >= a.k || c < lo || c >= hi) continue;
+        float q = st.iv * power_exact(en.val[i], st.mv, cv, cv_lo);
         if (twice) {  // (every place of the class writes the same sum)
             q = 0.0f;
             for (int o = 0; o < a.k; ++o)
-                if (class_at(a.classes, a.class_bytes, row * a.k + o) == i)
+                if (class_at(a.classes, a.class_bytes, row * a.k + o) == c)
                     q += st.iv * power_exact(a.values[row * a.k + o], st.mv, cv, cv_lo);
         }
-        const float p = st.is * power_exact(ld(z, i), st.m, a.c, a.c_lo);
-        const float o = g * (st.total * p - q);
-        store_vector<1>(d + i, &o);
+        const float o = g * (st.total * (st.is * power_exact(ze[i], st.m, a.c, a.c_lo)) - q);
+        store_vector<1>(d + c, &o);
     }
 }
 
@@ -461,7 +524,7 @@ extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const f
     if (rc != ISG_OK) return rc;
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && loss, ISG_EINVAL, "%s: null pointer", who);
-    const Cut cut = cut_forward(rows, cols, dtype);
+    const Cut cut = cut_forward(rows, cols, dtype, k);
     ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
     DistillArgs a{};
@@ -501,7 +564,7 @@ extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const f
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && stats && dloss && dlogits, ISG_EINVAL, "%s: null pointer", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
-    const Cut cut = cut_backward(rows, cols, dtype);
+    const Cut cut = cut_backward(rows, cols, dtype, k);
     hipStream_t s = static_cast<hipStream_t>(stream);
     DistillBwdArgs a{};
     a.values = values, a.classes = classes, a.stats = reinterpret_cast<const DistillStats*>(stats), a.dloss = dloss;

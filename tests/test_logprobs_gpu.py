@@ -114,6 +114,98 @@ def test_logprobs_over_masks_and_ties(kind, cols, dtype):
         _check_logprobs(t, z, 0.7, tokens, top, dtype, seed=cols + top)
 
 
+# Launches of thousands of rows hold several rows a wave: the same rows over and over, starting at every address.
+MANY = 37 * 113
+
+
+def _many(a):
+    return None if a is None else np.concatenate([a] * 113)
+
+
+def _check_many(t, z, T, tokens, top, live, dtype, rs):
+    decode = _decode()
+    big = t.repeat(113, 1).requires_grad_(True)
+    want = {k: _many(v) for k, v in ref.token_logprobs(z, T, tokens, top).items()}
+    on = _many(live)
+    out = decode.token_logprobs(big, torch.tensor(_many(tokens), device=DEV), top=top, temperature=T,
+                                live=torch.tensor(on, device=DEV))
+    for name in ("logprobs", "entropy", "top_logprobs"):
+        if name in want:
+            got = _f64(getattr(out, name))
+            ref.close(got[on], want[name][on], want[name + "_tol"][on])
+            assert np.all(got[~on] == 0)
+    if top:
+        got = out.top_classes.cpu().numpy()
+        assert np.array_equal(got[on], want["top_classes"][on]) and np.all(got[~on] == -1)
+    gl, gh = rs.randn(37).astype(np.float32), rs.randn(37).astype(np.float32)
+    gt = rs.randn(37, top).astype(np.float32) if top else None
+    outs = [out.logprobs, out.entropy] + ([out.top_logprobs] if top else [])
+    gs = [torch.tensor(_many(g), device=DEV) for g in (gl, gh, gt) if g is not None]
+    dz, = torch.autograd.grad(outs, big, gs)
+    f = lambda g: None if g is None else g.astype(np.float64)
+    classes = ref.token_logprobs(z, T, None, top).get("top_classes")
+    wd, wtol = ref.token_logprobs_grad(z, T, tokens, classes, f(gl), f(gh), f(gt), dtype)
+    got = _f64(dz)
+    ref.close(got[on], _many(wd)[on], _many(wtol)[on])
+    assert np.all(got[~on] == 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["peaked", "masked"])
+@pytest.mark.parametrize("cols", [1, 2, 9, 16, 17, 57, 61, 64, 120, 127, 250, 255, 377, 505, 640, 766, 785, 1015, 1016, 1024, 1400,
+                                  1530, 2041, 2044, 2046])
+def test_logprobs_of_thousands_of_rows(cols, kind, dtype):
+    rs = np.random.RandomState(cols)
+    t, z = _logits(37, cols, dtype, kind, cols)
+    tokens = rs.randint(0, cols, [37])
+    live = rs.rand(37) < 0.8
+    for top in sorted({0, min(cols, 5), min(cols, 64)}):
+        _check_many(t, z, 1.3, tokens, top, live, dtype, rs)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["ties", "rising", "constant", "lowest", "zeros"])
+@pytest.mark.parametrize("cols", [30, 785, 1500])
+def test_logprobs_of_thousands_of_odd_rows(cols, kind, dtype):
+    rs = np.random.RandomState(cols)
+    t, z = _logits(37, cols, dtype, kind, cols)
+    for top in (3, min(cols, 40)):
+        _check_many(t, z, 0.7, rs.randint(0, cols, [37]), top, np.ones([37], bool), dtype, rs)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols,k", [(1, 1), (2, 2), (9, 3), (17, 17), (61, 5), (64, 64), (120, 8), (250, 64), (505, 20), (785, 16),
+                                    (785, 64), (785, 65), (785, 300), (1016, 33), (1017, 4), (1500, 64), (2041, 64), (2045, 100),
+                                    (40, 300), (12, 20)])
+def test_distillation_of_thousands_of_rows(cols, k, dtype, tail):
+    decode = _decode()
+    rs = np.random.RandomState(cols + k)
+    t, z = _logits(37, cols, dtype, "peaked", cols)
+    values, classes = _teacher(z, min(k, cols), 1.3, tail, cols)
+    if k > cols:  # (more places than classes: absent ones)
+        values = np.concatenate([values, np.zeros([37, k - cols], np.float32)], axis=1)
+        classes = np.concatenate([classes, np.full([37, k - cols], -1, np.int32)], axis=1)
+    if k > 3:
+        classes[3, 1], classes[4, -1], classes[5, 2:] = classes[3, 0], -1, -1  # one twice, one absent, most absent
+        values[3] -= 1.0
+        classes[6, :] = -1
+    live = rs.rand(37) < 0.8
+    on = _many(live)
+    g = rs.randn(37).astype(np.float32)
+    big = t.repeat(113, 1).requires_grad_(True)
+    loss = decode.distill_rows(big, torch.tensor(_many(values), device=DEV), torch.tensor(_many(classes), device=DEV),
+                               temperature=1.3, tail=tail, live=torch.tensor(on, device=DEV))
+    want = ref.distill(z, values.astype(np.float64), classes, 1.3, tail, g.astype(np.float64), dtype)
+    got = _f64(loss)
+    ref.close(got[on], _many(want["loss"])[on], _many(want["loss_tol"])[on])
+    assert np.all(got[~on] == 0)
+    dz, = torch.autograd.grad(loss, big, torch.tensor(_many(g), device=DEV))
+    got = _f64(dz)
+    ref.close(got[on], _many(want["dlogits"])[on], _many(want["dlogits_tol"])[on])
+    assert np.all(got[~on] == 0)
+
+
 @pytest.mark.parametrize("T", [0.05, 0.7, 4.0, 1000.0])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_logprobs_over_temperatures(T, dtype):
@@ -199,7 +291,7 @@ def _teacher(z, k, T, tail, seed):
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,cols,k", [(1, 1, 1), (3, 2, 1), (2, 7, 7), (5, 8, 3), (4, 64, 64), (4, 65, 64), (6, 513, 20),
-                                         (33, 784, 5), (33, 785, 64), (2, 1025, 100), (3, 2047, 64), (3, 2048, 16),
+                                         (33, 784, 5), (33, 785, 64), (33, 785, 400), (2, 1025, 100), (3, 2047, 64), (3, 2048, 16),
                                          (3, 2049, 65), (2, 4097, 1024), (2, 8191, 3), (2, 8193, 64), (2, 16385, 20),
                                          (1, 50177, 64), (2, 131071, 32)])
 def test_distillation_over_sizes(rows, cols, k, dtype, tail):
