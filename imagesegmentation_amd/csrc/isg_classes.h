@@ -257,6 +257,18 @@ struct Span {
         const int s = start(t);
         if (s < hi && s + VE > lo) store_vector<VE>(d + inside(s), o);
     }
+    // the same without what they repeat (where a thread's values are its own alone)
+    __device__ __forceinline__ void store_own(T* d, int t, const T* o) const {
+        const int s = start(t);
+        if (s >= lo && s + VE <= hi) {
+            __builtin_memcpy(d + s, o, VE * sizeof(T));
+        } else if (s < hi && s + VE > lo) {
+            const int at = inside(s);
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                if (at + j >= s && at + j < s + VE) d[at + j] = o[j];
+        }
+    }
 };
 
 // a class index stored as 4 or 8 bytes

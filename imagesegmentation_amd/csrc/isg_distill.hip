@@ -57,8 +57,9 @@ __device__ __forceinline__ void distill_dead(const DistillArgs& a, long long row
     if (a.stats) a.stats[row] = DistillStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// A row's entries in the registers of its G threads: entry i * G + thread in place i < N.  (Four places; sixteen, for
-// every k there can be, where a wave closes a row of any length and for rows too short for a workgroup.)
+// A row's entries in the registers of its G threads: entry i * G + thread in place i < N.  (One place where
+// that holds a row's k, else four; sixteen, for every k there can be, where a wave closes a row of any length and for rows
+// too short for a workgroup.)
 template <int G, int N>
 struct Entries {
     int cls[N];    // -1: none, cols: a class the row does not have
@@ -220,7 +221,7 @@ __device__ __forceinline__ void mark_entries(const DistillArgs& a, const Entries
 }
 
 // A row in the registers of G lanes.
-template <typename T, int G, int NE, bool TAIL>
+template <typename T, int G, int NE, int PLACES, bool TAIL>
 __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restrict__ logits, DistillArgs a) {
     __shared__ u64 marks[TAIL ? kThreads : 1];  // a thread's elements that an entry names, one bit each
     const int lane = threadIdx.x & (G - 1);
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
     const T* z = logits + row * a.row_stride;
     using S = Span<T, G, NE>;
     const S span(z, 0, a.cols, lane);
-    constexpr int N = G == 64 && NE == 1 ? 16 : 4;
+    constexpr int N = G == 64 && NE == 1 ? 16 : PLACES;
     Entries<G, N> en;
     en.load(a.values, a.classes, a.class_bytes, row, a.k, a.cols);
     float v[NE], ze[N];
@@ -396,11 +397,12 @@ struct DistillBwdArgs {
     float c, c_lo, inv_t;
 };
 
-template <typename T, int G, int NE>
+template <typename T, int G, int NE, int PLACES>
 __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restrict__ logits, DistillBwdArgs a,
                                                               T* __restrict__ dlogits) {
     __shared__ u64 marks[kThreads];
     __shared__ unsigned repeated;
+    __shared__ __attribute__((aligned(16))) T image[G <= 64 ? kThreads * Span<T, G, NE>::VE : 1];
     const int tid = threadIdx.x & (G - 1);
     // (from the last unit back: what the forward pass read last is still in the last-level cache)
     const long long unit = a.units - 1 - (block_index() * (kThreads / G) + threadIdx.x / G);
@@ -414,89 +416,148 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     const DistillStats st = a.stats[row];
     const bool zero = st.is == 0.0f;  // a dead row, or no class has probability
     const T* z = logits + row * a.row_stride;
-    constexpr int N = G == 64 && NE == 1 ? 16 : 4;
+    constexpr int N = G == 64 && NE == 1 ? 16 : PLACES;
+    const float g = a.dloss[row] * a.inv_t, gc = g * st.coef * st.ib;
+    const bool plain = zero || st.coef != st.coef;  // (NaN: an entry the row does not have; the whole row is)
     Entries<G, N> en;
-    float v[NE], ze[N];
-    if (!zero) {
+    float v[NE], ze[N], own[N];
+    const auto fetch_entries = [&] {
         en.load(a.values, a.classes, a.class_bytes, row, a.k, a.cols);
-        span.template load<false>(z, v);
         en.gather(z, lo, hi, ze);
-    }
-    const float g = a.dloss[row] * a.inv_t;
-    const float gc = g * st.coef * st.ib;
-#pragma unroll
-    for (int t = 0; t < S::NV; ++t) {
-        if (span.beyond(t)) break;
-        float o[S::VE];
+    };
+    const auto dense = [&](int t, float(&o)[S::VE]) {
 #pragma unroll
         for (int j = 0; j < S::VE; ++j) {
             const float zi = v[t * S::VE + j];
             const float e = sizeof(T) == 4 ? power_exact(zi, st.mb, a.c, a.c_lo) : __builtin_amdgcn_exp2f((zi - st.mb) * a.c);
             o[j] = zero ? 0.0f : gc * e;
         }
-        span.store(d, t, o);
-    }
-    if (zero || st.coef != st.coef) return;  // (NaN: an entry the row does not have; the whole row is)
-    // the entries' classes once more, behind the dense part
-    u64* mine = marks + (threadIdx.x - tid);
-    mine[tid] = 0ull;
-    if (G > 64 && tid == 0) repeated = 0u;
-    together<G>();
-    bool twice = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i * G < a.k && en.cls[i] >= lo && en.cls[i] < hi) {
-            int thread, e;
-            span.locate(en.cls[i], thread, e);
-            twice |= (atomicOr(&mine[thread], 1ull << e) >> e & 1ull) != 0;
-        }
-    if constexpr (G <= 64) {
-        twice = group_any<G>(twice);
-    } else {
-        if (twice) repeated = 1u;
+    };
+    // the entries' own gradients
+    const auto own_gradients = [&] {
+        u64* mine = marks + (threadIdx.x - tid);
+        mine[tid] = 0ull;
+        if (G > 64 && tid == 0) repeated = 0u;
         together<G>();
-        twice = repeated != 0;
-    }
-    const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
+        bool twice = false;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c = en.cls[i];
-        if (i * G >= a.k || c < lo || c >= hi) continue;
-        float q = st.iv * power_exact(en.val[i], st.mv, cv, cv_lo);
-        if (twice) {  // (every place of the class writes the same sum)
-            q = 0.0f;
-            for (int o = 0; o < a.k; ++o)
-                if (class_at(a.classes, a.class_bytes, row * a.k + o) == c)
-                    q += st.iv * power_exact(a.values[row * a.k + o], st.mv, cv, cv_lo);
+        for (int i = 0; i < N; ++i)
+            if (i * G < a.k && en.cls[i] >= lo && en.cls[i] < hi) {
+                int thread, e;
+                span.locate(en.cls[i], thread, e);
+                twice |= (atomicOr(&mine[thread], 1ull << e) >> e & 1ull) != 0;
+            }
+        if constexpr (G <= 64) {
+            twice = group_any<G>(twice);
+        } else {
+            if (twice) repeated = 1u;
+            together<G>();
+            twice = repeated != 0;
         }
-        const float o = g * (st.total * (st.is * power_exact(ze[i], st.m, a.c, a.c_lo)) - q);
-        store_vector<1>(d + c, &o);
+        const float cv = a.tail ? kLog2e : a.c, cv_lo = a.tail ? kLog2eLo : a.c_lo;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = en.cls[i];
+            own[i] = 0.0f;
+            if (i * G >= a.k || c < lo || c >= hi) continue;
+            float q = st.iv * power_exact(en.val[i], st.mv, cv, cv_lo);
+            if (twice) {  // (every place of the class writes the same sum)
+                q = 0.0f;
+                for (int o = 0; o < a.k; ++o)
+                    if (class_at(a.classes, a.class_bytes, row * a.k + o) == c)
+                        q += st.iv * power_exact(a.values[row * a.k + o], st.mv, cv, cv_lo);
+            }
+            own[i] = g * (st.total * (st.is * power_exact(ze[i], st.m, a.c, a.c_lo)) - q);
+        }
+    };
+    if constexpr (G <= 64) {
+        // A slot's vectors go through LDS, where the entries' values take their places: stored one by one behind the row
+        // they cost a write of 64 bytes each (131,072 x 785 float with 64 entries: 230 us for 179; bf16 144 for 142).
+        if (!zero) {
+            fetch_entries();
+            span.template load<false>(z, v);
+            own_gradients();
+        }
+        int slot[N], place[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            slot[i] = -1, place[i] = 0;
+            if (i * G < a.k && !plain && en.cls[i] >= lo && en.cls[i] < hi) {
+                int thread, e;
+                span.locate(en.cls[i], thread, e);
+                slot[i] = e / S::VE, place[i] = (threadIdx.x - tid + thread) * S::VE + e % S::VE;
+            }
+        }
+        T* mine = image + threadIdx.x * S::VE;
+#pragma unroll
+        for (int t = 0; t < S::NV; ++t) {
+            if (span.beyond(t)) break;
+            float o[S::VE];
+            dense(t, o);
+            store_vector<S::VE>(mine, o);
+            together<G>();
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (slot[i] == t) store_vector<1>(image + place[i], own + i);
+            together<G>();
+            T out[S::VE];
+            __builtin_memcpy(out, mine, S::VE * sizeof(T));
+            span.store_own(d, t, out);
+        }
+    } else {
+        // (A row in parts: the entries' work waits until the dense part has been stored, for more waves and an earlier
+        // start of the stores.  Before it: 204 us for 188 at 2,048 x 131,071 bf16 in 17 parts, 134 for 141 at 8,192 x
+        // 12,545 float in 2.)
+        if (!zero) {
+            fetch_entries();
+            span.template load<false>(z, v);
+        }
+#pragma unroll
+        for (int t = 0; t < S::NV; ++t) {
+            if (span.beyond(t)) break;
+            float o[S::VE];
+            dense(t, o);
+            span.store(d, t, o);
+        }
+        if (plain) return;
+        own_gradients();  // (with the barrier between the dense stores and the entries')
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i * G < a.k && en.cls[i] >= lo && en.cls[i] < hi) store_vector<1>(d + en.cls[i], own + i);
     }
 }
 
-template <typename T, bool TAIL>
+template <typename T, bool TAIL, int PLACES>
 struct DistillFwd {
     template <int G, int NE>
     static void run(const void* logits, const DistillArgs& a, hipStream_t s) {
-        hipLaunchKernelGGL((distill_fwd_kernel<T, G, NE, TAIL>), grid_of(a.units, G), dim3(kThreads), 0, s,
+        hipLaunchKernelGGL((distill_fwd_kernel<T, G, NE, PLACES, TAIL>), grid_of(a.units, G), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a);
     }
-    static void launch(const Cut& cut, const void* logits, const DistillArgs& a, hipStream_t s) {
-        if (cut.lanes != kThreads)
-            with_wave<DistillFwd>(cut, logits, a, s);
-        else
-            hipLaunchKernelGGL((distill_stream_kernel<T, 16, TAIL>), grid_of(a.units, kThreads), dim3(kThreads), 0, s,
-                               static_cast<const T*>(logits), a);
-    }
 };
-template <typename T>
+template <typename T, bool TAIL>
+void launch_forward(const Cut& cut, const void* logits, const DistillArgs& a, hipStream_t s) {
+    if (cut.lanes == kThreads)
+        hipLaunchKernelGGL((distill_stream_kernel<T, 16, TAIL>), grid_of(a.units, kThreads), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits), a);
+    else if (a.k <= cut.lanes)
+        with_wave<DistillFwd<T, TAIL, 1>>(cut, logits, a, s);
+    else
+        with_wave<DistillFwd<T, TAIL, 4>>(cut, logits, a, s);
+}
+template <typename T, int PLACES>
 struct DistillBwd {
     template <int G, int NE>
     static void run(const void* logits, const DistillBwdArgs& a, void* dlogits, hipStream_t s) {
-        hipLaunchKernelGGL((distill_bwd_kernel<T, G, NE>), grid_of(a.units, G), dim3(kThreads), 0, s,
+        hipLaunchKernelGGL((distill_bwd_kernel<T, G, NE, PLACES>), grid_of(a.units, G), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a, static_cast<T*>(dlogits));
     }
 };
+template <typename T>
+void launch_gradient(const Cut& cut, const void* logits, const DistillBwdArgs& a, void* dlogits, hipStream_t s) {
+    if (a.k <= cut.lanes) launch_backward<DistillBwd<T, 1>>(cut, logits, a, dlogits, s);
+    else launch_backward<DistillBwd<T, 4>>(cut, logits, a, dlogits, s);
+}
 
 int check_entries(const char* who, int k, int tail) {
     ISG_REQUIRE(k >= 1 && k <= kMaxEntries, ISG_EINVAL, "%s: k=%d classes of the teacher (1 to %d)", who, k, kMaxEntries);
@@ -535,10 +596,10 @@ extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const f
     scale_of(temperature, a.c, a.c_lo, a.inv_t);
     a.c_near = (float)(1.4426950408889634074 / (double)temperature);
     if (dtype == ISG_F32)
-        tail ? DistillFwd<float, true>::launch(cut, logits, a, s) : DistillFwd<float, false>::launch(cut, logits, a, s);
+        tail ? launch_forward<float, true>(cut, logits, a, s) : launch_forward<float, false>(cut, logits, a, s);
     else
-        tail ? DistillFwd<__hip_bfloat16, true>::launch(cut, logits, a, s)
-             : DistillFwd<__hip_bfloat16, false>::launch(cut, logits, a, s);
+        tail ? launch_forward<__hip_bfloat16, true>(cut, logits, a, s)
+             : launch_forward<__hip_bfloat16, false>(cut, logits, a, s);
     rc = isg::check_launch("distill_fwd_kernel");
     if (rc != ISG_OK || cut.splits == 1) return rc;
     a.units = rows;
@@ -571,7 +632,7 @@ extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const f
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
     a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.k = k, a.tail = tail;
     scale_of(temperature, a.c, a.c_lo, a.inv_t);
-    if (dtype == ISG_F32) launch_backward<DistillBwd<float>>(cut, logits, a, dlogits, s);
-    else launch_backward<DistillBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
+    if (dtype == ISG_F32) launch_gradient<float>(cut, logits, a, dlogits, s);
+    else launch_gradient<__hip_bfloat16>(cut, logits, a, dlogits, s);
     return isg::check_launch("distill_bwd_kernel");
 }

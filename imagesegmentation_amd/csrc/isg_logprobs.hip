@@ -44,10 +44,10 @@ __device__ __forceinline__ unsigned reach_mask(const float (&v)[NE], float low) 
 }
 
 // The k first of the list (n keys), through emit(place, key); the G threads of the unit share the work.
-template <int G, typename Emit>
-__device__ __forceinline__ void rank_keys(const u64* keys, int n, int k, Emit emit) {
+template <int G, typename Key, typename Emit>
+__device__ __forceinline__ void rank_keys(const Key* keys, int n, int k, Emit emit) {
     for (int r = threadIdx.x & (G - 1); r < n; r += G) {
-        const u64 own = keys[r];
+        const Key own = keys[r];
         int place = 0;
 #pragma unroll 4
         for (int o = 0; o < n; ++o) place += keys[o] > own ? 1 : 0;
@@ -55,7 +55,8 @@ __device__ __forceinline__ void rank_keys(const u64* keys, int n, int k, Emit em
     }
 }
 
-// Lanes of one wave.  Q groups a lane.
+// Lanes of one wave.  Q groups a lane.  (Bisecting between the least and the largest group instead, nine steps for
+// sixteen, measured slower: 131,072 x 785 bf16 with five classes 78 us against 69.)
 template <int G, int Q>
 __device__ __forceinline__ unsigned lanes_bound(const float (&gm)[Q], int k) {
     unsigned g[Q], bound = 0;
@@ -88,8 +89,24 @@ __device__ __forceinline__ void group_maxima(const float (&v)[NE], float (&gm)[Q
 
 constexpr int candidates(int lanes) { return lanes == 16 ? 128 : 256; }  // places per unit
 
-template <int G, int NE, typename Reload, typename Emit>
-__device__ __forceinline__ void select_lanes(const float (&v)[NE], int k, u64* cand, Reload reload, Emit emit) {
+// The order of a row's classes in 32 bits where a logit has 16 (bf16) and a class 16: halves what ranking costs.
+struct ShortKey {
+    typedef unsigned type;
+    static __device__ __forceinline__ unsigned of(u64 k) { return (unsigned)(k >> 32 & 0xffff0000u) | ((unsigned)k & 0xffffu); }
+    static __device__ __forceinline__ u64 full(unsigned k) {
+        // (the lower half of a logit's key: zeros, or ones below 0, whose bits are inverted; NaN is 1)
+        const u64 bits = k >> 31 ? k & 0xffff0000u : (k >> 16 ? k | 0xffffu : 1u);
+        return bits << 32 | 0xffff0000u | (k & 0xffffu);
+    }
+};
+struct LongKey {
+    typedef u64 type;
+    static __device__ __forceinline__ u64 of(u64 k) { return k; }
+    static __device__ __forceinline__ u64 full(u64 k) { return k; }
+};
+
+template <int G, int NE, typename Keys, typename Reload, typename Emit>
+__device__ __forceinline__ void select_lanes(const float (&v)[NE], int k, typename Keys::type* cand, Reload reload, Emit emit) {
     constexpr int Q1 = 64 / G < NE ? 64 / G : NE, Q2 = 128 / G < NE ? 128 / G : NE, kCap = candidates(G);
     const int lane = threadIdx.x & (G - 1);
     float gm[Q2];
@@ -116,10 +133,10 @@ __device__ __forceinline__ void select_lanes(const float (&v)[NE], int k, u64* c
                 if (hit == 0) hit = later, later = 0, add = 32;
                 const int e = __builtin_ctz(hit);
                 hit &= hit - 1;
-                cand[at++] = reload(e + add);
+                cand[at++] = Keys::of(reload(e + add));
             }
             together<G>();
-            rank_keys<G>(cand, total, k, emit);
+            rank_keys<G>(cand, total, k, [&](int place, typename Keys::type key) { emit(place, Keys::full(key)); });
         }
     }
     if (total > kCap) {
@@ -306,7 +323,8 @@ __device__ __forceinline__ void row_alternative(const LogprobsArgs& a, long long
 // A row in the registers of G lanes.
 template <typename T, int G, int NE, bool TOP>
 __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restrict__ logits, LogprobsArgs a) {
-    __shared__ u64 cand[TOP ? kThreads / G * candidates(G) : 1];
+    typedef typename std::conditional<sizeof(T) == 2, ShortKey, LongKey>::type Keys;
+    __shared__ typename Keys::type cand[TOP ? kThreads / G * candidates(G) : 1];
     const int lane = threadIdx.x & (G - 1), unit = threadIdx.x / G;
     const long long row = block_index() * (kThreads / G) + unit;
     if (row >= a.units) return;
@@ -329,7 +347,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restr
     const RowStats r = row_stats(t, a.c_rel);
     if (lane == 0) row_outputs(a, z, row, r);
     if constexpr (TOP)
-        select_lanes<G, NE>(
+        select_lanes<G, NE, Keys>(
             v, a.top, cand + unit * candidates(G),
             [&](int e) {
                 const int i = span.cls(e);
@@ -547,7 +565,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __rest
     };
     const auto emit = [&](int place, u64 key) { row_alternative(a, row, r, place, key); };
     if constexpr (G == 64)
-        select_lanes<G, NE>(v, a.top, shared + (threadIdx.x / G) * candidates(G), reload, emit);
+        select_lanes<G, NE, LongKey>(v, a.top, shared + (threadIdx.x / G) * candidates(G), reload, emit);
     else
         select_workgroup<NE>(v, a.top, shared, reload, emit);
 }
