@@ -700,6 +700,24 @@ class Model:
             metrics = dict(loss=loss.detach(), accuracy=m[0] / m[3], avg_error=m[1] / m[3], max_error=m[2])
         return loss, metrics
 
+    def _live_steps(self, durations, batch):
+        """bool [batch, max_timesteps] on the device: the steps within each sample's duration."""
+        dur = self._to_dev(durations, torch.int32).reshape(batch, 1)
+        return torch.arange(self.max_timesteps, dtype=torch.int32, device=self.device) < dur
+
+    def score(self, images, durations, histories, targets=None, top=0, temperature=1.0):
+        """What the model thinks of given vertices: log-probability of each (x, y) of ``targets`` [B,T,2] (None: none),
+        entropy of each step's distribution over the grid and its ``top`` most probable classes, under
+        softmax(logits / temperature); ``decode.TokenLogprobs`` of [B,T(,top)] tensors on the device, zeros (class -1)
+        past a sample's duration.  With ``top`` it is also what ``distill`` takes as a teacher."""
+        with torch.no_grad(), self._derived:
+            logits, _ = self.forward(images, durations, histories)
+            tokens = None
+            if targets is not None:
+                xy = self._to_dev(targets, torch.int32)
+                tokens = xy[..., 0] * self.head_size + xy[..., 1]  # x-major (reference polyrnn/Model.py:39)
+            return decode.token_logprobs(logits, tokens, top, temperature, self._live_steps(durations, logits.shape[0]))
+
     # -- optimiser (reference Model.py:106-112) --------------------------------------------------
     def _apply_gradients(self, clip=True, all_reduce=True, average=True):
         """All-reduce of the flat gradient bucket across ranks (one RCCL collective), global-norm
@@ -727,8 +745,9 @@ class Model:
     #: overlaps the head's share of the gradient exchange with the backward pass, the graph step exchanges after it.
     step_graphs = False
 
-    def _step_body(self, images, durations, histories, targets, steps=None, arm=False):
-        """Zero fill, forward, loss, metrics, backward: everything of a step up to the gradient exchange."""
+    def _step_body(self, images, durations, histories, targets, steps=None, arm=False, soft=None):
+        """Zero fill, forward, loss, metrics, backward: everything of a step up to the gradient exchange.  ``soft``:
+        (teacher's ``TokenLogprobs``, temperature, weight) of a ``distill`` step."""
         # Every parameter is used once per step, so the hand-written backward passes ASSIGN their gradients into
         # the flat bucket (ops.grad_sinks) - the dense head's 9.8 M elements included; the zero fill is for what
         # autograd still accumulates itself (layers on library kernels), i.e. everything but the head's share.
@@ -736,6 +755,13 @@ class Model:
         with self._derived, ops.grad_sinks(self._sinks, self._on_gradient_delivered) as sinks:
             logits, _ = self.forward(images, durations, histories, steps=steps)
             loss, metrics = self._loss_and_metrics(logits, durations, targets)
+            if soft is not None:
+                teacher, temperature, weight = soft
+                # (over all B * T rows as the labels' term is, so that the mean over ranks is the mean over the batch)
+                apart = decode.distill_rows(logits, teacher.top_logprobs, teacher.top_classes, temperature, True,
+                                            self._live_steps(durations, logits.shape[0])).mean()
+                loss = (1.0 - weight) * loss + (weight * temperature ** 2) * apart
+                metrics = dict(metrics, loss=loss.detach(), distill=apart.detach())
             if arm:
                 self._early_reduce.arm()
             if self._grad_one is None:
@@ -810,7 +836,9 @@ class Model:
         done = self._graphed_step(images, durations, histories, targets) if self.step_graphs else None
         if done is None:
             done = self._step_body(images, durations, histories, targets, arm=True)
-        loss, metrics = done
+        return self._finish_step(*done)
+
+    def _finish_step(self, loss, metrics):
         self._apply_gradients()
         if isinstance(self._derived, ops.DerivedWeights):
             self._derived.compile()  # (what this step packed for the first time joins the one refresh launch)
@@ -821,6 +849,26 @@ class Model:
     # -- reference surface -----------------------------------------------------------------------
     def train(self, images, durations, histories, targets, additional_feed_args={}):
         self.train_step(images, durations, histories, targets)
+        self._add_summaries('train')
+
+    def distill(self, images, durations, histories, targets, teacher, top=16, temperature=2.0, weight=0.5,
+                additional_feed_args={}):
+        """A training step towards a teacher: loss = (1 - weight) * cross-entropy + weight * temperature^2 * divergence
+        from the teacher's ``top`` most probable classes and the mass they leave, at this temperature, over the steps
+        within each duration (``decode.distill_rows``).  ``teacher``: another model of the same grid and number of steps,
+        or what its ``score(..., top=, temperature=)`` gave for this batch earlier (at the same temperature)."""
+        temperature, weight = float(temperature), float(weight)
+        if not 0.0 <= weight <= 1.0:
+            raise ValueError("distill: weight %g (0 to 1)" % weight)
+        if isinstance(teacher, Model):
+            if (teacher.num_classes, teacher.max_timesteps) != (self.num_classes, self.max_timesteps):
+                raise ValueError("distill: a teacher of %d classes and %d steps for a student of %d and %d" % (
+                    teacher.num_classes, teacher.max_timesteps, self.num_classes, self.max_timesteps))
+            teacher = teacher.score(images, durations, histories, None, top, temperature)
+        if not isinstance(teacher, decode.TokenLogprobs) or teacher.top_logprobs is None:
+            raise TypeError("distill: teacher must be a Model or what its score(..., top=) returned")
+        self._finish_step(*self._step_body(images, durations, histories, targets, arm=True,
+                                           soft=(teacher, temperature, weight)))
         self._add_summaries('train')
 
     def validate(self, images, durations, histories, targets, additional_feed_args={}):

@@ -1,0 +1,129 @@
+"""A model's scores and its distillation step: what ``Model.score`` and ``Model.distill`` hand to token_logprobs and
+distill_rows, against float64 references over the model's own logits."""
+import numpy as np
+import pytest
+
+import helpers_logprobs as ref
+from helpers_convlstm import make_batch
+
+torch = pytest.importorskip("torch")
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _model(name, dtype, seed=0, device="cuda:0"):
+    from imagesegmentation_amd.polyrnn import experiments
+    return experiments.make(name, image_size=28, compute_dtype=DT[dtype], device=device, seed=seed)
+
+
+def _batch(model, B=3, seed=5):
+    images, histories, durations, targets = make_batch(np.random.RandomState(seed), B, model.max_timesteps, 28,
+                                                       model.history_length, end_token=model.end_token)
+    durations[1] = min(durations[1], 2)
+    return images, durations, histories, targets
+
+
+def _rows(model):
+    z = model.prediction_logits.detach().double().cpu().numpy()
+    return z.reshape(-1, z.shape[-1])
+
+
+def _tokens(model, targets):
+    t = np.asarray(targets).astype(np.int64)
+    return (t[..., 0] * model.head_size + t[..., 1]).reshape(-1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,dtype", [("History0", "f32"), ("EndToken", "bf16")])
+def test_score_of_a_batch(name, dtype):
+    model = _model(name, dtype)
+    images, durations, histories, targets = _batch(model)
+    got = model.score(images, durations, histories, targets, top=5, temperature=1.5)
+    B, T = 3, model.max_timesteps
+    assert got.logprobs.shape == (B, T) and got.top_classes.shape == (B, T, 5)
+    live = (np.arange(T)[None] < np.asarray(durations).reshape(-1, 1)).reshape(-1)
+    assert 0 < live.sum() < B * T
+    z = _rows(model)
+    want = ref.token_logprobs(z, 1.5, _tokens(model, targets), 5)
+    flat = lambda t: t.double().cpu().numpy().reshape((B * T,) + tuple(t.shape[2:]))
+    lp, ent = flat(got.logprobs), flat(got.entropy)
+    ref.close(lp[live], want["logprobs"][live], want["logprobs_tol"][live])
+    ref.close(ent[live], want["entropy"][live], want["entropy_tol"][live])
+    assert (flat(got.top_classes)[live] == want["top_classes"][live]).all()
+    assert (lp[~live] == 0).all() and (ent[~live] == 0).all() and (flat(got.top_classes)[~live] == -1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,dtype", [("History0", "f32"), ("EndToken", "f32"), ("History2Large", "bf16")])
+def test_distillation_step_gradient(name, dtype):
+    """The head's bias gradient is the column sum of the logits' gradient."""
+    teacher, model = _model(name, dtype, seed=1), _model(name, dtype, seed=2)
+    images, durations, histories, targets = _batch(model)
+    T_, w, k = 2.0, 0.25, 16
+    soft = teacher.score(images, durations, histories, top=k, temperature=T_)
+    loss, metrics = model._step_body(images, durations, histories, targets, soft=(soft, T_, w))
+    z = _rows(model)
+    rows, n = z.shape
+    live = (np.arange(model.max_timesteps)[None] < np.asarray(durations).reshape(-1, 1)).reshape(-1)
+    values = soft.top_logprobs.double().cpu().numpy().reshape(rows, k)
+    classes = soft.top_classes.cpu().numpy().reshape(rows, k)
+    g = np.full([rows], w * T_ ** 2 / rows)
+    d = ref.distill(z, values, classes, T_, True, g, dtype)
+    d["dlogits"][~live], d["dlogits_tol"][~live], d["loss"][~live], d["loss_tol"][~live] = 0, 0, 0, 0
+    logp, p, _ = ref.softmax(z, 1.0)
+    tokens = _tokens(model, targets)
+    hard = p.copy()
+    hard[np.arange(rows), tokens] -= 1
+    hard *= (1 - w) / rows
+    # the label term: p to the rounding of its sum and exponent, the difference and its scale a rounding each, then its type
+    hard_tol = (1 - w) / rows * p * (ref.kappa(z, 1.0, p)[:, None] + 4 * ref.U * np.abs(logp) + 16 * ref.U) + \
+        (4 * ref.U + ref.HALF_STEP[dtype]) * np.abs(hard)
+    both = np.abs(hard) + np.abs(d["dlogits"])
+    # (the two terms are added in the logits' type, the rows in 32 bits)
+    tol = (hard_tol + d["dlogits_tol"] + (ref.HALF_STEP[dtype] + rows * ref.U) * both).sum(axis=0)
+    ref.close(model.dense_bias.grad.double().cpu().numpy(), (hard + d["dlogits"]).sum(axis=0), tol)
+    apart = d["loss"].mean()
+    assert abs(float(metrics["distill"]) - apart) <= d["loss_tol"].mean() + rows * ref.U * np.abs(d["loss"]).mean()
+    want = (1 - w) * -logp[np.arange(rows), tokens].mean() + w * T_ ** 2 * apart
+    slack = (1 - w) * (ref.kappa(z, 1.0, p) + 16 * ref.U * (1 + np.abs(z).max())).mean() + w * T_ ** 2 * d["loss_tol"].mean()
+    assert abs(float(loss) - want) <= slack + rows * ref.U * want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,dtype", [("History0", "f32"), ("EndToken", "bf16")])
+def test_a_model_learns_from_another(name, dtype):
+    """A teacher that scores by itself and one that scored earlier give the same step; padded steps count for nothing;
+    one weight leaves the labels out, the other the teacher."""
+    teacher = _model(name, dtype, seed=1)
+    first, second = _model(name, dtype, seed=2), _model(name, dtype, seed=2)
+    images, durations, histories, targets = _batch(first)
+    soft = teacher.score(images, durations, histories, top=8, temperature=2.0)
+    before = first._flat_param.clone()
+    first.distill(images, durations, histories, targets, teacher, top=8, temperature=2.0, weight=1.0)
+    second.distill(images, durations, histories, targets, soft, temperature=2.0, weight=1.0)
+    assert float(first.loss) == pytest.approx(float(second.loss), rel=1e-5)
+    assert float(first.loss) == pytest.approx(4.0 * float(first.last_metrics["distill"]), rel=1e-6)
+    assert first.global_step == 1 and torch.isfinite(first._flat_param).all() and (first._flat_param != before).any()
+    third, fourth = _model(name, dtype, seed=2), _model(name, dtype, seed=2)
+    third.distill(images, durations, histories, targets, soft, temperature=2.0, weight=0.0)
+    fourth.train(images, durations, histories, targets)
+    assert float(third.loss) == pytest.approx(float(fourth.loss), rel=1e-5)
+    # A student that is its own teacher is no distance away: the sums of its classes' rounding; in bf16 the scoring and
+    # the training pass may round a logit each in its own way, two half steps apart, and distributions whose logits are
+    # within d of each other diverge by d^2 / 2 at most.
+    own = fourth.score(images, durations, histories, top=64, temperature=2.0)
+    fourth.distill(images, durations, histories, targets, own, temperature=2.0, weight=1.0)
+    d = 2 * ref.HALF_STEP[dtype] * float(fourth.prediction_logits.detach().abs().max()) / 2.0
+    assert abs(float(fourth.last_metrics["distill"])) < fourth.num_classes * 2 * ref.U + d * d / 2
+
+
+def test_distillation_refuses_teachers_that_do_not_fit():
+    model = _model("History0", "f32", device="cpu")
+    args = (None, None, None, None)
+    with pytest.raises(ValueError, match="classes"):
+        model.distill(*args, _model("EndToken", "f32", device="cpu"))
+    with pytest.raises(ValueError, match="weight"):
+        model.distill(*args, model, weight=1.5)
+    with pytest.raises(ValueError, match="weight"):
+        model.distill(*args, model, weight=float("nan"))
+    with pytest.raises(TypeError, match="teacher"):
+        model.distill(*args, None)
