@@ -395,6 +395,7 @@ struct DistillBwdArgs {
     long long row_stride, units;
     int class_bytes, cols, splits, per, k, tail;
     float c, c_lo, inv_t;
+    int past;
 };
 
 template <typename T, int G, int NE, int PLACES>
@@ -517,7 +518,8 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
             if (span.beyond(t)) break;
             float o[S::VE];
             dense(t, o);
-            span.store(d, t, o);
+            if (a.past) span.store_past(d, t, o);
+            else span.store(d, t, o);
         }
         if (plain) return;
         own_gradients();  // (with the barrier between the dense stores and the entries')
@@ -631,6 +633,7 @@ extern "C" int isg_distill_bwd(const void* logits, long long row_stride, const f
     a.values = values, a.classes = classes, a.stats = reinterpret_cast<const DistillStats*>(stats), a.dloss = dloss;
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
     a.class_bytes = class_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.k = k, a.tail = tail;
+    a.past = beyond_cache(rows, cols, dtype);
     scale_of(temperature, a.c, a.c_lo, a.inv_t);
     if (dtype == ISG_F32) launch_gradient<float>(cut, logits, a, dlogits, s);
     else launch_gradient<__hip_bfloat16>(cut, logits, a, dlogits, s);

@@ -580,7 +580,7 @@ struct LogprobsBwdArgs {
     const float* dentropy;
     const float* dtop;
     long long row_stride, units;
-    int token_bytes, cols, splits, per, top;
+    int token_bytes, cols, splits, per, top, past;
     float c, c_lo, inv_t;
 };
 
@@ -631,6 +631,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restr
         float o[S::VE];
 #pragma unroll
         for (int j = 0; j < S::VE; ++j) o[j] = zero ? 0.0f : dense(v[t * S::VE + j]);
+        if constexpr (G > 64) {
+            if (a.past) {
+                span.store_past(d, t, o);
+                continue;
+            }
+        }
         span.store(d, t, o);
     }
     if (zero) return;
@@ -767,6 +773,7 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
     a.dlogprobs = dlogprobs, a.dentropy = dentropy, a.dtop = dtop_logprobs;
     a.row_stride = row_stride, a.units = (long long)rows * cut.splits;
     a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.top = top;
+    a.past = beyond_cache(rows, cols, dtype);
     scale_of(temperature, a.c, a.c_lo, a.inv_t);
     if (dtype == ISG_F32) launch_backward<LogprobsBwd<float>>(cut, logits, a, dlogits, s);
     else launch_backward<LogprobsBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);

@@ -628,3 +628,37 @@ def test_rows_past_two_to_the_thirty_one_elements():
     ref.close(_f64(loss[-2:]), want["loss"], want["loss_tol"])
     ref.close(_f64(g[-2:]), want["dlogits"], want["dlogits_tol"])
     assert not loss[:-2].any() and not g[:-2].any()
+
+
+@pytest.mark.parametrize("dtype,rows,cols", [("bf16", 1100, 131071), ("f32", 5500, 12545)])
+def test_gradients_larger_than_the_last_level_cache(dtype, rows, cols):
+    """They are written past it: the same values as from two calls over half the rows, which are not.  (Given the rows'
+    statistics: the forward pass cuts fewer rows into more parts, whose sums round in another order.)"""
+    from imagesegmentation_amd import _lib
+    decode, lib = _decode(), _lib.lib()
+    es, code = (2, 1) if dtype == "bf16" else (4, 0)
+    assert rows * cols * es > 256 << 20 > rows * cols * es / 2
+    g = torch.Generator(device=DEV).manual_seed(1)
+    z = torch.randn([rows, cols], generator=g, device=DEV, dtype=torch.float32).mul_(3).to(DT[dtype])
+    tokens = torch.randint(cols, [rows], generator=g, device=DEV)
+    up = torch.randn([rows], generator=g, device=DEV)
+    classes = torch.randint(cols, [rows, 8], generator=g, device=DEV)
+    values = torch.randn([rows, 8], generator=g, device=DEV)
+    whole = z.clone().requires_grad_(True)
+    out = decode.token_logprobs(whole, tokens)
+    dz, = torch.autograd.grad([out.logprobs, out.entropy], whole, [up, up.flip(0)])
+    dd, = torch.autograd.grad(decode.distill_rows(whole, values, classes, temperature=2.0), whole, up)
+    stats = decode._logprobs_forward(z, (rows, cols, cols), tokens, None, 0, 1.0, True)[4]
+    apart = decode._distill_forward(z, (rows, cols, cols), values, classes, None, 2.0, 0, True)[1]
+    h, want, flipped = rows // 2, torch.empty_like(z), up.flip(0).contiguous()
+    for r in (0, h):
+        s = torch.cuda.current_stream().cuda_stream
+        _lib.check(lib.isg_token_logprobs_bwd(z[r:].data_ptr(), cols, tokens[r:].data_ptr(), 8, None, stats[r:].data_ptr(),
+                                              up[r:].data_ptr(), flipped[r:].data_ptr(), None, h, cols, code, 1.0, 0,
+                                              want[r:].data_ptr(), s), "isg_token_logprobs_bwd")
+    assert torch.equal(dz, want)
+    for r in (0, h):
+        _lib.check(lib.isg_distill_bwd(z[r:].data_ptr(), cols, values[r:].data_ptr(), classes[r:].data_ptr(), 8,
+                                       apart[r:].data_ptr(), up[r:].data_ptr(), h, cols, 8, code, 2.0, 0,
+                                       want[r:].data_ptr(), s), "isg_distill_bwd")
+    assert torch.equal(dd, want)
