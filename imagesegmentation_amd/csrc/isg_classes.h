@@ -323,10 +323,14 @@ __device__ __forceinline__ long long block_index() { return (long long)blockIdx.
 
 // ---- launches ------------------------------------------------------------------------------------------------------
 // How a row is cut: `lanes` lanes of a wave for what their registers hold.  Beyond, the forward passes walk over parts of
-// a row, as many as give kUnits workgroups but of at least kPartCols classes; the backward passes have nothing to join
-// and take workgroups of at most 32 classes a thread.  Parts are equal but for the rounding to 8 classes; there is room
-// for those that start between two boundaries (Span).
-constexpr long long kUnits = 4096;
+// a row, as many as give about `units_of` workgroups but of at least kPartCols classes; the backward passes have nothing
+// to join and take workgroups of at most 32 classes a thread.  Parts are equal but for the rounding to 8 classes; there is
+// room for those that start between two boundaries (Span).
+//
+// bf16: 2,048 workgroups are on the chip all at once, eight to a CU (64 registers a thread); 2,048 x 131,071 with 64
+// alternatives 139 us so, in 4,096 workgroups (two parts a row) 155 and 9 more to join them.  Float kernels need more
+// registers, five to seven to a CU: 2,048 x 65,537 with 20 alternatives 120 us in 2,048, 105 + 6 in 4,096.
+inline long long units_of(int dtype) { return dtype == ISG_F32 ? 4096 : 2048; }
 constexpr int kPartCols = 2048;
 constexpr int kMaxSplits = 128;
 constexpr int kMarkCols = 131072;  // classes a part may have (one mark each in LDS, 16 KB)
@@ -352,7 +356,7 @@ inline Cut cut_wave(long long rows, int cols, int dtype, int entries) {
 inline Cut cut_forward(long long rows, int cols, int dtype, int entries = 0) {
     const Cut wave = cut_wave(rows, cols, dtype, entries);
     if (wave.lanes) return wave;
-    long long splits = (kUnits + rows - 1) / (rows > 0 ? rows : 1);
+    long long splits = (units_of(dtype) + rows - 1) / (rows > 0 ? rows : 1);
     const int most = cols / kPartCols < kMaxSplits ? cols / kPartCols : kMaxSplits, least = (cols + kMarkCols - 1) / kMarkCols;
     splits = splits > most ? most : splits;
     splits = splits < least ? least : splits;

@@ -280,7 +280,8 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, const T* z, lon
 // meanwhile.  Every wave keeps its own maximum and its lanes their own sums until the end.  The marks are one bit a class
 // of the part.
 template <typename T, int NE, bool TAIL>
-__global__ __launch_bounds__(kThreads) void distill_stream_kernel(const T* __restrict__ logits, DistillArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 7 : 8) void distill_stream_kernel(const T* __restrict__ logits,
+                                                                                           DistillArgs a) {
     __shared__ DistillPart red[4];
     __shared__ unsigned char marks[TAIL ? kMarkCols / 8 + 16 : 16] __attribute__((aligned(16)));
     __shared__ unsigned repeated;
@@ -571,7 +572,7 @@ int check_entries(const char* who, int k, int tail) {
 
 extern "C" long long isg_distill_workspace_bytes(int rows, int cols) {
     if (rows < 0 || cols < 1 || cols > kMaxCols) return -1;
-    const Cut cut = cut_forward(rows, cols, ISG_BF16);  // (the same for float: types differ in rows of one part)
+    const Cut cut = cut_forward(rows, cols, ISG_F32);  // (bf16 rows are in as many parts or fewer)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * (long long)sizeof(DistillPart);
 }
 

@@ -414,7 +414,8 @@ __device__ __forceinline__ int trim_list(TopList& list, int count, int k, float&
 // the list's own bound, which rises whenever the list has grown to kListTrim and is cut back.  Steps that would overrun
 // the list (rising rows, ties) or have no finite bound hand it their k first by select_workgroup instead.
 template <typename T, int NE, bool TOP>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 6) void logprobs_stream_kernel(const T* __restrict__ logits, LogprobsArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 8) void logprobs_stream_kernel(const T* __restrict__ logits,
+                                                                                            LogprobsArgs a) {
     __shared__ float red[4][4];
     __shared__ typename std::conditional<TOP, TopShared, char>::type shared;
     __shared__ typename std::conditional<TOP, TopList, char>::type list;
@@ -703,7 +704,7 @@ int check_top(const char* who, int top, int cols) {
 
 extern "C" long long isg_token_logprobs_workspace_bytes(int rows, int cols, int top) {
     if (rows < 0 || cols < 1 || cols > kMaxCols || top < 0 || top > kMaxTop) return -1;
-    const Cut cut = cut_forward(rows, cols, ISG_BF16);  // (the same for float: types differ in rows of one part)
+    const Cut cut = cut_forward(rows, cols, ISG_F32);  // (bf16 rows are in as many parts or fewer)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * ((long long)sizeof(Sums) + 8 * top) + 8;
 }
 
