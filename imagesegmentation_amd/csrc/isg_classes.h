@@ -337,7 +337,11 @@ constexpr int kMarkCols = 131072;  // classes a part may have (one mark each in 
 struct Cut {
     int lanes, ne, splits, per;  // lanes = kThreads: workgroups
 };
-inline int equal_part(int cols, int splits) { return ((cols + splits - 1) / splits + 7) / 8 * 8; }
+// (The rounding must not use up the last part, where the others are hundreds: a vector has to fit into it.)
+inline int equal_part(int cols, int splits) {
+    const int even = (cols + splits - 1) / splits, per = (even + 7) / 8 * 8, last = (cols - 1) % per + 1;
+    return splits > 1 && last < 64 ? even : per;
+}
 // lanes = 0: too long for a wave's registers.  16 lanes a row (32 for the longer) where there are rows enough for every
 // SIMD to have waves, else a whole wave: 16 rows of 785 classes take 4.6 us so and 6.8 us in 16 lanes each, 131,072 rows
 // 64 and 47 us.  `entries`: places a row needs in its threads' registers, four a thread (sixteen in rows of 64 classes).
@@ -375,10 +379,10 @@ inline Cut cut_backward(long long rows, int cols, int dtype, int entries = 0) {
 }
 
 // Whether a gradient is more than the last-level cache holds (256 MB).  What reads it next does not find it there either,
-// and left in the cache it has to be written back under the next kernel's reads: 2,048 x 131,071 bf16 distilled, forward
-// and backward 118 + 185 us, written past the cache 95 + 191; 8,192 x 12,545 float 105 + 140 and 77 + 157.  (Long rows
-// only: of short ones, whose vectors are 256 bytes of a row, a float gradient is slower so by more than that, 131,072 x 785
-// 103 + 150 and 73 + 190.)
+// and left in the cache it has to be written back under the next kernel's reads: 2,048 x 131,071 bf16 distilled (two parts
+// a row), forward and backward 118 + 185 us, written past the cache 95 + 191; 8,192 x 12,545 float 105 + 140 and 77 + 157.
+// (Long rows only: of short ones, whose vectors are 256 bytes of a row, a float gradient is slower so by more than that,
+// 131,072 x 785 103 + 150 and 73 + 190.)
 inline bool beyond_cache(long long rows, int cols, int dtype) {
     return rows * cols * (dtype == ISG_F32 ? 4 : 2) > (256ll << 20);
 }

@@ -320,7 +320,10 @@ __device__ __forceinline__ void row_alternative(const LogprobsArgs& a, long long
     a.top_classes[row * a.top + place] = (int)~(unsigned)key;
 }
 
-// A row in the registers of G lanes.
+// A row in the registers of G lanes: maximum first, then the sums of 2^x and 2^x x over the same registers, then the
+// alternatives out of them.  One read of the logits bounds it without alternatives, the search for them with: 131,072 x
+// 785 bf16 46 us (4.5 TB/s; 38 us where nothing has left the last-level cache dirty), with 5 alternatives 70, 20 98, 64
+// 202; float 103 (4.0 TB/s), with 20 117; 20,480 rows bf16 11.4.
 template <typename T, int G, int NE, bool TOP>
 __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restrict__ logits, LogprobsArgs a) {
     typedef typename std::conditional<sizeof(T) == 2, ShortKey, LongKey>::type Keys;
@@ -413,6 +416,10 @@ __device__ __forceinline__ int trim_list(TopList& list, int count, int k, float&
 // a list: of the first step all that reach the bound select_workgroup would take, of the later steps what exceeds
 // the list's own bound, which rises whenever the list has grown to kListTrim and is cut back.  Steps that would overrun
 // the list (rising rows, ties) or have no finite bound hand it their k first by select_workgroup instead.
+//
+// 2,048 x 131,071 bf16 with 64 alternatives: 140 us, 3.8 TB/s, the vector units busy for four fifths of it (some 8
+// instructions a class for the sums, one of them an exponential that takes four times an addition; 9 for the
+// alternatives); without alternatives 104 us, 5.2 TB/s.  2,048 x 65,537 float with 20: 104 us, 5.2 TB/s.
 template <typename T, int NE, bool TOP>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 8) void logprobs_stream_kernel(const T* __restrict__ logits,
                                                                                             LogprobsArgs a) {
@@ -530,7 +537,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 8) void logprobs_str
     }
 }
 
-// Joins the parts of a row: G threads, NE keys each.
+// Joins the parts of a row: G threads, NE keys each.  Its latency is what it costs: 4 us for one row in 24 parts, 5 for
+// 320 rows in 7.
 template <typename T, int G, int NE>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const T* __restrict__ logits, LogprobsArgs a) {
     __shared__ typename std::conditional<G == 64, u64[4 * candidates(64)], TopShared>::type shared;
@@ -585,6 +593,11 @@ struct LogprobsBwdArgs {
     float c, c_lo, inv_t;
 };
 
+// A row, or a part of one, by G lanes:
+//   dz_c = 1/T [ g_a [c = a] + sum_j g_j [c = i_j] - p_c (g_a + sum_j g_j + g_H (log p_c + H)) ],
+// the dense part first, from the row's kept m, s and H, then the few classes with a gradient of their own over it.  Reads
+// the logits, writes as much, and is bound by that: 131,072 x 785 bf16 88 us (4.7 TB/s read and written), 2,050 x 131,071
+// bf16 193 us (5.6), 2,048 x 65,537 float 195 us (5.5).
 template <typename T, int G, int NE>
 __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restrict__ logits, LogprobsBwdArgs a,
                                                                T* __restrict__ dlogits) {

@@ -662,3 +662,37 @@ def test_gradients_larger_than_the_last_level_cache(dtype, rows, cols):
                                        apart[r:].data_ptr(), up[r:].data_ptr(), h, cols, 8, code, 2.0, 0,
                                        want[r:].data_ptr(), s), "isg_distill_bwd")
     assert torch.equal(dd, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1, 518161), (1, 1001641), (1, 1 << 20), (2, 2041 * 257 + 3)])
+def test_gradients_of_few_rows_in_hundreds_of_parts(rows, cols, dtype):
+    """Every class has its gradient and nothing behind the last row is written (parts whose rounded size would leave
+    less than a vector to the last one)."""
+    from imagesegmentation_amd import _lib
+    decode, lib, code = _decode(), _lib.lib(), 1 if dtype == "bf16" else 0
+    guard = 64
+    g = torch.Generator(device=DEV).manual_seed(2)
+    held = torch.full([rows * cols + guard], float("nan"), dtype=DT[dtype], device=DEV)
+    z = held[:rows * cols].view(rows, cols)
+    z.copy_(torch.randn([rows, cols], generator=g, device=DEV) * 3)
+    tokens = torch.tensor([cols - 1, 0][:rows], device=DEV)
+    up = torch.randn([rows], generator=g, device=DEV)
+    classes = torch.tensor([[cols - 1, cols - 2, 5]] * rows, device=DEV)
+    values = torch.randn([rows, 3], generator=g, device=DEV)
+    stats = decode._logprobs_forward(z, (rows, cols, cols), tokens, None, 0, 1.0, True)[4]
+    apart = decode._distill_forward(z, (rows, cols, cols), values, classes, None, 2.0, 0, True)[1]
+    f64 = _f64(z)
+    stream = torch.cuda.current_stream().cuda_stream
+    out = torch.full([rows * cols + guard], 7.0, dtype=DT[dtype], device=DEV)
+    _lib.check(lib.isg_token_logprobs_bwd(z.data_ptr(), cols, tokens.data_ptr(), 8, None, stats.data_ptr(), up.data_ptr(),
+                                          None, None, rows, cols, code, 1.0, 0, out.data_ptr(), stream), "bwd")
+    want, tol = ref.token_logprobs_grad(f64, 1.0, tokens.cpu().numpy(), None, _f64(up), None, None, dtype)
+    ref.close(_f64(out[:rows * cols].view(rows, cols)), want, tol)
+    assert (out[rows * cols:] == 7).all()
+    out.fill_(7.0)
+    _lib.check(lib.isg_distill_bwd(z.data_ptr(), cols, values.data_ptr(), classes.data_ptr(), 8, apart.data_ptr(),
+                                   up.data_ptr(), rows, cols, 3, code, 2.0, 0, out.data_ptr(), stream), "bwd")
+    want = ref.distill(f64, _f64(values), classes.cpu().numpy(), 2.0, False, _f64(up), dtype)
+    ref.close(_f64(out[:rows * cols].view(rows, cols)), want["dlogits"], want["dlogits_tol"])
+    assert (out[rows * cols:] == 7).all()
