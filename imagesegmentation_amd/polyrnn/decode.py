@@ -257,7 +257,16 @@ def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
 
 
 # Backward passes run on autograd's own thread, where every line of Python costs two to three times what it does in the
-# caller's: what they pass to the library is put together in the forward pass, and their checks are the forward's.
+# caller's: sizes and types are put together in the forward pass, and their checks are the forward's.  The tensors are
+# asked for their addresses here: saved-tensor hooks (checkpoints, copies in host memory) may hand back others.
+def _saved_rows(z, cols, what):
+    """The logits as the forward pass saved them, and the elements from row to row."""
+    if z.is_contiguous():
+        return z, cols
+    z, _, _, stride = _class_rows(z, what)
+    return z, stride
+
+
 def _gradient_like(z, shape):
     """The tensor a gradient is written into: the logits' shape, dense."""
     if z.is_contiguous():
@@ -287,8 +296,6 @@ class _TokenLogprobs(torch.autograd.Function):
         logp, entropy, top_logp, top_cls, stats = _logprobs_forward(z, (rows, cols, stride), tokens, live, top,
                                                                     temperature, True)
         ctx.save_for_backward(z, tokens, top_cls, stats)
-        ctx.first = (z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4,
-                     _lib.ptr(top_cls), stats.data_ptr())
         ctx.last = (rows, cols, dtype_code(z.dtype), temperature, top)
         ctx.shape, ctx.in_dtype, ctx.device = logits.shape, logits.dtype, z.device.index
         if top_cls is not None:
@@ -301,11 +308,13 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, dlogp, dentropy, dtop, _):
         if dlogp is None and dentropy is None and dtop is None:
             return None, None, None, None, None
-        z = ctx.saved_tensors[0]  # (all of them are checked for changes in place)
+        z, tokens, top_cls, stats = ctx.saved_tensors
+        z, stride = _saved_rows(z, ctx.last[1], "token_logprobs")
         dlogp, dentropy, dtop = _float_gradient(dlogp), _float_gradient(dentropy), _float_gradient(dtop)
         dz = _gradient_like(z, ctx.shape)
         rc = _lib.lib().isg_token_logprobs_bwd(
-            *ctx.first, None if dlogp is None else dlogp.data_ptr(), None if dentropy is None else dentropy.data_ptr(),
+            z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4, _lib.ptr(top_cls),
+            stats.data_ptr(), None if dlogp is None else dlogp.data_ptr(), None if dentropy is None else dentropy.data_ptr(),
             None if dtop is None else dtop.data_ptr(), *ctx.last, dz.data_ptr(),
             torch._C._cuda_getCurrentRawStream(ctx.device))
         if rc:
@@ -374,8 +383,6 @@ class _Distill(torch.autograd.Function):
         z, rows, cols, stride = _class_rows(logits, "distill_rows")
         loss, stats = _distill_forward(z, (rows, cols, stride), values, classes, live, temperature, tail, True)
         ctx.save_for_backward(z, values, classes, stats)
-        ctx.first = (z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(), classes.element_size(),
-                     stats.data_ptr())
         ctx.last = (rows, cols, values.shape[-1], dtype_code(z.dtype), temperature, tail)
         ctx.shape, ctx.in_dtype, ctx.device = logits.shape, logits.dtype, z.device.index
         return loss
@@ -383,10 +390,12 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     @_first_derivative_only
     def backward(ctx, dloss):
-        z = ctx.saved_tensors[0]
+        z, values, classes, stats = ctx.saved_tensors
+        z, stride = _saved_rows(z, ctx.last[1], "distill_rows")
         g = _float_gradient(dloss)
         dz = _gradient_like(z, ctx.shape)
-        rc = _lib.lib().isg_distill_bwd(*ctx.first, g.data_ptr(), *ctx.last, dz.data_ptr(),
+        rc = _lib.lib().isg_distill_bwd(z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(),
+                                        classes.element_size(), stats.data_ptr(), g.data_ptr(), *ctx.last, dz.data_ptr(),
                                         torch._C._cuda_getCurrentRawStream(ctx.device))
         if rc:
             _lib.check(rc, "isg_distill_bwd")
@@ -437,7 +446,7 @@ def distill_mean(logits, teacher_values, teacher_classes, temperature=1.0, tail=
     loss = distill_rows(logits, teacher_values, teacher_classes, temperature, tail, live)
     if live is None:
         return loss.mean()
-    return loss.sum() / live.sum().clamp(min=1)
+    return loss.sum() / torch.count_nonzero(live).clamp(min=1)
 
 
 def decode_begin(true_vertices, num_true, hist, steps):

@@ -458,6 +458,7 @@ def test_shapes_types_and_orders_of_the_arguments():
     want = a[live].double().mean()
     assert abs(float(m) - float(want)) <= 1e-6 * float(want)
     assert float(decode.distill_mean(z, v, c, live=torch.zeros_like(live))) == 0.0
+    assert float(decode.distill_mean(z, v, c, live=live.to(torch.uint8) * 255)) == float(m)
     assert abs(float(decode.distill_mean(z, v, c)) - float(a.double().mean())) <= 1e-6 * float(a.double().mean())
 
 
@@ -696,3 +697,86 @@ def test_gradients_of_few_rows_in_hundreds_of_parts(rows, cols, dtype):
     want = ref.distill(f64, _f64(values), classes.cpu().numpy(), 2.0, False, _f64(up), dtype)
     ref.close(_f64(out[:rows * cols].view(rows, cols)), want["dlogits"], want["dlogits_tol"])
     assert (out[rows * cols:] == 7).all()
+
+
+@pytest.mark.parametrize("width", [785, 800])
+def test_saved_tensors_that_come_back_at_other_addresses(width):
+    """Under a checkpoint, and with what autograd keeps held in host memory (which comes back dense)."""
+    from torch.utils.checkpoint import checkpoint
+    decode = _decode()
+    g = torch.Generator(device=DEV).manual_seed(4)
+    held = torch.randn([64, width], generator=g, device=DEV)
+    tokens = torch.randint(785, [64], generator=g, device=DEV)
+    values, classes = torch.randn([64, 9], generator=g, device=DEV), torch.randint(785, [64, 9], generator=g, device=DEV)
+
+    def both(w):
+        z = (w * 1.0)[:, :785]
+        out = decode.token_logprobs(z, tokens, top=3)
+        return out.logprobs.sum() + (out.entropy ** 2).sum() + out.top_logprobs[:, 1].sum() + \
+            decode.distill_rows(z, values, classes, temperature=2.0).sum()
+
+    def gradient(how):
+        w = held.clone().requires_grad_(True)
+        loss = how(w)
+        torch.randn([1 << 20], device=DEV)  # (what has been freed is used again)
+        return torch.autograd.grad(loss, w)[0]
+
+    want = gradient(both)
+    assert torch.equal(gradient(lambda w: checkpoint(both, w, use_reentrant=False)), want)
+
+    def on_host(w):
+        with torch.autograd.graph.save_on_cpu():
+            return both(w)
+    assert torch.equal(gradient(on_host), want)
+
+
+def test_two_calls_at_once():
+    """On two streams, with a workspace each."""
+    decode = _decode()
+    g = torch.Generator(device=DEV).manual_seed(6)
+    z = [torch.randn([9, 50177], generator=g, device=DEV, dtype=torch.float32) for _ in range(2)]
+    tokens = torch.randint(50177, [9], generator=g, device=DEV)
+
+    def call(x):
+        x = x.clone().requires_grad_(True)
+        out = decode.token_logprobs(x, tokens, top=7)
+        loss = decode.distill_rows(x, out.top_logprobs, out.top_classes, temperature=2.0, tail=True)
+        return (out.logprobs.detach(), out.entropy.detach(), out.top_classes, loss.detach()) + \
+            torch.autograd.grad([out.entropy, loss], x, [torch.ones_like(loss), torch.ones_like(loss)])
+    want = [call(x) for x in z]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(z[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for result in got[i]:
+            for a, b in zip(result, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_tens_of_millions_of_rows():
+    """More workgroups than one axis of a grid is given."""
+    decode = _decode()
+    rows, cols = (1 << 24) + 4099, 3
+    z = torch.randn([rows, cols], generator=torch.Generator(device=DEV).manual_seed(8), device=DEV).requires_grad_(True)
+    tokens = torch.arange(rows, device=DEV) % cols
+    out = decode.token_logprobs(z, tokens, top=1)
+    loss = decode.distill_rows(z, torch.zeros([rows, 1], device=DEV), tokens[:, None])
+    dz, = torch.autograd.grad(out.entropy.sum() + loss.sum(), z)
+    with torch.no_grad():
+        logp = torch.log_softmax(z.double(), dim=1)
+        p = logp.exp()
+        entropy = -(p * logp).sum(dim=1)
+        chosen = logp.gather(1, tokens[:, None])[:, 0]
+        # three classes: each of a dozen roundings is of a value below |log p| + 1
+        tol = 16 * 2.0 ** -24 * (logp.abs().max(dim=1).values + z.detach().abs().max(dim=1).values + 2)
+        assert ((out.logprobs - chosen).abs() <= tol).all() and ((loss + chosen).abs() <= tol).all()
+        assert ((out.entropy - entropy).abs() <= tol).all()
+        assert (z.gather(1, out.top_classes.long())[:, 0] == z.max(dim=1).values).all()
+        want = p * (1 - (logp + entropy[:, None]))
+        want.scatter_add_(1, tokens[:, None], torch.full([rows, 1], -1.0, dtype=torch.float64, device=DEV))
+        assert ((dz - want).abs() <= 4 * tol[:, None]).all()
