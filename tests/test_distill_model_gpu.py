@@ -116,6 +116,32 @@ def test_a_model_learns_from_another(name, dtype):
     assert abs(float(fourth.last_metrics["distill"])) < fourth.num_classes * 2 * ref.U + d * d / 2
 
 
+@pytest.mark.gpu
+def test_distillation_between_graph_replayed_steps():
+    """Steps towards a teacher, launched one by one, between training steps that replay captured graphs: the same
+    losses and parameters, bit for bit, as without graphs."""
+    from oracle import raster as oracle_raster
+    from imagesegmentation_amd import data
+    ds = data.PolygonDataset.synthetic(24, 28, 28, 10, 2, seed=9, shape_mask_fn=oracle_raster.create_shape_mask)
+    teacher = _model("History2Large", "bf16", seed=1)
+    runs = []
+    for graphs in (False, True):
+        model = _model("History2Large", "bf16", seed=5)
+        model.step_graphs = graphs
+        np.random.seed(77)
+        losses = []
+        for n in range(6):
+            d, images, pts, t, _ = ds.get_batch_points(8)
+            if n % 2:
+                model.distill(images, d, pts, t, teacher, top=20)
+                losses.append(model.loss.clone())
+            else:
+                losses.append(model.train_step(images, d, pts, t).clone())
+        runs.append((torch.stack(losses), model._flat_param.clone(), len(model._step_graph_cache)))
+    assert runs[0][2] == 0 and runs[1][2] >= 1
+    assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
+
+
 def test_distillation_refuses_teachers_that_do_not_fit():
     model = _model("History0", "f32", device="cpu")
     args = (None, None, None, None)
