@@ -6,8 +6,9 @@ namespace {
 
 constexpr int kMaxTop = ISG_TOP_MAX;  // classes kept per row
 constexpr int kListMax = 1024;        // alternatives a workgroup collects along its part of a row
-constexpr int kListTrim = 256;        // ... before it goes back to the best, of which it may keep
-constexpr int kListKeep = 128;        // this many
+// ... before it goes back to the best, of which it may keep twice as many as are asked for
+constexpr int list_limit(int k) { return 2 * k + 32; }
+constexpr int kListKeep = 2 * kMaxTop;
 
 // ---- the `top` first keys of a unit ----------------------------------------------------------------------------------
 // The k-th largest of the threads' group maxima is a lower bound of the k-th largest element (k groups hold one at
@@ -400,7 +401,7 @@ __device__ __forceinline__ int trim_list(TopList& list, int count, int k, float&
     }
     __syncthreads();
     int n = list.count;
-    if (n > kListKeep) {
+    if (n > 2 * k) {
         rank_keys<kThreads>(list.keys, count, k, [&](int place, u64 key) { list.kept[place] = key; });
         __syncthreads();
         n = count < k ? count : k;
@@ -414,7 +415,7 @@ __device__ __forceinline__ int trim_list(TopList& list, int count, int k, float&
 // A part of a longer row: a workgroup walks over it, kThreads * NE classes at a time, the next ones being loaded
 // meanwhile.  Every wave keeps its own maximum and its lanes their own sums until the end.  The best classes gather in
 // a list: of the first step all that reach the bound select_workgroup would take, of the later steps what exceeds
-// the list's own bound, which rises whenever the list has grown to kListTrim and is cut back.  Steps that would overrun
+// the list's own bound, which rises whenever the list has grown to its limit and is cut back.  Steps that would overrun
 // the list (rising rows, ties) or have no finite bound hand it their k first by select_workgroup instead.
 //
 // 2,048 x 131,071 bf16 with 64 alternatives: 140 us, 3.8 TB/s, the vector units busy for four fifths of it (some 8
@@ -508,7 +509,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 8) void logprobs_str
                 __syncthreads();
                 count += a.top;
             }
-            if (count > kListTrim || !fits) {
+            if (count > list_limit(a.top) || !fits) {
                 count = trim_list(list, count, a.top, low);
                 bounded = low > -INFINITY;  // (no bound from classes at -inf or NaN)
             }
