@@ -342,23 +342,29 @@ inline int equal_part(int cols, int splits) {
     const int even = (cols + splits - 1) / splits, per = (even + 7) / 8 * 8, last = (cols - 1) % per + 1;
     return splits > 1 && last < 64 ? even : per;
 }
-// lanes = 0: too long for a wave's registers.  16 lanes a row (32 for the longer) where there are rows enough for every
-// SIMD to have waves, else a whole wave: 16 rows of 785 classes take 4.6 us so and 6.8 us in 16 lanes each, 131,072 rows
-// 64 and 47 us.  `entries`: places a row needs in its threads' registers, four a thread (sixteen in rows of 64 classes).
-inline Cut cut_wave(long long rows, int cols, int dtype, int entries) {
+// A row by 16 lanes of a wave where `narrow` classes a lane hold it (beyond 64: also by 32 lanes), else by a whole wave;
+// lanes = 0: too long for that.  `entries`: places a row needs in its threads' registers, four a thread (sixteen in rows of
+// 64 classes).
+inline Cut cut_wave(int cols, int dtype, int entries, int narrow) {
     const int most = dtype == ISG_F32 ? 4 : 8;
-    if (rows > 4096 && entries <= 64) {
-        for (int ne : {1, 4, 8, 16, 24, 32, 40, 48, 56, 64})
-            if (cols + (ne < most ? ne : most) - 1 <= 16 * ne) return Cut{16, ne, 1, cols};
+    for (int ne : {1, 4, 8, 16, 24, 32, 40, 48, 56, 64})
+        if (ne <= narrow && cols + (ne < most ? ne : most) - 1 <= 16 * ne) return Cut{16, ne, 1, cols};
+    if (narrow > 64)
         for (int ne : {48, 64})
             if (cols + most - 1 <= 32 * ne) return Cut{32, ne, 1, cols};
-    }
     for (int ne : {1, 4, 8, 16, 24, 32})
         if ((ne == 1 || entries <= 256) && cols + (ne < most ? ne : most) - 1 <= 64 * ne) return Cut{64, ne, 1, cols};
     return Cut{0, 0, 1, cols};
 }
-inline Cut cut_forward(long long rows, int cols, int dtype, int entries = 0) {
-    const Cut wave = cut_wave(rows, cols, dtype, entries);
+// Few rows take a wave each (5,000 x 785 bf16 5.0 us, by 16 lanes 5.8; 20 best 8.4 and 12.5).  Many take 16 lanes each: what
+// a row costs once is paid for four of them in the same instructions (131,072 x 785 bf16 47 us, by waves 63; 5 best 70 and
+// 91; distilled with 16 entries and a tail 61 and 97).  What grows with the best classes or the entries is paid by fewer
+// lanes so: many of those in long rows are a whole wave's again (20 best of 10,240 x 785 bf16 12.7 us, by 16 lanes 14.7, of
+// 66,000 x 1,000 57 and 66; 64 entries of 131,072 x 785 74 and 86, of 66,000 x 380 28 and 24).
+inline Cut cut_forward(long long rows, int cols, int dtype, int entries, int best) {
+    int narrow = rows > 8192 && entries <= 64 ? 65 : 0;
+    if (narrow && (entries > 16 || best > 16)) narrow = best > 16 && rows <= 49152 ? 24 : 40;
+    const Cut wave = cut_wave(cols, dtype, entries, narrow);
     if (wave.lanes) return wave;
     long long splits = (units_of(dtype) + rows - 1) / (rows > 0 ? rows : 1);
     const int most = cols / kPartCols < kMaxSplits ? cols / kPartCols : kMaxSplits, least = (cols + kMarkCols - 1) / kMarkCols;
@@ -367,8 +373,13 @@ inline Cut cut_forward(long long rows, int cols, int dtype, int entries = 0) {
     const int per = equal_part(cols, (int)splits);
     return Cut{kThreads, 16, (cols + per - 1) / per, per};
 }
-inline Cut cut_backward(long long rows, int cols, int dtype, int entries = 0) {
-    const Cut wave = cut_wave(rows, cols, dtype, entries);
+// The backward passes have less to pay once a row, and longer runs of memory by a whole wave: 131,072 x 785 bf16 84 us, by
+// 16 lanes 88; float 138 and 150; 64 entries bf16 100 and 142; 66,000 x 380 bf16 22.9 and 22.4, float 32.6 and 33.8; x 120
+// 20 and 9.5; x 250 with 64 entries 29 and 33.
+constexpr int kNarrowBackward = 32;
+inline Cut cut_backward(long long rows, int cols, int dtype, int entries) {
+    const int narrow = rows <= 8192 || entries > 64 ? 0 : (entries > 16 ? 8 : (dtype == ISG_F32 ? 24 : kNarrowBackward));
+    const Cut wave = cut_wave(cols, dtype, entries, narrow);
     if (wave.lanes) return wave;
     const auto parts = [&](int ne) { return (cols + kThreads * ne - 8 - 1) / (kThreads * ne - 8); };
     for (int ne = 8;; ne *= 2) {
@@ -394,14 +405,15 @@ inline dim3 grid_of(long long units, int threads) {
     return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
 
-// F::template run<G, NE>(...) for a wave's cut
-template <typename F, typename... A>
+// F::template run<G, NE>(...) for a wave's cut, up to NARROW classes a lane by 16 lanes
+template <typename F, int NARROW, typename... A>
 void with_wave(const Cut& cut, A&&... args) {
-    if (cut.lanes == 32) {
-        if (cut.ne == 48) F::template run<32, 48>(args...);
-        else F::template run<32, 64>(args...);
-        return;
-    }
+    if constexpr (NARROW > 64)
+        if (cut.lanes == 32) {
+            if (cut.ne == 48) F::template run<32, 48>(args...);
+            else F::template run<32, 64>(args...);
+            return;
+        }
     if (cut.lanes == 64) {
         switch (cut.ne) {
             case 1: F::template run<64, 1>(args...); break;
@@ -420,15 +432,17 @@ void with_wave(const Cut& cut, A&&... args) {
         case 16: F::template run<16, 16>(args...); break;
         case 24: F::template run<16, 24>(args...); break;
         case 32: F::template run<16, 32>(args...); break;
+    }
+    if constexpr (NARROW > 32) switch (cut.ne) {
         case 40: F::template run<16, 40>(args...); break;
         case 48: F::template run<16, 48>(args...); break;
         case 56: F::template run<16, 56>(args...); break;
-        default: F::template run<16, 64>(args...);
+        case 64: F::template run<16, 64>(args...); break;
     }
 }
 template <typename F, typename... A>
 void launch_backward(const Cut& cut, A&&... args) {
-    if (cut.lanes != kThreads) with_wave<F>(cut, args...);
+    if (cut.lanes != kThreads) with_wave<F, kNarrowBackward>(cut, args...);
     else if (cut.ne == 8) F::template run<kThreads, 8>(args...);
     else if (cut.ne == 16) F::template run<kThreads, 16>(args...);
     else F::template run<kThreads, 32>(args...);

@@ -556,9 +556,9 @@ void launch_forward(const Cut& cut, const void* logits, const DistillArgs& a, hi
         hipLaunchKernelGGL((distill_stream_kernel<T, 16, TAIL>), grid_of(a.units, kThreads), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a);
     else if (a.k <= cut.lanes)
-        with_wave<DistillFwd<T, TAIL, 1>>(cut, logits, a, s);
+        with_wave<DistillFwd<T, TAIL, 1>, 65>(cut, logits, a, s);
     else
-        with_wave<DistillFwd<T, TAIL, 4>>(cut, logits, a, s);
+        with_wave<DistillFwd<T, TAIL, 4>, 65>(cut, logits, a, s);
 }
 template <typename T, int PLACES>
 struct DistillBwd {
@@ -584,7 +584,7 @@ int check_entries(const char* who, int k, int tail) {
 
 extern "C" long long isg_distill_workspace_bytes(int rows, int cols) {
     if (rows < 0 || cols < 1 || cols > kMaxCols) return -1;
-    const Cut cut = cut_forward(rows, cols, ISG_F32);  // (bf16 rows are in as many parts or fewer)
+    const Cut cut = cut_forward(rows, cols, ISG_F32, 0, 0);  // (bf16 rows are in as many parts or fewer)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * (long long)sizeof(DistillPart);
 }
 
@@ -600,7 +600,7 @@ extern "C" int isg_distill_fwd(const void* logits, long long row_stride, const f
     if (rc != ISG_OK) return rc;
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && values && classes && loss, ISG_EINVAL, "%s: null pointer", who);
-    const Cut cut = cut_forward(rows, cols, dtype, k);
+    const Cut cut = cut_forward(rows, cols, dtype, k, 0);
     ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     hipStream_t s = static_cast<hipStream_t>(stream);
     DistillArgs a{};

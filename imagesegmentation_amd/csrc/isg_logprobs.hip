@@ -679,7 +679,7 @@ struct LogprobsFwd {
     }
     static void launch(const Cut& cut, const void* logits, const LogprobsArgs& a, hipStream_t s) {
         if (cut.lanes != kThreads)
-            with_wave<LogprobsFwd>(cut, logits, a, s);
+            with_wave<LogprobsFwd, 65>(cut, logits, a, s);
         else
             hipLaunchKernelGGL((logprobs_stream_kernel<T, 16, TOP>), grid_of(a.units, kThreads), dim3(kThreads), 0, s,
                                static_cast<const T*>(logits), a);
@@ -718,7 +718,7 @@ int check_top(const char* who, int top, int cols) {
 
 extern "C" long long isg_token_logprobs_workspace_bytes(int rows, int cols, int top) {
     if (rows < 0 || cols < 1 || cols > kMaxCols || top < 0 || top > kMaxTop) return -1;
-    const Cut cut = cut_forward(rows, cols, ISG_F32);  // (bf16 rows are in as many parts or fewer)
+    const Cut cut = cut_forward(rows, cols, ISG_F32, 0, top);  // (bf16 rows are in as many parts or fewer)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * ((long long)sizeof(Sums) + 8 * top) + 8;
 }
 
@@ -736,7 +736,7 @@ extern "C" int isg_token_logprobs_fwd(const void* logits, long long row_stride, 
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && entropy && (!tokens || logprobs) && (top == 0 || (top_logprobs && top_classes)), ISG_EINVAL,
                 "%s: null pointer", who);
-    const Cut cut = cut_forward(rows, cols, dtype);
+    const Cut cut = cut_forward(rows, cols, dtype, 0, top);
     ISG_REQUIRE(cut.splits == 1 || workspace, ISG_EINVAL, "%s: %d x %d logits need a workspace", who, rows, cols);
     ISG_REQUIRE(((uintptr_t)workspace | (uintptr_t)stats) % 8 == 0 && (uintptr_t)stats % 16 == 0, ISG_EINVAL,
                 "%s: workspace and stats must be aligned to 8 and 16 bytes", who);
@@ -781,7 +781,7 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
     ISG_REQUIRE(logits && stats && dlogits && (!dlogprobs || tokens) && (!dtop_logprobs || (top > 0 && top_classes)),
                 ISG_EINVAL, "%s: null pointer", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
-    const Cut cut = cut_backward(rows, cols, dtype);
+    const Cut cut = cut_backward(rows, cols, dtype, 0);
     hipStream_t s = static_cast<hipStream_t>(stream);
     LogprobsBwdArgs a{};
     a.tokens = tokens, a.top_classes = top_classes, a.stats = stats;

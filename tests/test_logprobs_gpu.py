@@ -118,16 +118,20 @@ def test_logprobs_over_masks_and_ties(kind, cols, dtype):
 MANY = 37 * 113
 
 
-def _many(a):
-    return None if a is None else np.concatenate([a] * 113)
+# (37 rows, so many times over: a wave a row, 16 lanes a row)
+TIMES = (113, 223)
 
 
-def _check_many(t, z, T, tokens, top, live, dtype, rs):
+def _many(a, times):
+    return None if a is None else np.concatenate([a] * times)
+
+
+def _check_many(t, z, T, tokens, top, live, dtype, rs, times):
     decode = _decode()
-    big = t.repeat(113, 1).requires_grad_(True)
-    want = {k: _many(v) for k, v in ref.token_logprobs(z, T, tokens, top).items()}
-    on = _many(live)
-    out = decode.token_logprobs(big, torch.tensor(_many(tokens), device=DEV), top=top, temperature=T,
+    big = t.repeat(times, 1).requires_grad_(True)
+    want = {k: _many(v, times) for k, v in ref.token_logprobs(z, T, tokens, top).items()}
+    on = _many(live, times)
+    out = decode.token_logprobs(big, torch.tensor(_many(tokens, times), device=DEV), top=top, temperature=T,
                                 live=torch.tensor(on, device=DEV))
     for name in ("logprobs", "entropy", "top_logprobs"):
         if name in want:
@@ -140,45 +144,56 @@ def _check_many(t, z, T, tokens, top, live, dtype, rs):
     gl, gh = rs.randn(37).astype(np.float32), rs.randn(37).astype(np.float32)
     gt = rs.randn(37, top).astype(np.float32) if top else None
     outs = [out.logprobs, out.entropy] + ([out.top_logprobs] if top else [])
-    gs = [torch.tensor(_many(g), device=DEV) for g in (gl, gh, gt) if g is not None]
+    gs = [torch.tensor(_many(g, times), device=DEV) for g in (gl, gh, gt) if g is not None]
     dz, = torch.autograd.grad(outs, big, gs)
     f = lambda g: None if g is None else g.astype(np.float64)
     classes = ref.token_logprobs(z, T, None, top).get("top_classes")
     wd, wtol = ref.token_logprobs_grad(z, T, tokens, classes, f(gl), f(gh), f(gt), dtype)
     got = _f64(dz)
-    ref.close(got[on], _many(wd)[on], _many(wtol)[on])
+    ref.close(got[on], _many(wd, times)[on], _many(wtol, times)[on])
     assert np.all(got[~on] == 0)
 
 
+@pytest.mark.parametrize("times", TIMES)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("kind", ["peaked", "masked"])
 @pytest.mark.parametrize("cols", [1, 2, 9, 16, 17, 57, 61, 64, 120, 127, 250, 255, 377, 505, 640, 766, 785, 1015, 1016, 1024, 1400,
                                   1530, 2041, 2044, 2046])
-def test_logprobs_of_thousands_of_rows(cols, kind, dtype):
+def test_logprobs_of_thousands_of_rows(cols, kind, dtype, times):
     rs = np.random.RandomState(cols)
     t, z = _logits(37, cols, dtype, kind, cols)
     tokens = rs.randint(0, cols, [37])
     live = rs.rand(37) < 0.8
     for top in sorted({0, min(cols, 5), min(cols, 64)}):
-        _check_many(t, z, 1.3, tokens, top, live, dtype, rs)
+        _check_many(t, z, 1.3, tokens, top, live, dtype, rs, times)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols,top", [(130, 20), (500, 17), (640, 64), (785, 20)])
+def test_the_best_classes_of_tens_of_thousands_of_rows(cols, top, dtype):
+    rs = np.random.RandomState(cols)
+    t, z = _logits(37, cols, dtype, "peaked", cols)
+    _check_many(t, z, 1.3, rs.randint(0, cols, [37]), top, rs.rand(37) < 0.8, dtype, rs, 1330)
+
+
+@pytest.mark.parametrize("times", TIMES)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("kind", ["ties", "rising", "constant", "lowest", "zeros"])
 @pytest.mark.parametrize("cols", [30, 785, 1500])
-def test_logprobs_of_thousands_of_odd_rows(cols, kind, dtype):
+def test_logprobs_of_thousands_of_odd_rows(cols, kind, dtype, times):
     rs = np.random.RandomState(cols)
     t, z = _logits(37, cols, dtype, kind, cols)
     for top in (3, min(cols, 40)):
-        _check_many(t, z, 0.7, rs.randint(0, cols, [37]), top, np.ones([37], bool), dtype, rs)
+        _check_many(t, z, 0.7, rs.randint(0, cols, [37]), top, np.ones([37], bool), dtype, rs, times)
 
 
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("times", TIMES)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cols,k", [(1, 1), (2, 2), (9, 3), (17, 17), (61, 5), (64, 64), (120, 8), (250, 64), (505, 20), (785, 16),
                                     (785, 64), (785, 65), (785, 300), (1016, 33), (1017, 4), (1500, 64), (2041, 64), (2045, 100),
                                     (40, 300), (12, 20)])
-def test_distillation_of_thousands_of_rows(cols, k, dtype, tail):
+def test_distillation_of_thousands_of_rows(cols, k, dtype, tail, times):
     decode = _decode()
     rs = np.random.RandomState(cols + k)
     t, z = _logits(37, cols, dtype, "peaked", cols)
@@ -191,18 +206,18 @@ def test_distillation_of_thousands_of_rows(cols, k, dtype, tail):
         values[3] -= 1.0
         classes[6, :] = -1
     live = rs.rand(37) < 0.8
-    on = _many(live)
+    on = _many(live, times)
     g = rs.randn(37).astype(np.float32)
-    big = t.repeat(113, 1).requires_grad_(True)
-    loss = decode.distill_rows(big, torch.tensor(_many(values), device=DEV), torch.tensor(_many(classes), device=DEV),
-                               temperature=1.3, tail=tail, live=torch.tensor(on, device=DEV))
+    big = t.repeat(times, 1).requires_grad_(True)
+    loss = decode.distill_rows(big, torch.tensor(_many(values, times), device=DEV),
+                               torch.tensor(_many(classes, times), device=DEV), temperature=1.3, tail=tail, live=torch.tensor(on, device=DEV))
     want = ref.distill(z, values.astype(np.float64), classes, 1.3, tail, g.astype(np.float64), dtype)
     got = _f64(loss)
-    ref.close(got[on], _many(want["loss"])[on], _many(want["loss_tol"])[on])
+    ref.close(got[on], _many(want["loss"], times)[on], _many(want["loss_tol"], times)[on])
     assert np.all(got[~on] == 0)
-    dz, = torch.autograd.grad(loss, big, torch.tensor(_many(g), device=DEV))
+    dz, = torch.autograd.grad(loss, big, torch.tensor(_many(g, times), device=DEV))
     got = _f64(dz)
-    ref.close(got[on], _many(want["dlogits"])[on], _many(want["dlogits_tol"])[on])
+    ref.close(got[on], _many(want["dlogits"], times)[on], _many(want["dlogits_tol"], times)[on])
     assert np.all(got[~on] == 0)
 
 
