@@ -1,5 +1,5 @@
 // What the kernels over the class axis share (isg_logprobs.hip, isg_distill.hip): how a row lies over the lanes, sums and
-// maxima across them, exponents, the order of the classes.
+// maxima across them, exponents, the order of the classes, and how launches cut them.
 //
 // A row z of n logits at temperature T has, with m = max z and x_c = (z_c - m) log2(e) / T,
 //   log p_c = ln 2 (x_c - log2 s),   s = sum 2^x_c,   H = -sum p_c log p_c = ln 2 (log2 s - (sum 2^x_c x_c) / s);
@@ -9,8 +9,8 @@
 //
 // Layout.  A row is read once, into registers: up to about 1,000 classes by 16 lanes (four rows a wave: what a row costs
 // once - reductions, logarithms, outputs - is paid for four rows in the same instructions), up to about 2,000 by 32
-// lanes, or by a whole wave where there are few rows.  Longer rows are walked over by workgroups, a part of the row each,
-// whose results a second launch joins.
+// lanes, or by a whole wave where there are few rows or much to do for each class that counts (cut_forward, cut_backward).
+// Longer rows are walked over by workgroups, a part of the row each, whose results a second launch joins.
 #pragma once
 #include <hip/hip_bf16.h>
 
@@ -391,9 +391,9 @@ inline Cut cut_backward(long long rows, int cols, int dtype, int entries) {
 
 // Whether a gradient is more than the last-level cache holds (256 MB).  What reads it next does not find it there either,
 // and left in the cache it has to be written back under the next kernel's reads: 2,048 x 131,071 bf16 distilled (two parts
-// a row), forward and backward 118 + 185 us, written past the cache 95 + 191; 8,192 x 12,545 float 105 + 140 and 77 + 157.
-// (Long rows only: of short ones, whose vectors are 256 bytes of a row, a float gradient is slower so by more than that,
-// 131,072 x 785 103 + 150 and 73 + 190.)
+// a row), forward and backward 118 + 185 us, written past the cache 95 + 191; 8,192 x 12,545 float 105 + 140 and 77 + 157;
+// log-probabilities of 131,072 x 785 float 100 + 136 and 74 + 148.  (Not by 16 lanes, whose vectors are 256 bytes of a row:
+// 103 + 150 and 73 + 190; and not of short rows distilled, whose forward pass waits for less: nothing gained.)
 inline bool beyond_cache(long long rows, int cols, int dtype) {
     return rows * cols * (dtype == ISG_F32 ? 4 : 2) > (256ll << 20);
 }

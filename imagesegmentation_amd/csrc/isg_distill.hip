@@ -225,9 +225,9 @@ __device__ __forceinline__ void mark_entries(const DistillArgs& a, const Entries
 }
 
 // A row in the registers of G lanes, its entries beside them; with a tail the entries' classes are marked in LDS (a bit
-// each), taken out of the registers and summed apart.  131,072 x 785 bf16 with 16 entries and a tail 61 us (3.4 TB/s;
-// sums, marks and the closing logarithms weigh as much as the read), with 64 entries without 85; float, 64 and a tail,
-// 115 (3.6 TB/s); 20,480 rows bf16 13.4.
+// each), taken out of the registers and summed apart.  131,072 x 785 bf16 with 16 entries and a tail 52 to 61 us (3.4 TB/s;
+// sums, marks and the closing logarithms weigh as much as the read), with 64 entries without 68 to 74; float, 64 and a
+// tail, 97 to 113 (3.6 TB/s); 20,480 rows bf16 13.4.  (More where a gradient before it has left the cache dirty.)
 template <typename T, int G, int NE, int PLACES, bool TAIL>
 __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restrict__ logits, DistillArgs a) {
     __shared__ u64 marks[TAIL ? kThreads : 1];  // a thread's elements that an entry names, one bit each
@@ -410,7 +410,7 @@ struct DistillBwdArgs {
 
 // A row, or a part of one, by G lanes: the dense part from the row's kept constants, the entries' own values over it.  Reads
 // the logits and writes as much: 2,048 x 131,071 bf16 191 us (5.6 TB/s read and written), 8,192 x 12,545 float 154 us
-// (5.3), 131,072 x 785 bf16 with 16 entries 96 us (4.3), float with 64 179 us (4.6).
+// (5.3), 131,072 x 785 bf16 with 16 entries 81 to 100 us (4.6), float with 64 153 us (5.4).
 template <typename T, int G, int NE, int PLACES>
 __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restrict__ logits, DistillBwdArgs a,
                                                               T* __restrict__ dlogits) {
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     };
     if constexpr (G <= 64) {
         // A slot's vectors go through LDS, where the entries' values take their places: stored one by one behind the row
-        // they cost a write of 64 bytes each (131,072 x 785 float with 64 entries: 230 us for 179; bf16 144 for 142).
+        // they cost a write of 64 bytes each (131,072 x 785 float with 64 entries, by 16 lanes: 230 us for 179; bf16 144 for 142).
         if (!zero) {
             fetch_entries();
             span.template load<false>(z, v);

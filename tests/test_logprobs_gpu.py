@@ -646,7 +646,8 @@ def test_rows_past_two_to_the_thirty_one_elements():
     assert not loss[:-2].any() and not g[:-2].any()
 
 
-@pytest.mark.parametrize("dtype,rows,cols", [("bf16", 1100, 131071), ("f32", 5500, 12545)])
+@pytest.mark.parametrize("dtype,rows,cols", [("bf16", 1100, 131071), ("f32", 5500, 12545), ("f32", 90000, 785),
+                                             ("bf16", 120000, 1400)])
 def test_gradients_larger_than_the_last_level_cache(dtype, rows, cols):
     """They are written past it: the same values as from two calls over half the rows, which are not.  (Given the rows'
     statistics: the forward pass cuts fewer rows into more parts, whose sums round in another order.)"""
