@@ -160,10 +160,3 @@ def ptr(t):
 def current_stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
-
-
-def stream_of(t):
-    """The current stream of a tensor's device, as the C entries take it (a fifth of ``current_stream``'s time, which a
-    call from an autograd thread pays six-fold)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(t.device.index)

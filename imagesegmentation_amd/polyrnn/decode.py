@@ -1,6 +1,5 @@
 """Softmax cross-entropy, argmax, sampling, log-probabilities and distillation over the vertex class grid, on the libisg
 kernels (isg_softmax_xent_fwd / _bwd, isg_argmax_rows, isg_sample_rows, isg_token_logprobs_*, isg_distill_*)."""
-import contextlib
 import typing
 
 import torch
@@ -217,14 +216,15 @@ def _temperature(value, what):
     return value
 
 
-def _on_device(t):
-    """The kernels launch on the current device's stream: for a tensor of another device that one is made current."""
-    if t.device.index == torch.cuda.current_device():
-        return _here
-    return torch.cuda.device(t.device)
-
-
-_here = contextlib.nullcontext()
+def _launch(function, device, args):
+    """A launch on the current stream of the device, which is made the current one where it is not."""
+    if device == torch._C._cuda_getDevice():
+        rc = function(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _lib.check(rc, function.__name__)
 
 
 _ONE_UNIT_CLASSES = 2048  # rows up to here take no workspace
@@ -234,11 +234,11 @@ _ROW_MASKS = (torch.bool, torch.uint8)
 
 def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
     rows, cols, stride = geometry
-    lib, dev = _lib.lib(), z.device
-    f32 = torch.float32
+    lib, dev, f32 = _lib.lib(), z.device, torch.float32
     entropy = torch.empty([rows], dtype=f32, device=dev)
-    logp = torch.empty_like(entropy) if tokens is not None else None
-    top_logp = top_cls = stats = space = None
+    logp = top_logp = top_cls = stats = space = None
+    if tokens is not None:
+        logp = torch.empty_like(entropy)
     if top:
         top_logp = torch.empty([rows, top], dtype=f32, device=dev)
         top_cls = torch.empty([rows, top], dtype=torch.int32, device=dev)
@@ -246,32 +246,27 @@ def _logprobs_forward(z, geometry, tokens, live, top, temperature, keep):
         stats = torch.empty([rows, 4], dtype=f32, device=dev)
     if cols > _ONE_UNIT_CLASSES:
         space = torch.empty([lib.isg_token_logprobs_workspace_bytes(rows, cols, top)], dtype=torch.uint8, device=dev)
-    with _on_device(z):
-        rc = lib.isg_token_logprobs_fwd(
-            z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4, _lib.ptr(live),
-            rows, cols, dtype_code(z.dtype), temperature, top, _lib.ptr(logp), entropy.data_ptr(), _lib.ptr(top_logp),
-            _lib.ptr(top_cls), _lib.ptr(stats), _lib.ptr(space), _lib.stream_of(z))
-    if rc:
-        _lib.check(rc, "isg_token_logprobs_fwd")
+    _launch(lib.isg_token_logprobs_fwd, dev.index, (
+        z.data_ptr(), stride, _address(tokens), tokens.element_size() if tokens is not None else 4, _address(live), rows,
+        cols, dtype_code(z.dtype), temperature, top, _address(logp), entropy.data_ptr(), _address(top_logp),
+        _address(top_cls), _address(stats), _address(space)))
     return logp, entropy, top_logp, top_cls, stats
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 # Backward passes run on autograd's own thread, where every line of Python costs two to three times what it does in the
 # caller's: sizes and types are put together in the forward pass, and their checks are the forward's.  The tensors are
 # asked for their addresses here: saved-tensor hooks (checkpoints, copies in host memory) may hand back others.
 def _saved_rows(z, cols, what):
-    """The logits as the forward pass saved them, and the elements from row to row."""
+    """The logits the forward pass saved, the elements from row to row, and the (dense) tensor for their gradient."""
     if z.is_contiguous():
-        return z, cols
+        return z, cols, torch.empty_like(z)
+    dense = torch.empty(z.shape, dtype=z.dtype, device=z.device)
     z, _, _, stride = _class_rows(z, what)
-    return z, stride
-
-
-def _gradient_like(z, shape):
-    """The tensor a gradient is written into: the logits' shape, dense."""
-    if z.is_contiguous():
-        return torch.empty_like(z)
-    return torch.empty(shape, dtype=z.dtype, device=z.device)
+    return z, stride, dense
 
 
 def _float_gradient(g):
@@ -291,13 +286,10 @@ def _first_derivative_only(function):
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, live, top, temperature):
-        z, rows, cols, stride = _class_rows(logits, "token_logprobs")
-        logp, entropy, top_logp, top_cls, stats = _logprobs_forward(z, (rows, cols, stride), tokens, live, top,
-                                                                    temperature, True)
+    def forward(ctx, z, geometry, tokens, live, top, temperature):
+        logp, entropy, top_logp, top_cls, stats = _logprobs_forward(z, geometry, tokens, live, top, temperature, True)
         ctx.save_for_backward(z, tokens, top_cls, stats)
-        ctx.last = (rows, cols, dtype_code(z.dtype), temperature, top)
-        ctx.shape, ctx.in_dtype, ctx.device = logits.shape, logits.dtype, z.device.index
+        ctx.last = (geometry[0], geometry[1], dtype_code(z.dtype), temperature, top)
         if top_cls is not None:
             ctx.mark_non_differentiable(top_cls)
         ctx.set_materialize_grads(False)
@@ -307,19 +299,14 @@ class _TokenLogprobs(torch.autograd.Function):
     @_first_derivative_only
     def backward(ctx, dlogp, dentropy, dtop, _):
         if dlogp is None and dentropy is None and dtop is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         z, tokens, top_cls, stats = ctx.saved_tensors
-        z, stride = _saved_rows(z, ctx.last[1], "token_logprobs")
+        z, stride, dz = _saved_rows(z, ctx.last[1], "token_logprobs")
         dlogp, dentropy, dtop = _float_gradient(dlogp), _float_gradient(dentropy), _float_gradient(dtop)
-        dz = _gradient_like(z, ctx.shape)
-        rc = _lib.lib().isg_token_logprobs_bwd(
-            z.data_ptr(), stride, _lib.ptr(tokens), tokens.element_size() if tokens is not None else 4, _lib.ptr(top_cls),
-            stats.data_ptr(), None if dlogp is None else dlogp.data_ptr(), None if dentropy is None else dentropy.data_ptr(),
-            None if dtop is None else dtop.data_ptr(), *ctx.last, dz.data_ptr(),
-            torch._C._cuda_getCurrentRawStream(ctx.device))
-        if rc:
-            _lib.check(rc, "isg_token_logprobs_bwd")
-        return dz if dz.dtype == ctx.in_dtype else dz.to(ctx.in_dtype), None, None, None, None
+        _launch(_lib.lib().isg_token_logprobs_bwd, dz.get_device(), (
+            z.data_ptr(), stride, _address(tokens), tokens.element_size() if tokens is not None else 4, _address(top_cls),
+            stats.data_ptr(), _address(dlogp), _address(dentropy), _address(dtop), *ctx.last, dz.data_ptr()))
+        return dz, None, None, None, None, None
 
 
 def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
@@ -345,12 +332,11 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
         tokens = _row_argument(tokens, lead, _ROW_CLASSES, logits.device, "token_logprobs: tokens")
     if live is not None:
         live = _row_argument(live, lead, _ROW_MASKS, logits.device, "token_logprobs: live")
-    if torch.is_grad_enabled() and logits.requires_grad:
-        logp, entropy, top_logp, top_cls = _TokenLogprobs.apply(logits, tokens, live, top, temperature)
+    z, *geometry = _class_rows(logits, "token_logprobs")
+    if z.requires_grad and torch.is_grad_enabled():
+        logp, entropy, top_logp, top_cls = _TokenLogprobs.apply(z, geometry, tokens, live, top, temperature)
     else:
-        z, rows, cols, stride = _class_rows(logits.detach(), "token_logprobs")
-        logp, entropy, top_logp, top_cls, _ = _logprobs_forward(z, (rows, cols, stride), tokens, live, top, temperature,
-                                                                False)
+        logp, entropy, top_logp, top_cls, _ = _logprobs_forward(z, geometry, tokens, live, top, temperature, False)
     if len(lead) != 1:
         logp = logp.reshape(lead) if logp is not None else None
         entropy = entropy.reshape(lead)
@@ -362,44 +348,36 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
 # ---- distillation -----------------------------------------------------------------------------------------------------
 def _distill_forward(z, geometry, values, classes, live, temperature, tail, keep):
     rows, cols, stride = geometry
-    lib, dev = _lib.lib(), z.device
-    loss = torch.empty([rows], dtype=torch.float32, device=dev)
-    stats = torch.empty([rows, 8], dtype=torch.float32, device=dev) if keep else None
+    lib, dev, f32 = _lib.lib(), z.device, torch.float32
+    loss = torch.empty([rows], dtype=f32, device=dev)
+    stats = torch.empty([rows, 8], dtype=f32, device=dev) if keep else None
     space = None
     if cols > _ONE_UNIT_CLASSES:
         space = torch.empty([lib.isg_distill_workspace_bytes(rows, cols)], dtype=torch.uint8, device=dev)
-    with _on_device(z):
-        rc = lib.isg_distill_fwd(z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(), classes.element_size(),
-                                 _lib.ptr(live), rows, cols, values.shape[-1], dtype_code(z.dtype), temperature, tail,
-                                 loss.data_ptr(), _lib.ptr(stats), _lib.ptr(space), _lib.stream_of(z))
-    if rc:
-        _lib.check(rc, "isg_distill_fwd")
+    _launch(lib.isg_distill_fwd, dev.index, (
+        z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(), classes.element_size(), _address(live), rows, cols,
+        values.shape[-1], dtype_code(z.dtype), temperature, tail, loss.data_ptr(), _address(stats), _address(space)))
     return loss, stats
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, values, classes, live, temperature, tail):
-        z, rows, cols, stride = _class_rows(logits, "distill_rows")
-        loss, stats = _distill_forward(z, (rows, cols, stride), values, classes, live, temperature, tail, True)
+    def forward(ctx, z, geometry, values, classes, live, temperature, tail):
+        loss, stats = _distill_forward(z, geometry, values, classes, live, temperature, tail, True)
         ctx.save_for_backward(z, values, classes, stats)
-        ctx.last = (rows, cols, values.shape[-1], dtype_code(z.dtype), temperature, tail)
-        ctx.shape, ctx.in_dtype, ctx.device = logits.shape, logits.dtype, z.device.index
+        ctx.last = (geometry[0], geometry[1], values.shape[-1], dtype_code(z.dtype), temperature, tail)
         return loss
 
     @staticmethod
     @_first_derivative_only
     def backward(ctx, dloss):
         z, values, classes, stats = ctx.saved_tensors
-        z, stride = _saved_rows(z, ctx.last[1], "distill_rows")
-        g = _float_gradient(dloss)
-        dz = _gradient_like(z, ctx.shape)
-        rc = _lib.lib().isg_distill_bwd(z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(),
-                                        classes.element_size(), stats.data_ptr(), g.data_ptr(), *ctx.last, dz.data_ptr(),
-                                        torch._C._cuda_getCurrentRawStream(ctx.device))
-        if rc:
-            _lib.check(rc, "isg_distill_bwd")
-        return dz if dz.dtype == ctx.in_dtype else dz.to(ctx.in_dtype), None, None, None, None, None
+        z, stride, dz = _saved_rows(z, ctx.last[1], "distill_rows")
+        dloss = _float_gradient(dloss)
+        _launch(_lib.lib().isg_distill_bwd, dz.get_device(), (
+            z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(), classes.element_size(), stats.data_ptr(),
+            dloss.data_ptr(), *ctx.last, dz.data_ptr()))
+        return dz, None, None, None, None, None, None
 
 
 def distill_rows(logits, teacher_values, teacher_classes, temperature=1.0, tail=False, live=None):
@@ -433,11 +411,11 @@ def distill_rows(logits, teacher_values, teacher_classes, temperature=1.0, tail=
     classes = _row_argument(teacher_classes, shape, _ROW_CLASSES, logits.device, "distill_rows: teacher_classes")
     if live is not None:
         live = _row_argument(live, lead, _ROW_MASKS, logits.device, "distill_rows: live")
-    if torch.is_grad_enabled() and logits.requires_grad:
-        loss = _Distill.apply(logits, values, classes, live, temperature, int(bool(tail)))
+    z, *geometry = _class_rows(logits, "distill_rows")
+    if z.requires_grad and torch.is_grad_enabled():
+        loss = _Distill.apply(z, geometry, values, classes, live, temperature, int(bool(tail)))
     else:
-        z, rows, cols, stride = _class_rows(logits.detach(), "distill_rows")
-        loss, _ = _distill_forward(z, (rows, cols, stride), values, classes, live, temperature, int(bool(tail)), False)
+        loss, _ = _distill_forward(z, geometry, values, classes, live, temperature, int(bool(tail)), False)
     return loss if len(lead) == 1 else loss.reshape(lead)
 
 
