@@ -780,6 +780,7 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
     if (rows == 0) return ISG_OK;
     ISG_REQUIRE(logits && stats && dlogits && (!dlogprobs || tokens) && (!dtop_logprobs || (top > 0 && top_classes)),
                 ISG_EINVAL, "%s: null pointer", who);
+    ISG_REQUIRE((uintptr_t)stats % 16 == 0, ISG_EINVAL, "%s: stats must be aligned to 16 bytes", who);
     ISG_REQUIRE(dlogits != logits, ISG_EINVAL, "%s: dlogits must not alias the logits", who);
     const Cut cut = cut_backward(rows, cols, dtype, 0);
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -86,7 +86,8 @@ def token_logprobs_grad(z, T, tokens, top_classes, g_logp, g_ent, g_top, dtype):
     sum_g = np.abs(g) if g_top is None else np.abs(g_top).sum(axis=1) + (0 if g_logp is None else np.abs(g_logp))
     inner = sum_g[:, None] + np.abs(gh)[:, None] * (np.abs(lp) + H[:, None])
     err_h = token_logprobs(z, T)["entropy_tol"][:, None] + k
-    bound = (p * (inner * (k + 8 * U) + np.abs(gh)[:, None] * err_h) + 4 * U * np.abs(own)) / T
+    # (an exponential below the smallest normal float comes out as 0: 2^-126 of p, times what p is multiplied by)
+    bound = (p * (inner * (k + 8 * U) + np.abs(gh)[:, None] * err_h) + 2.0 ** -126 * inner + 4 * U * np.abs(own)) / T
     dz[empty], bound[empty] = 0.0, 0.0
     return dz, bound + HALF_STEP[dtype] * np.abs(dz) + 1e-37
 

@@ -97,6 +97,7 @@ def test_entry_points_refuse_what_is_their_own():
     assert _fwd(cols=50177, stride=50177) == -1 and b"workspace" in err()
     assert _dfwd(cols=50177, stride=50177) == -1 and b"workspace" in err()
     assert _fwd(stats=ctypes.c_void_p(4100)) == -1 and b"aligned" in err()
+    assert _bwd(stats=ctypes.c_void_p(4100)) == -1 and b"aligned" in err()
     assert _bwd(top=65) == -1 and _bwd(tokens=None) == -1 and _bwd(stats=None) == -1
     assert _bwd(gt=ONE) == -1 and _bwd(gt=ONE, top=3, tc=None) == -1  # gradients of alternatives there are none of
     assert _bwd(out=ONE) == -1 and b"alias" in err()
