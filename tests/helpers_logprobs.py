@@ -165,7 +165,8 @@ def distill(z, values, classes, T, tail, g=None, dtype="f32"):
             perr = perr + np.where(inside, 0.0, among * (d_rest + rest * (kap + kap_r + 8 * U))[:, None] +
                                    among * rest[:, None] * 4 * U * lr + p * (kap_r[:, None] + 4 * U * lr))
     dz = (p * total[:, None] - target) * (g / T)[:, None]
-    bound = (perr + qerr) * np.abs(g / T)[:, None]
+    # (exponentials below the smallest normal float come out as 0, as in the gradient above)
+    bound = (perr + qerr + 2.0 ** -126 * np.maximum(total, 1)[:, None]) * np.abs(g / T)[:, None]
     dz[empty], bound[empty] = 0.0, 0.0
     dz[bad] = np.nan
     out["dlogits"], out["dlogits_tol"] = dz, bound + (HALF_STEP[dtype] + 4 * U) * np.abs(np.nan_to_num(dz)) + 1e-37
