@@ -361,10 +361,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restr
 }
 
 // What a workgroup has found of a part of a row's best classes so far: the k first are among them, in no order.
+// `count` is the walk's alone: every wave reads it behind a barrier, and until the next barrier nothing but that same value
+// is written to it.  `kept_count` is trim_list's: read between its barriers, set back behind its last one.  (As one counter
+// a wave that ran ahead into trim_list set it back before the others had read it.)
 struct TopList {
     u64 keys[kListMax];
     u64 kept[kListKeep];
-    int count;
+    int count, kept_count;
 };
 
 // The largest 16-bit prefix that at least k of the n keys (n <= kListMax) reach; uniform, every wave for itself.
@@ -390,17 +393,17 @@ __device__ __forceinline__ int trim_list(TopList& list, int count, int k, float&
     const unsigned bound = count <= 4 * 64 ? prefix_of<4>(list.keys, count, k)
                                            : (count <= 8 * 64 ? prefix_of<8>(list.keys, count, k)
                                                               : prefix_of<kListMax / 64>(list.keys, count, k));
-    if (threadIdx.x == 0) list.count = 0;
+    if (threadIdx.x == 0) list.kept_count = 0;
     __syncthreads();
     for (int r = threadIdx.x; r < count; r += kThreads) {
         const u64 own = list.keys[r];
         if ((unsigned)(own >> 48) >= bound) {
-            const int at = atomicAdd(&list.count, 1);
+            const int at = atomicAdd(&list.kept_count, 1);
             if (at < kListKeep) list.kept[at] = own;
         }
     }
     __syncthreads();
-    int n = list.count;
+    int n = list.kept_count;
     if (n > 2 * k) {
         rank_keys<kThreads>(list.keys, count, k, [&](int place, u64 key) { list.kept[place] = key; });
         __syncthreads();
