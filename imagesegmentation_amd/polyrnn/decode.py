@@ -3,6 +3,7 @@ kernels (isg_softmax_xent_fwd / _bwd, isg_argmax_rows, isg_sample_rows, isg_toke
 import typing
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -177,6 +178,12 @@ class TokenLogprobs(typing.NamedTuple):
     top_classes: typing.Optional[torch.Tensor]
 
 
+def _refuse_tangent(t, what):
+    """The kernels read a tensor's values only.  (A dual tensor need not require a gradient, so nothing else would notice.)"""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError("%s: forward-mode derivatives are not implemented" % what)
+
+
 def _class_rows(logits, what):
     """(logits, rows, classes, elements from row to row) as the kernels read them: float32 or bfloat16, a row's classes
     adjacent, rows evenly spaced - in place where the tensor is that (a column slice of padded logits, every other step of a batch), a
@@ -186,6 +193,7 @@ def _class_rows(logits, what):
     cols = logits.shape[-1]
     if not 1 <= cols <= CLASSES_MAX:
         raise ValueError("%s: %d classes (1 to %d)" % (what, cols, CLASSES_MAX))
+    _refuse_tangent(logits, what)
     if not logits.is_cuda:
         raise RuntimeError("%s: logits must live on the GPU: libisg has no CPU path" % what)
     z = logits if logits.dtype in (torch.float32, torch.bfloat16) else logits.float()
@@ -269,8 +277,11 @@ def _saved_rows(z, cols, what):
     return z, stride, dense
 
 
-def _float_gradient(g):
-    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+def _float_gradient(g, what):
+    if g is None:
+        return None
+    _refuse_tangent(g, what)
+    if g.dtype == torch.float32 and g.is_contiguous():
         return g
     return g.to(torch.float32).contiguous()
 
@@ -301,8 +312,9 @@ class _TokenLogprobs(torch.autograd.Function):
         if dlogp is None and dentropy is None and dtop is None:
             return None, None, None, None, None, None
         z, tokens, top_cls, stats = ctx.saved_tensors
-        z, stride, dz = _saved_rows(z, ctx.last[1], "token_logprobs")
-        dlogp, dentropy, dtop = _float_gradient(dlogp), _float_gradient(dentropy), _float_gradient(dtop)
+        what = "token_logprobs"
+        z, stride, dz = _saved_rows(z, ctx.last[1], what)
+        dlogp, dentropy, dtop = _float_gradient(dlogp, what), _float_gradient(dentropy, what), _float_gradient(dtop, what)
         _launch(_lib.lib().isg_token_logprobs_bwd, dz.get_device(), (
             z.data_ptr(), stride, _address(tokens), tokens.element_size() if tokens is not None else 4, _address(top_cls),
             stats.data_ptr(), _address(dlogp), _address(dentropy), _address(dtop), *ctx.last, dz.data_ptr()))
@@ -312,7 +324,7 @@ class _TokenLogprobs(torch.autograd.Function):
 def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
     """Log-probabilities of given classes, entropies and the most probable classes of softmax(logits / temperature),
     from one pass over the logits (isg_token_logprobs_fwd); differentiable in the logits through everything but the
-    classes (isg_token_logprobs_bwd; first derivatives only).
+    classes (isg_token_logprobs_bwd; first derivatives only, in reverse mode).
 
     logits [..., K] (float32 and bfloat16 as they are, also with rows evenly apart; others through float32),
     tokens int32 or int64 [...] or None, top = how many of the largest logits to report (0 to 64, at most K; equal
@@ -373,7 +385,7 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, dloss):
         z, values, classes, stats = ctx.saved_tensors
         z, stride, dz = _saved_rows(z, ctx.last[1], "distill_rows")
-        dloss = _float_gradient(dloss)
+        dloss = _float_gradient(dloss, "distill_rows")
         _launch(_lib.lib().isg_distill_bwd, dz.get_device(), (
             z.data_ptr(), stride, values.data_ptr(), classes.data_ptr(), classes.element_size(), stats.data_ptr(),
             dloss.data_ptr(), *ctx.last, dz.data_ptr()))
@@ -382,8 +394,8 @@ class _Distill(torch.autograd.Function):
 
 def distill_rows(logits, teacher_values, teacher_classes, temperature=1.0, tail=False, live=None):
     """Per-row divergence of softmax(logits / temperature) from a teacher's k most probable classes (isg_distill_fwd /
-    isg_distill_bwd), float32 [...], differentiable in the logits (first derivatives only): sum_j q_j (log q_j -
-    log p_j).  The teacher takes no gradient.
+    isg_distill_bwd), float32 [...], differentiable in the logits (first derivatives only, in reverse mode):
+    sum_j q_j (log q_j - log p_j).  The teacher takes no gradient and no tangent.
 
     logits [..., K] as ``token_logprobs`` takes them; teacher_values float [..., k] and teacher_classes int32 or int64
     [..., k], k from 1 to 1024: what ``token_logprobs(teacher_logits, top=k, temperature=temperature)`` returns.  A

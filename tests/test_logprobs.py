@@ -152,3 +152,25 @@ def test_python_calls_refuse_what_they_cannot_take():
         decode.distill_rows(z, v, v)
     with pytest.raises(ValueError):
         decode.distill_rows(z, v, c, live=torch.ones([3], dtype=torch.bool))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not require a gradient; without the refusal its tangent would be gone from the results."""
+    from torch.autograd import forward_ad
+    z, v, c = torch.randn([4, 10]), torch.zeros([4, 3]), torch.zeros([4, 3], dtype=torch.int64)
+    calls = [lambda y: decode.token_logprobs(y, c[:, 0], top=2).logprobs, lambda y: decode.distill_rows(y, v, c),
+             lambda y: decode.distill_mean(y, v, c)]
+    for call in calls:
+        with forward_ad.dual_level():
+            for dual in (forward_ad.make_dual(z, torch.ones_like(z)),
+                         forward_ad.make_dual(z.clone().requires_grad_(True), torch.ones_like(z)),
+                         forward_ad.make_dual(z.half(), torch.ones_like(z.half()))):
+                for y in (dual, dual[::2].repeat(2, 1)):
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(y)
+                    with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(y)
+            with pytest.raises(RuntimeError, match="no CPU path"):  # (a plain tensor while a level is open)
+                call(z)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (z,), (torch.ones_like(z),))

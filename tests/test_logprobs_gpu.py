@@ -796,3 +796,19 @@ def test_tens_of_millions_of_rows():
         want = p * (1 - (logp + entropy[:, None]))
         want.scatter_add_(1, tokens[:, None], torch.full([rows, 1], -1.0, dtype=torch.float64, device=DEV))
         assert ((dz - want).abs() <= 4 * tol[:, None]).all()
+
+
+def test_a_tangent_on_an_incoming_gradient_is_refused():
+    """It arrives at the backward pass alone where the logits have none; the results' gradient would be without it."""
+    from torch.autograd import forward_ad
+    decode = _decode()
+    z = torch.randn([6, 50], device=DEV, requires_grad=True)
+    tokens, classes = torch.arange(6, device=DEV), torch.randint(50, [6, 3], device=DEV)
+    one = torch.ones([6], device=DEV)
+    for call in (lambda: decode.token_logprobs(z, tokens).logprobs, lambda: decode.token_logprobs(z, tokens).entropy,
+                 lambda: decode.distill_rows(z, torch.zeros([6, 3], device=DEV), classes)):
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(call(), z, forward_ad.make_dual(one, one))
+            plain, = torch.autograd.grad(call(), z, one)
+        assert torch.equal(plain, torch.autograd.grad(call(), z, one)[0])
