@@ -168,6 +168,7 @@ def sample_actions(logits, seed, grid_side, row_offset=0, row_offset_dev=None, o
 TOP_MAX = 64             # ISG_TOP_MAX
 DISTILL_MAX = 1024       # ISG_DISTILL_MAX
 CLASSES_MAX = 1 << 20    # ISG_CLASSES_MAX
+ROWS_MAX = (1 << 31) - 1  # the entry points' int
 
 
 class TokenLogprobs(typing.NamedTuple):
@@ -193,11 +194,13 @@ def _class_rows(logits, what):
     cols = logits.shape[-1]
     if not 1 <= cols <= CLASSES_MAX:
         raise ValueError("%s: %d classes (1 to %d)" % (what, cols, CLASSES_MAX))
+    rows = logits.numel() // cols
+    if rows > ROWS_MAX:  # (an int argument would keep its lower 32 bits without a word)
+        raise ValueError("%s: %d rows (at most %d)" % (what, rows, ROWS_MAX))
     _refuse_tangent(logits, what)
     if not logits.is_cuda:
         raise RuntimeError("%s: logits must live on the GPU: libisg has no CPU path" % what)
     z = logits if logits.dtype in (torch.float32, torch.bfloat16) else logits.float()
-    rows = z.numel() // cols
     if z.is_contiguous():
         return z, rows, cols, cols
     stride = pixel_stride(z) if z.dim() > 1 else None
@@ -326,10 +329,10 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
     from one pass over the logits (isg_token_logprobs_fwd); differentiable in the logits through everything but the
     classes (isg_token_logprobs_bwd; first derivatives only, in reverse mode).
 
-    logits [..., K] (float32 and bfloat16 as they are, also with rows evenly apart; others through float32),
-    tokens int32 or int64 [...] or None, top = how many of the largest logits to report (0 to 64, at most K; equal
-    logits lowest class first), live bool or uint8 [...] or None: rows without it are not read and give zeros (class
-    -1) and no gradient - steps past a sequence's duration.  Logits of -inf are classes without probability.
+    logits [..., K] (float32 and bfloat16 as they are, also with rows evenly apart; others through float32; fewer than
+    2^31 rows), tokens int32 or int64 [...] or None, top = how many of the largest logits to report (0 to 64, at most
+    K; equal logits lowest class first), live bool or uint8 [...] or None: rows without it are not read and give zeros
+    (class -1) and no gradient - steps past a sequence's duration.  Logits of -inf are classes without probability.
 
     Returns ``TokenLogprobs``: logprobs float32 [...] (NaN for a class outside [0, K)), entropy float32 [...],
     top_logprobs float32 [..., top], top_classes int32 [..., top]."""

@@ -174,3 +174,19 @@ def test_forward_mode_derivatives_are_refused():
                 call(z)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(call, (z,), (torch.ones_like(z),))
+
+
+@pytest.mark.parametrize("rows", [1 << 31, (1 << 32) + 3])
+def test_more_rows_than_an_int_holds_are_refused(rows):
+    """(1 << 32) + 3 rows would be three rows to the entry points."""
+    z = torch.empty([rows, 2], dtype=torch.bfloat16, device="meta")
+    tokens, values = torch.empty([rows], dtype=torch.int32, device="meta"), torch.empty([rows, 1], device="meta")
+    with pytest.raises(ValueError, match="rows"):
+        decode.token_logprobs(z, tokens, top=1)
+    with pytest.raises(ValueError, match="rows"):
+        decode.token_logprobs(z.reshape(-1, 1, 1, 2))
+    for call in (decode.distill_rows, decode.distill_mean):
+        with pytest.raises(ValueError, match="rows"):
+            call(z, values, tokens[:, None])
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        decode.token_logprobs(z[:(1 << 31) - 1])
