@@ -24,7 +24,9 @@ def sources():
 def _stale():
     if not os.path.exists(OUT):
         return True
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.h")) + [os.path.join(_HERE, "..", "include", "isg.h")]
+    # (this file as well: it holds the compiler's flags)
+    deps = sources() + glob.glob(os.path.join(CSRC, "*.h")) + [os.path.join(_HERE, "..", "include", "isg.h"),
+                                                               os.path.abspath(__file__)]
     newest = max(os.path.getmtime(p) for p in deps)
     return os.path.getmtime(OUT) < newest
 
