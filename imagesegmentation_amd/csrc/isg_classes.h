@@ -361,9 +361,10 @@ inline Cut cut_wave(int cols, int dtype, int entries, int narrow) {
 // 91; distilled with 16 entries and a tail 61 and 97).  What grows with the best classes or the entries is paid by fewer
 // lanes so: many of those in long rows are a whole wave's again (20 best of 10,240 x 785 bf16 12.7 us, by 16 lanes 14.7, of
 // 66,000 x 1,000 57 and 66; 64 entries of 131,072 x 785 74 and 86, of 66,000 x 380 28 and 24).
+constexpr int kNarrow = 65, kNarrowMany = 40;  // (kNarrowMany: more than 16 entries or best classes)
 inline Cut cut_forward(long long rows, int cols, int dtype, int entries, int best) {
-    int narrow = rows > 8192 && entries <= 64 ? 65 : 0;
-    if (narrow && (entries > 16 || best > 16)) narrow = best > 16 && rows <= 49152 ? 24 : 40;
+    int narrow = rows > 8192 && entries <= 64 ? kNarrow : 0;
+    if (narrow && (entries > 16 || best > 16)) narrow = best > 16 && rows <= 49152 ? 24 : kNarrowMany;
     const Cut wave = cut_wave(cols, dtype, entries, narrow);
     if (wave.lanes) return wave;
     long long splits = (units_of(dtype) + rows - 1) / (rows > 0 ? rows : 1);
@@ -376,9 +377,9 @@ inline Cut cut_forward(long long rows, int cols, int dtype, int entries, int bes
 // The backward passes have less to pay once a row, and longer runs of memory by a whole wave: 131,072 x 785 bf16 84 us, by
 // 16 lanes 88; float 138 and 150; 64 entries bf16 100 and 142; 66,000 x 380 bf16 22.9 and 22.4, float 32.6 and 33.8; x 120
 // 20 and 9.5; x 250 with 64 entries 29 and 33.
-constexpr int kNarrowBackward = 32;
+constexpr int narrow_backward(int dtype, bool many) { return many ? 8 : (dtype == ISG_F32 ? 24 : 32); }
 inline Cut cut_backward(long long rows, int cols, int dtype, int entries) {
-    const int narrow = rows <= 8192 || entries > 64 ? 0 : (entries > 16 ? 8 : (dtype == ISG_F32 ? 24 : kNarrowBackward));
+    const int narrow = rows <= 8192 || entries > 64 ? 0 : narrow_backward(dtype, entries > 16);
     const Cut wave = cut_wave(cols, dtype, entries, narrow);
     if (wave.lanes) return wave;
     const auto parts = [&](int ne) { return (cols + kThreads * ne - 8 - 1) / (kThreads * ne - 8); };
@@ -405,7 +406,7 @@ inline dim3 grid_of(long long units, int threads) {
     return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
 
-// F::template run<G, NE>(...) for a wave's cut, up to NARROW classes a lane by 16 lanes
+// F::template run<G, NE>(...) for a wave's cut, up to NARROW classes a lane by 16 lanes (beyond 64: also by 32 lanes)
 template <typename F, int NARROW, typename... A>
 void with_wave(const Cut& cut, A&&... args) {
     if constexpr (NARROW > 64)
@@ -429,20 +430,24 @@ void with_wave(const Cut& cut, A&&... args) {
         case 1: F::template run<16, 1>(args...); break;
         case 4: F::template run<16, 4>(args...); break;
         case 8: F::template run<16, 8>(args...); break;
+    }
+    if constexpr (NARROW >= 24) switch (cut.ne) {
         case 16: F::template run<16, 16>(args...); break;
         case 24: F::template run<16, 24>(args...); break;
-        case 32: F::template run<16, 32>(args...); break;
     }
-    if constexpr (NARROW > 32) switch (cut.ne) {
-        case 40: F::template run<16, 40>(args...); break;
+    if constexpr (NARROW >= 32)
+        if (cut.ne == 32) F::template run<16, 32>(args...);
+    if constexpr (NARROW >= 40)
+        if (cut.ne == 40) F::template run<16, 40>(args...);
+    if constexpr (NARROW >= 64) switch (cut.ne) {
         case 48: F::template run<16, 48>(args...); break;
         case 56: F::template run<16, 56>(args...); break;
         case 64: F::template run<16, 64>(args...); break;
     }
 }
-template <typename F, typename... A>
+template <typename F, int NARROW, typename... A>
 void launch_backward(const Cut& cut, A&&... args) {
-    if (cut.lanes != kThreads) with_wave<F, kNarrowBackward>(cut, args...);
+    if (cut.lanes != kThreads) with_wave<F, NARROW>(cut, args...);
     else if (cut.ne == 8) F::template run<kThreads, 8>(args...);
     else if (cut.ne == 16) F::template run<kThreads, 16>(args...);
     else F::template run<kThreads, 32>(args...);

@@ -64,6 +64,7 @@ __device__ __forceinline__ void distill_dead(const DistillArgs& a, long long row
 // A row's entries in the registers of its G threads: entry i * G + thread in place i < N.  (One place where
 // that holds a row's k, else four; sixteen, for every k there can be, where a wave closes a row of any length and for rows
 // too short for a workgroup.)
+constexpr int places(int lanes, int ne, int n) { return lanes == 64 && ne == 1 ? 16 : n; }
 template <int G, int N>
 struct Entries {
     int cls[N];    // -1: none, cols: a class the row does not have
@@ -228,7 +229,7 @@ __device__ __forceinline__ void mark_entries(const DistillArgs& a, const Entries
 // each), taken out of the registers and summed apart.  131,072 x 785 bf16 with 16 entries and a tail 52 to 61 us (3.4 TB/s;
 // sums, marks and the closing logarithms weigh as much as the read), with 64 entries without 68 to 74; float, 64 and a
 // tail, 97 to 113 (3.6 TB/s); 20,480 rows bf16 13.4.  (More where a gradient before it has left the cache dirty.)
-template <typename T, int G, int NE, int PLACES, bool TAIL>
+template <typename T, int G, int NE, int N, bool TAIL>
 __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restrict__ logits, DistillArgs a) {
     __shared__ u64 marks[TAIL ? kThreads : 1];  // a thread's elements that an entry names, one bit each
     const int lane = threadIdx.x & (G - 1);
@@ -241,7 +242,6 @@ __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restri
     const T* z = logits + row * a.row_stride;
     using S = Span<T, G, NE>;
     const S span(z, 0, a.cols, lane);
-    constexpr int N = G == 64 && NE == 1 ? 16 : PLACES;
     Entries<G, N> en;
     en.load(a.values, a.classes, a.class_bytes, row, a.k, a.cols);
     float v[NE], ze[N];
@@ -411,7 +411,7 @@ struct DistillBwdArgs {
 // A row, or a part of one, by G lanes: the dense part from the row's kept constants, the entries' own values over it.  Reads
 // the logits and writes as much: 2,048 x 131,071 bf16 191 us (5.6 TB/s read and written), 8,192 x 12,545 float 154 us
 // (5.3), 131,072 x 785 bf16 with 16 entries 81 to 100 us (4.6), float with 64 153 us (5.4).
-template <typename T, int G, int NE, int PLACES>
+template <typename T, int G, int NE, int N>
 __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restrict__ logits, DistillBwdArgs a,
                                                               T* __restrict__ dlogits) {
     __shared__ u64 marks[kThreads];
@@ -430,7 +430,6 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restri
     const DistillStats st = a.stats[row];
     const bool zero = st.is == 0.0f;  // a dead row, or no class has probability
     const T* z = logits + row * a.row_stride;
-    constexpr int N = G == 64 && NE == 1 ? 16 : PLACES;
     const float g = a.dloss[row] * a.inv_t, gc = g * st.coef * st.ib;
     const bool plain = zero || st.coef != st.coef;  // (NaN: an entry the row does not have; the whole row is)
     Entries<G, N> en;
@@ -546,7 +545,7 @@ template <typename T, bool TAIL, int PLACES>
 struct DistillFwd {
     template <int G, int NE>
     static void run(const void* logits, const DistillArgs& a, hipStream_t s) {
-        hipLaunchKernelGGL((distill_fwd_kernel<T, G, NE, PLACES, TAIL>), grid_of(a.units, G), dim3(kThreads), 0, s,
+        hipLaunchKernelGGL((distill_fwd_kernel<T, G, NE, places(G, NE, PLACES), TAIL>), grid_of(a.units, G), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a);
     }
 };
@@ -556,22 +555,24 @@ void launch_forward(const Cut& cut, const void* logits, const DistillArgs& a, hi
         hipLaunchKernelGGL((distill_stream_kernel<T, 16, TAIL>), grid_of(a.units, kThreads), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a);
     else if (a.k <= cut.lanes)
-        with_wave<DistillFwd<T, TAIL, 1>, 65>(cut, logits, a, s);
+        with_wave<DistillFwd<T, TAIL, 1>, kNarrow>(cut, logits, a, s);
     else
-        with_wave<DistillFwd<T, TAIL, 4>, 65>(cut, logits, a, s);
+        with_wave<DistillFwd<T, TAIL, 4>, kNarrowMany>(cut, logits, a, s);
 }
 template <typename T, int PLACES>
 struct DistillBwd {
     template <int G, int NE>
     static void run(const void* logits, const DistillBwdArgs& a, void* dlogits, hipStream_t s) {
-        hipLaunchKernelGGL((distill_bwd_kernel<T, G, NE, PLACES>), grid_of(a.units, G), dim3(kThreads), 0, s,
+        hipLaunchKernelGGL((distill_bwd_kernel<T, G, NE, places(G, NE, PLACES)>), grid_of(a.units, G), dim3(kThreads), 0, s,
                            static_cast<const T*>(logits), a, static_cast<T*>(dlogits));
     }
 };
 template <typename T>
 void launch_gradient(const Cut& cut, const void* logits, const DistillBwdArgs& a, void* dlogits, hipStream_t s) {
-    if (a.k <= cut.lanes) launch_backward<DistillBwd<T, 1>>(cut, logits, a, dlogits, s);
-    else launch_backward<DistillBwd<T, 4>>(cut, logits, a, dlogits, s);
+    constexpr int dtype = std::is_same<T, float>::value ? ISG_F32 : ISG_BF16;
+    // (16 lanes hold 16 entries in one place each: more of them are cut_backward's `many`)
+    if (a.k <= cut.lanes) launch_backward<DistillBwd<T, 1>, narrow_backward(dtype, false)>(cut, logits, a, dlogits, s);
+    else launch_backward<DistillBwd<T, 4>, narrow_backward(dtype, true)>(cut, logits, a, dlogits, s);
 }
 
 int check_entries(const char* who, int k, int tail) {

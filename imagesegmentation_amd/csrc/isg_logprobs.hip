@@ -682,7 +682,7 @@ struct LogprobsFwd {
     }
     static void launch(const Cut& cut, const void* logits, const LogprobsArgs& a, hipStream_t s) {
         if (cut.lanes != kThreads)
-            with_wave<LogprobsFwd, 65>(cut, logits, a, s);
+            with_wave<LogprobsFwd, kNarrow>(cut, logits, a, s);
         else
             hipLaunchKernelGGL((logprobs_stream_kernel<T, 16, TOP>), grid_of(a.units, kThreads), dim3(kThreads), 0, s,
                                static_cast<const T*>(logits), a);
@@ -794,7 +794,7 @@ extern "C" int isg_token_logprobs_bwd(const void* logits, long long row_stride, 
     a.token_bytes = token_bytes, a.cols = cols, a.splits = cut.splits, a.per = cut.per, a.top = top;
     a.past = beyond_cache(rows, cols, dtype);
     scale_of(temperature, a.c, a.c_lo, a.inv_t);
-    if (dtype == ISG_F32) launch_backward<LogprobsBwd<float>>(cut, logits, a, dlogits, s);
-    else launch_backward<LogprobsBwd<__hip_bfloat16>>(cut, logits, a, dlogits, s);
+    if (dtype == ISG_F32) launch_backward<LogprobsBwd<float>, narrow_backward(ISG_F32, false)>(cut, logits, a, dlogits, s);
+    else launch_backward<LogprobsBwd<__hip_bfloat16>, narrow_backward(ISG_BF16, false)>(cut, logits, a, dlogits, s);
     return isg::check_launch("logprobs_bwd_kernel");
 }
