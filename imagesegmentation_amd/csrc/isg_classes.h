@@ -3,9 +3,12 @@
 //
 // A row z of n logits at temperature T has, with m = max z and x_c = (z_c - m) log2(e) / T,
 //   log p_c = ln 2 (x_c - log2 s),   s = sum 2^x_c,   H = -sum p_c log p_c = ln 2 (log2 s - (sum 2^x_c x_c) / s);
-// every term of H has one sign, so a confident row loses nothing to cancellation, and z_c - m comes first, so that
-// rows of the type's lowest value are uniform rows and not overflows.  A class at -inf has no probability and adds
-// nothing (its x is kept from meeting 0 * inf by a lower bound far below the smallest float).  All sums are float.
+// both terms of H have one sign, and z_c - m comes first, so that rows of the type's lowest value are uniform rows and not
+// overflows.  A class at -inf has no probability and adds nothing (its x is kept from meeting 0 * inf by a lower bound far
+// below the smallest float).  All sums are float.  s is 1 + e in a row whose other classes have e of the mass together, and
+// is rounded before its logarithm: log p and H are good to some 1e-7 absolutely, not relatively.  Of an e below 6e-8 nothing
+// is left in log p of the row's class (0 for -e), and H = e (1 - log e) lacks its first e, a twentieth or so.  (A sum
+// without the maximum would keep it, at an operation more a class.)
 //
 // Layout.  A row is read once, into registers: up to about 1,000 classes by 16 lanes (four rows a wave: what a row costs
 // once - reductions, logarithms, outputs - is paid for four rows in the same instructions), up to about 2,000 by 32
@@ -361,6 +364,10 @@ inline Cut cut_wave(int cols, int dtype, int entries, int narrow) {
 // 91; distilled with 16 entries and a tail 61 and 97).  What grows with the best classes or the entries is paid by fewer
 // lanes so: many of those in long rows are a whole wave's again (20 best of 10,240 x 785 bf16 12.7 us, by 16 lanes 14.7, of
 // 66,000 x 1,000 57 and 66; 64 entries of 131,072 x 785 74 and 86, of 66,000 x 380 28 and 24).
+// From some 380 to 640 classes it depends on the rows, as 16 lanes first fill the chip's waves at many of them: 20 best of
+// 505 bf16 by a wave and by 16 lanes 15.2 and 16.1 us at 20,480 rows, 32.2 and 31.5 at 49,152, 78 and 69 at 131,072; float
+// 16.8 and 17.8, 33.6 and 34.4, 89 and 83; 64 best bf16 28.5 and 35.2, 60.8 and 65.6, 152 and 147; beyond 512 classes 20 best
+// of bf16 would cross earlier (570: 18.5 and 17.2 at 20,480 rows) and 64 of float later (182 and 197 at 131,072 x 633).
 constexpr int kNarrow = 65, kNarrowMany = 40;  // (kNarrowMany: more than 16 entries or best classes)
 inline Cut cut_forward(long long rows, int cols, int dtype, int entries, int best) {
     int narrow = rows > 8192 && entries <= 64 ? kNarrow : 0;

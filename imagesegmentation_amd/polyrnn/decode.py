@@ -335,7 +335,8 @@ def token_logprobs(logits, tokens=None, top=0, temperature=1.0, live=None):
     (class -1) and no gradient - steps past a sequence's duration.  Logits of -inf are classes without probability.
 
     Returns ``TokenLogprobs``: logprobs float32 [...] (NaN for a class outside [0, K)), entropy float32 [...],
-    top_logprobs float32 [..., top], top_classes int32 [..., top]."""
+    top_logprobs float32 [..., top], top_classes int32 [..., top].  Near 0 they are good to some 1e-7 absolutely: where
+    all other classes together have less than 6e-8, a class's log-probability is 0."""
     if not torch.is_tensor(logits) or logits.dim() < 1:
         raise TypeError("token_logprobs: logits must be a floating-point tensor of at least one axis")
     lead = logits.shape[:-1]

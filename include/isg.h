@@ -380,6 +380,7 @@ int isg_a3c_loss_bwd(const void* logits, const float* vf, const int32_t* actions
  *   top_classes / top_logprobs [r][top]: the classes of the `top` largest logits in falling order, equal logits by
  *     class (lowest first, NaN last), and their log-probabilities
  *   stats float [r][4] (may be NULL; 16-byte aligned): what isg_token_logprobs_bwd reads.
+ * Values near 0 are good to some 1e-7 absolutely (the sum of a row's exponentials is rounded at 1).
  * A logit of -inf is a class without probability; a row of nothing else has log-probability -inf everywhere, entropy 0
  * and a zero gradient.  live uint8 [rows] (may be NULL): rows with 0 are not read, their outputs are 0 (classes -1)
  * and their gradient is 0.  logits `dtype` with rows row_stride >= cols elements apart; tokens are int32 or int64
