@@ -326,14 +326,15 @@ __device__ __forceinline__ long long block_index() { return (long long)blockIdx.
 
 // ---- launches ------------------------------------------------------------------------------------------------------
 // How a row is cut: `lanes` lanes of a wave for what their registers hold.  Beyond, the forward passes walk over parts of
-// a row, as many as give about `units_of` workgroups but of at least kPartCols classes; the backward passes have nothing
+// a row, as many as give about kUnits workgroups but of at least kPartCols classes; the backward passes have nothing
 // to join and take workgroups of at most 32 classes a thread.  Parts are equal but for the rounding to 8 classes; there is
 // room for those that start between two boundaries (Span).
 //
-// bf16: 2,048 workgroups are on the chip all at once, eight to a CU (64 registers a thread); 2,048 x 131,071 with 64
-// alternatives 139 us so, in 4,096 workgroups (two parts a row) 155 and 9 more to join them.  Float kernels need more
-// registers, five to seven to a CU: 2,048 x 65,537 with 20 alternatives 120 us in 2,048, 105 + 6 in 4,096.
-inline long long units_of(int dtype) { return dtype == ISG_F32 ? 4096 : 2048; }
+// About 2,048 workgroups are on the chip at once, eight to a CU for bf16 (64 registers a thread), five to seven for float.
+// Twice as many (more parts a row) measured the same without alternatives beyond 100,000 classes (2,048 x 131,071 bf16 98
+// and 101 us, float 182 and 180), and slower where a part costs something of its own: 2,048 x 9,001 float 15 and 19, with 20
+// alternatives 25 and 32; 2,048 x 50,177 float with 20 82 and 88; 2,048 x 131,071 bf16 with 64 128 and 148.
+constexpr long long kUnits = 2048;
 constexpr int kPartCols = 2048;
 constexpr int kMaxSplits = 128;
 constexpr int kMarkCols = 131072;  // classes a part may have (one mark each in LDS, 16 KB)
@@ -374,7 +375,7 @@ inline Cut cut_forward(long long rows, int cols, int dtype, int entries, int bes
     if (narrow && (entries > 16 || best > 16)) narrow = best > 16 && rows <= 49152 ? 24 : kNarrowMany;
     const Cut wave = cut_wave(cols, dtype, entries, narrow);
     if (wave.lanes) return wave;
-    long long splits = (units_of(dtype) + rows - 1) / (rows > 0 ? rows : 1);
+    long long splits = (kUnits + rows - 1) / (rows > 0 ? rows : 1);
     const int most = cols / kPartCols < kMaxSplits ? cols / kPartCols : kMaxSplits, least = (cols + kMarkCols - 1) / kMarkCols;
     splits = splits > most ? most : splits;
     splits = splits < least ? least : splits;

@@ -585,7 +585,7 @@ int check_entries(const char* who, int k, int tail) {
 
 extern "C" long long isg_distill_workspace_bytes(int rows, int cols) {
     if (rows < 0 || cols < 1 || cols > kMaxCols) return -1;
-    const Cut cut = cut_forward(rows, cols, ISG_F32, 0, 0);  // (bf16 rows are in as many parts or fewer)
+    const Cut cut = cut_forward(rows, cols, ISG_F32, 0, 0);  // (rows of both types are in as many parts)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * (long long)sizeof(DistillPart);
 }
 

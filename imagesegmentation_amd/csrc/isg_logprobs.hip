@@ -721,7 +721,7 @@ int check_top(const char* who, int top, int cols) {
 
 extern "C" long long isg_token_logprobs_workspace_bytes(int rows, int cols, int top) {
     if (rows < 0 || cols < 1 || cols > kMaxCols || top < 0 || top > kMaxTop) return -1;
-    const Cut cut = cut_forward(rows, cols, ISG_F32, 0, top);  // (bf16 rows are in as many parts or fewer)
+    const Cut cut = cut_forward(rows, cols, ISG_F32, 0, top);  // (rows of both types are in as many parts)
     return cut.splits == 1 ? 0 : (long long)rows * cut.splits * ((long long)sizeof(Sums) + 8 * top) + 8;
 }
 
