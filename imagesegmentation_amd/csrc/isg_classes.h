@@ -399,10 +399,11 @@ inline Cut cut_backward(long long rows, int cols, int dtype, int entries) {
 }
 
 // Whether a gradient is more than the last-level cache holds (256 MB).  What reads it next does not find it there either,
-// and left in the cache it has to be written back under the next kernel's reads: 2,048 x 131,071 bf16 distilled (two parts
-// a row), forward and backward 118 + 185 us, written past the cache 95 + 191; 8,192 x 12,545 float 105 + 140 and 77 + 157;
-// log-probabilities of 131,072 x 785 float 100 + 136 and 74 + 148.  (Not by 16 lanes, whose vectors are 256 bytes of a row:
-// 103 + 150 and 73 + 190; and not of short rows distilled, whose forward pass waits for less: nothing gained.)
+// and left in the cache it has to be written back under the next kernel's reads.  Both ways in one run each: 2,048 x 131,071
+// bf16 distilled (two parts a row then), forward and backward 118 + 185 us, written past the cache 95 + 191; 8,192 x 12,545
+// float 105 + 140 and 77 + 157; log-probabilities of 131,072 x 785 float 100 + 136 and 74 + 148.  (Not by 16 lanes, whose
+// vectors are 256 bytes of a row: 103 + 150 and 73 + 190; and not of short rows distilled, whose forward pass waits for less:
+// nothing gained.)
 inline bool beyond_cache(long long rows, int cols, int dtype) {
     return rows * cols * (dtype == ISG_F32 ? 4 : 2) > (256ll << 20);
 }

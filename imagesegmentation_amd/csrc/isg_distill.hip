@@ -226,9 +226,9 @@ __device__ __forceinline__ void mark_entries(const DistillArgs& a, const Entries
 }
 
 // A row in the registers of G lanes, its entries beside them; with a tail the entries' classes are marked in LDS (a bit
-// each), taken out of the registers and summed apart.  131,072 x 785 bf16 with 16 entries and a tail 52 to 61 us (3.4 TB/s;
-// sums, marks and the closing logarithms weigh as much as the read), with 64 entries without 68 to 74; float, 64 and a
-// tail, 97 to 113 (3.6 TB/s); 20,480 rows bf16 13.4.  (More where a gradient before it has left the cache dirty.)
+// each), taken out of the registers and summed apart.  131,072 x 785 bf16 with 16 entries and a tail 59 us (3.5 TB/s;
+// sums, marks and the closing logarithms weigh as much as the read), with 64 entries without 76; float, 64 and a tail,
+// 113 (3.6 TB/s); 20,480 rows bf16 13.5.  (Behind backward passes, whose gradients have left the cache dirty.)
 template <typename T, int G, int NE, int N, bool TAIL>
 __global__ __launch_bounds__(kThreads) void distill_fwd_kernel(const T* __restrict__ logits, DistillArgs a) {
     __shared__ u64 marks[TAIL ? kThreads : 1];  // a thread's elements that an entry names, one bit each
@@ -285,9 +285,9 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, const T* z, lon
 
 // A part of a longer row: a workgroup walks over it, kThreads * NE classes at a time, the next ones being loaded
 // meanwhile.  Every wave keeps its own maximum and its lanes their own sums until the end.  The marks are one bit a class
-// of the part.  Bound by the read: 2,048 x 131,071 bf16 with 64 entries 105 us (5.1 TB/s), 8,192 x 12,545 float with 32
+// of the part.  Bound by the read: 2,048 x 131,071 bf16 with 64 entries 104 us (5.2 TB/s), 8,192 x 12,545 float with 32
 // 76 us (5.4 TB/s); with a tail the marks add to it, 1,500 x 65,537 float with 64 72 us (5.4), 1,002 x 100,003 bf16 with
-// 256 43 us (4.6).
+// 256 44 us (4.6).
 template <typename T, int NE, bool TAIL>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 7 : 8) void distill_stream_kernel(const T* __restrict__ logits,
                                                                                            DistillArgs a) {
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 7 : 8) void distill_stre
         a.part[unit] = t;
 }
 
-// Joins the parts of a row: one wave.  Latency: 5.7 us for 640 rows in 4 parts, 10 for 1,002 rows of 256 entries.
+// Joins the parts of a row: one wave.  Latency: 5.4 us for 640 rows in 4 parts, 10 for 1,002 rows of 256 entries.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void distill_join_kernel(const T* __restrict__ logits, DistillArgs a) {
     const int lane = threadIdx.x & 63;
@@ -409,8 +409,8 @@ struct DistillBwdArgs {
 };
 
 // A row, or a part of one, by G lanes: the dense part from the row's kept constants, the entries' own values over it.  Reads
-// the logits and writes as much: 2,048 x 131,071 bf16 191 us (5.6 TB/s read and written), 8,192 x 12,545 float 154 us
-// (5.3), 131,072 x 785 bf16 with 16 entries 81 to 100 us (4.6), float with 64 153 us (5.4).
+// the logits and writes as much: 2,048 x 131,071 bf16 190 us (5.6 TB/s read and written), 8,192 x 12,545 float 155 us
+// (5.3), 131,072 x 785 bf16 with 16 entries 101 us (4.1), float with 64 152 us (5.4).
 template <typename T, int G, int NE, int N>
 __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const T* __restrict__ logits, DistillBwdArgs a,
                                                               T* __restrict__ dlogits) {

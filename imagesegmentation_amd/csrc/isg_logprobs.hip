@@ -323,8 +323,8 @@ __device__ __forceinline__ void row_alternative(const LogprobsArgs& a, long long
 
 // A row in the registers of G lanes: maximum first, then the sums of 2^x and 2^x x over the same registers, then the
 // alternatives out of them.  One read of the logits bounds it without alternatives, the search for them with: 131,072 x
-// 785 bf16 46 us (4.5 TB/s; 38 us where nothing has left the last-level cache dirty), with 5 alternatives 70, 20 104, 64
-// 195; float 74 (5.6 TB/s), with 20 112; 20,480 rows bf16 9.6, 10,240 x 784 float with 20 12.9.
+// 785 bf16 46 us (4.5 TB/s; 38 us where nothing has left the last-level cache dirty), with 5 alternatives 69, 20 105, 64
+// 193; float 73 (5.7 TB/s), with 20 110; 20,480 rows bf16 9.6, behind a backward pass 11.5; 10,240 x 784 float with 20 13.1.
 template <typename T, int G, int NE, bool TOP>
 __global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(const T* __restrict__ logits, LogprobsArgs a) {
     typedef typename std::conditional<sizeof(T) == 2, ShortKey, LongKey>::type Keys;
@@ -421,9 +421,10 @@ __device__ __forceinline__ int trim_list(TopList& list, int count, int k, float&
 // the list's own bound, which rises whenever the list has grown to its limit and is cut back.  Steps that would overrun
 // the list (rising rows, ties) or have no finite bound hand it their k first by select_workgroup instead.
 //
-// 2,048 x 131,071 bf16 with 64 alternatives: 133 us, 4.0 TB/s, the vector units busy for four fifths of it (some 8
-// instructions a class for the sums, one of them an exponential that takes four times an addition; 9 for the
-// alternatives); without alternatives 104 us, 5.2 TB/s.  2,048 x 65,537 float with 20: 104 us, 5.2 TB/s.
+// 2,048 x 131,071 bf16 with 64 alternatives: 125 us a call where calls follow each other, 4.3 TB/s (single launches 128 to
+// 148), the vector units busy for four fifths of it (some 8 instructions a class for the sums, one of them an exponential
+// that takes four times an addition; 9 for the alternatives); without alternatives 103 us, 5.2 TB/s.  2,048 x 65,537 float
+// with 20: 103 us, 5.2 TB/s.
 template <typename T, int NE, bool TOP>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 5 : 8) void logprobs_stream_kernel(const T* __restrict__ logits,
                                                                                             LogprobsArgs a) {
@@ -600,8 +601,8 @@ struct LogprobsBwdArgs {
 // A row, or a part of one, by G lanes:
 //   dz_c = 1/T [ g_a [c = a] + sum_j g_j [c = i_j] - p_c (g_a + sum_j g_j + g_H (log p_c + H)) ],
 // the dense part first, from the row's kept m, s and H, then the few classes with a gradient of their own over it.  Reads
-// the logits, writes as much, and is bound by that: 131,072 x 785 bf16 84 us (4.9 TB/s read and written), float 148 us (5.6),
-// 2,050 x 131,071 bf16 193 us (5.6), 2,048 x 65,537 float 195 us (5.5).
+// the logits, writes as much, and is bound by that: 131,072 x 785 bf16 84 us (4.9 TB/s read and written), float 145 us (5.7),
+// 2,050 x 131,071 bf16 188 us (5.7), 2,048 x 65,537 float 196 us (5.5).
 template <typename T, int G, int NE>
 __global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(const T* __restrict__ logits, LogprobsBwdArgs a,
                                                                T* __restrict__ dlogits) {
