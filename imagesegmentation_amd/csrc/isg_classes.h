@@ -333,7 +333,8 @@ __device__ __forceinline__ long long block_index() { return (long long)blockIdx.
 // About 2,048 workgroups are on the chip at once, eight to a CU for bf16 (64 registers a thread), five to seven for float.
 // Twice as many (more parts a row) measured the same without alternatives beyond 100,000 classes (2,048 x 131,071 bf16 98
 // and 101 us, float 182 and 180), and slower where a part costs something of its own: 2,048 x 9,001 float 15 and 19, with 20
-// alternatives 25 and 32; 2,048 x 50,177 float with 20 82 and 88; 2,048 x 131,071 bf16 with 64 128 and 148.
+// alternatives 25 and 32; 2,048 x 50,177 float with 20 82 and 88; 2,048 x 131,071 bf16 with 64 128 and 148.  (They gain
+// where 2,048 leave an uneven rest: 1,300 x 131,071 float with 20 131 for 137, 1,500 x 9,001 without 14.5 for 16.)
 constexpr long long kUnits = 2048;
 constexpr int kPartCols = 2048;
 constexpr int kMaxSplits = 128;
